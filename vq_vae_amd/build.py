@@ -25,7 +25,9 @@ HEADERS = [os.path.join(CSRC, "vq_common.h"), os.path.join(os.path.dirname(PKG),
 # -ffp-contract=off: the kernels spell out every fused multiply-add they want; nothing else may fuse,
 # or the distances would stop matching the documented rounding.
 FLAGS = ["-O3", "--offload-arch=gfx950", "-ffp-contract=off", "-fPIC", "-std=c++17", "-Wall",
-         "-Wno-unused-function", "-fno-gpu-rdc"]
+         "-Wno-unused-function", "-fno-gpu-rdc",
+         # packed fp32 instructions off: some of their forms have given wrong results on this hardware
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 STAMP = LIB + ".sha256"
