@@ -324,6 +324,61 @@ int vq_conv1x1_wgrad(const float* gy, const float* x, int layout, int64_t N, int
                      float* dW, float* db, void* work, void* stream);
 
 /*
+ * Product with bias, activation and residual in its epilogue, and its backward pass: the projections either
+ * side of the quantizer (quant_conv / post_quant_conv as rows, vqvae/custom_vqgan.py:50-51) in training
+ * precision, and the hidden layers of a model over the codes.  Element type of every tensor of a call: dtype
+ * (VQ_F32 / VQ_BF16 / VQ_F16); sums are fp32, each output is rounded once.  x [M][K] with rows ldx elements
+ * apart, W [N][K] (ldw), residual [M][N] (ldr; NULL: none), bias [N] (NULL: none); y, pre, dp, gx [M][.] and gW
+ * are dense.  Any K, N from 1 to 2^20, any M >= 0 (M = 0: y and gx are empty, gW and gbias zero), any element-
+ * aligned pointers.  Limits beyond these: VQ_ERR_UNSUPPORTED (rows more than 8 MiB apart, M > 2^31).
+ *
+ * vq_linear:          p = x W^T + bias;  y = act(p) + residual;  pre (NULL: not wanted) = p in dtype.
+ * vq_linear_act_grad: dp = gy * act'(pre) for `count` elements, act other than VQ_ACT_NONE.  May run in place.
+ * vq_linear_dgrad:    gx = dp W.
+ * vq_linear_wgrad:    gW = dp^T x;  gbias[n] = sum_m dp[m][n].  One of the two may be NULL.
+ * Sums split over workgroups are added in a fixed order: the same bits on every run.
+ * `work`: vq_linear_work_bytes(VQ_LINEAR_*, ...) bytes, 16-byte aligned, contents irrelevant before and after
+ * the call; calls that may overlap need one each.
+ */
+enum { VQ_F32 = 0, VQ_BF16 = 1, VQ_F16 = 2 };
+enum { VQ_ACT_NONE = 0, VQ_ACT_RELU = 1, VQ_ACT_SILU = 2, VQ_ACT_GELU = 3, VQ_ACT_GELU_TANH = 4 };
+enum { VQ_LINEAR_FORWARD = 0, VQ_LINEAR_DGRAD = 1, VQ_LINEAR_WGRAD = 2 };
+int64_t vq_linear_work_bytes(int pass, int64_t M, int K, int N, int dtype);
+int vq_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* residual,
+              int64_t ldr, int dtype, int act, int64_t M, int K, int N, void* y, void* pre, void* work, void* stream);
+int vq_linear_act_grad(const void* gy, const void* pre, int dtype, int act, int64_t count, void* dp, void* stream);
+int vq_linear_dgrad(const void* dp, const void* W, int64_t ldw, int dtype, int64_t M, int K, int N, void* gx, void* work,
+                    void* stream);
+int vq_linear_wgrad(const void* dp, const void* x, int64_t ldx, int dtype, int64_t M, int K, int N, void* gW, void* gbias,
+                    void* work, void* stream);
+
+/*
+ * Global gradient norm over a list of tensors, and clipping by it: what stands between the gradients and the
+ * trainer's optimiser step (vqvae/vqgan_trainer.py:98-104).  `refs` is a host array, read before the call
+ * returns; src and dst are device pointers to numel dense elements of src_type / dst_type (VQ_F32, VQ_BF16,
+ * VQ_F16), at any element-aligned address.  kind: VQ_NORM_*.
+ *
+ * vq_grad_norm:  norm[0] = (sum |g|^p)^(1/p) over all elements of all tensors, summed in 64 bits, a NaN or
+ *                infinity included (no tensor at all, or only empty ones: 0).  dst is not looked at.
+ * vq_clip_grads: that norm, then dst = round(src * min(1, max_norm / (norm + 1e-6))).  dst_type is src_type, or
+ *                VQ_F32; dst == src (of one type) scales in place.  Otherwise no dst may overlap any src or other dst,
+ *                and in place no tensor may be listed twice.  max_norm >= 0.
+ * The result is the same bits on every run.  `work`: vq_grad_norm_work_bytes(n) bytes, 8-byte aligned, contents
+ * irrelevant; calls that may overlap need one each.  At most 65536 tensors (VQ_ERR_TOO_LARGE).
+ */
+enum { VQ_NORM_INF = 0, VQ_NORM_1 = 1, VQ_NORM_2 = 2 };
+typedef struct vq_tensor_ref {
+  const void* src;
+  void* dst;
+  int64_t numel;
+  int32_t src_type;
+  int32_t dst_type;
+} vq_tensor_ref;
+int64_t vq_grad_norm_work_bytes(int n);
+int vq_grad_norm(const vq_tensor_ref* refs, int n, int kind, float* norm, void* work, void* stream);
+int vq_clip_grads(const vq_tensor_ref* refs, int n, int kind, float max_norm, float* norm, void* work, void* stream);
+
+/*
  * Re-seed codes in place (maintenance).  ref: the per-code loops of
  * vqvae/ema_vector_quantizer.py:185-196 (reset_dead_codes: noise 0.2, scale 0.1), :262-274
  * (reset_low_usage_codes: noise 0.4, scale 0.2) and the new rows of :131-148 (expand_codebook:

@@ -1,0 +1,394 @@
+"""The linear layer (product with bias, activation and residual) and its gradients against the formulas in 64 bits.
+
+Tolerances are error bounds, element by element, u = 2^-24 being half a step of the fp32 sums and h half a step of the
+tensors' type (fp32 2^-24, bf16 2^-8, fp16 2^-11, relative to the value; fp16 also 2^-25 near zero):
+  * a sum of n products in fp32, in any order: (n + 1) u sum|a b|; the bias adds one rounding of the result;
+  * the activation: at most 1.13 times the error of its argument (the largest slope, that of gelu), plus its own evaluation,
+    at most 32 u (|p| + 1): a dozen operations, a 1-ulp exponential and reciprocal;
+  * an output: h |y| + u (|p| + |r| ...) for its additions;
+  * gradients: dp = gy act'(pre) has the error |gy| (0.8 (h |p| + error of p) + 32 u (|p| + 1)) -- 0.8 bounds |act''| -- and its
+    own rounding h |dp|; for relu the slope may also be the other one where |p| is within its error of 0.  The two
+    products carry that error through |W| and |x| and add their own.
+"""
+import math
+
+import pytest
+import torch
+
+import vq_vae_amd as vq
+from vq_vae_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda:0")
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25}
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+ACTS = ["none", "relu", "silu", "gelu", "gelu_tanh"]
+
+
+def act64(p, act):
+    if act == "none":
+        return p, torch.ones_like(p)
+    if act == "relu":
+        return p.clamp(min=0), (p > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(p)
+        return p * s, s * (1 + p * (1 - s))
+    if act == "gelu":
+        c = 0.5 * torch.special.erfc(-p / math.sqrt(2))
+        return p * c, c + p * torch.exp(-p * p / 2) / math.sqrt(2 * math.pi)
+    k = math.sqrt(2 / math.pi)
+    t = torch.tanh(k * (p + 0.044715 * p ** 3))
+    return 0.5 * p * (1 + t), 0.5 * (1 + t) + 0.5 * p * (1 - t * t) * k * (1 + 3 * 0.044715 * p * p)
+
+
+def forward64(x, w, b, act, r):
+    """y, pre, slope and the bounds of y and pre."""
+    kind, K = x.dtype, x.shape[-1]
+    h = HALF[kind]
+    x, w = x.double(), w.double()
+    p = x @ w.t()
+    ep = (K + 1) * U * (x.abs() @ w.abs().t())
+    if b is not None:
+        p = p + b.double()
+        ep = ep + U * p.abs()
+    a, slope = act64(p, act)
+    ey = 1.13 * ep + (32 * U * (p.abs() + 1) if act not in ("none", "relu") else 0)
+    y = a
+    if r is not None:
+        y = y + r.double()
+        ey = ey + U * y.abs()
+    return y, p, slope, ey * 1.001 + h * y.abs() + TINY[kind], ep
+
+
+def backward64(gy, x, w, p, ep, slope, act):
+    """gradients of input, weight and bias with their bounds."""
+    kind = x.dtype
+    h, (M, K), N = HALF[kind], x.shape, w.shape[0]
+    gy, x, w = gy.double(), x.double(), w.double()
+    dp = gy * slope
+    if act == "none":
+        ed = torch.zeros_like(dp)
+    else:
+        d_slope = 0.8 * (h * p.abs() + TINY[kind] + ep) + 32 * U * (p.abs() + 1)
+        if act == "relu":
+            d_slope = (p.abs() <= ep + TINY[kind]).double()
+        ed = gy.abs() * d_slope * 1.01 + h * dp.abs() * 1.01 + TINY[kind]
+    gx, gw, gb = dp @ w, dp.t() @ x, dp.sum(0)
+    ad = dp.abs() + ed
+    ex = ed @ w.abs() + (N + 1) * U * (ad @ w.abs()) + h * 1.01 * gx.abs() + TINY[kind]
+    ew = ed.t() @ x.abs() + (M + 1) * U * (ad.t() @ x.abs()) + h * 1.01 * gw.abs() + TINY[kind]
+    eb = ed.sum(0) + (M + 1) * U * ad.sum(0) + h * 1.01 * gb.abs() + TINY[kind]
+    return (gx, ex), (gw, ew), (gb, eb)
+
+
+def close(got, want, bound, what):
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bool(bad.any()), (f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst {float((err / bound).max()):.3g} of the bound "
+                                 f"at {[int(v) for v in bad.nonzero()[0]]}")
+
+
+def make(M, K, N, kind, bias, residual, strided, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def normal(*shape, scale=1.0):
+        return (torch.randn(*shape, generator=g, device=DEV) * scale).to(kind)
+    x = normal(M, 2 * K)[:, K:] if strided else normal(M, K)
+    w = normal(N, K + 5, scale=K ** -0.5)[:, :K] if strided else normal(N, K, scale=K ** -0.5)
+    return x, w, normal(N) if bias else None, (normal(M, N + 3)[:, :N] if strided else normal(M, N)) if residual else None, normal(M, N)
+
+
+# one row, a few, tiles that end inside, one element over a tile, reductions shorter than a step and split ones
+SIZES = [(1, 1, 1), (1, 256, 1024), (2, 7, 5), (3, 64, 2), (16, 130, 33), (17, 64, 64), (5, 20000, 40), (40, 8192, 72), (63, 65, 66),
+         (64, 64, 64), (129, 257, 127), (300, 515, 130), (1000, 96, 520), (777, 130, 515), (256, 512, 256), (2048, 40, 16),
+         (515, 1024, 2048), (2049, 1032, 2056)]
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_forward_and_gradients(size, kind):
+    M, K, N = size
+    i = SIZES.index(size) + TYPES.index(kind)
+    for act, bias, residual, strided in ((ACTS[i % 5], True, True, i % 2 == 1), (ACTS[(i + 2) % 5], i % 2 == 0, False, i % 2 == 0)):
+        x, w, b, r, gy = make(M, K, N, kind, bias, residual, strided, 100 * i)
+        y, p, slope, ey, ep = forward64(x, w, b, act, r)
+        close(vq.linear(x, w, b, act, r), y, ey, "forward")
+        leaves = [t.requires_grad_() for t in (x.detach(), w.detach(), b, r) if t is not None]
+        x2, w2 = leaves[0], leaves[1]
+        out = vq.linear(x2, w2, b, act, r)
+        close(out.detach(), y, ey, "forward with gradients")
+        grads = torch.autograd.grad(out, leaves, gy)
+        (gx, ex), (gw, ew), (gb, eb) = backward64(gy, x, w, p, ep, slope, act)
+        close(grads[0], gx, ex, "input gradient")
+        close(grads[1], gw, ew, "weight gradient")
+        if b is not None:
+            close(grads[2], gb, eb, "bias gradient")
+        if r is not None:
+            assert torch.equal(grads[-1], gy)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("act", ACTS)
+def test_every_activation(act, kind):
+    # values from the tails to the middle: the product is one-hot, so that p is an input
+    p = torch.cat([torch.linspace(-12, 12, 481), torch.tensor([0.0, -0.0, 1e-7, -1e-7, 60.0, -60.0, 200.0, -200.0])]).to(DEV, kind)
+    x = p.view(-1, 1)
+    w = torch.ones(1, 1, device=DEV, dtype=kind)
+    y, q, slope, ey, ep = forward64(x, w, None, act, None)
+    xr = x.clone().requires_grad_()
+    out = vq.linear(xr, w, activation=act)
+    close(out.detach(), y, ey, "forward")
+    (gx,) = torch.autograd.grad(out, xr, torch.ones_like(out))
+    (want, ex), _, _ = backward64(torch.ones_like(out), x, w, q, ep, slope, act)
+    close(gx, want, ex, "gradient")
+
+
+def test_differences():
+    # along a random direction, fp32: the loss is summed in 64 bits; the step's error is h^2 f''' / 6 with f''' of order 1 per
+    # element, the kernel's rounding error of y (1e-6 an element) is divided by 2 h
+    x, w, b, r, gy = make(40, 33, 21, torch.float32, True, True, False, 5)
+    for act in ("silu", "gelu", "gelu_tanh"):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+        out = vq.linear(leaves[0], leaves[1], leaves[2], act, leaves[3])
+        grads = torch.autograd.grad(out, leaves, gy)
+        g = torch.Generator(device=DEV).manual_seed(9)
+        step = 2.0 ** -7
+        for t, gt in zip(leaves, grads):
+            d = torch.randn(t.shape, generator=g, device=DEV)
+            d /= d.abs().max()
+
+            def loss(sign):
+                args = [(u + sign * step * d if u is t else u).detach() for u in leaves]
+                return (vq.linear(args[0], args[1], args[2], act, args[3]).double() * gy.double()).sum()
+            num = float((loss(1) - loss(-1)) / (2 * step))
+            ana = float((gt.double() * d.double()).sum())
+            n = gy.abs().double().sum().item()
+            # direction of x: |p'| <= sum|w| of about 4.6, of w: sum|x| of about 27; f''' <= 2 |p'|^3; errors of random sign add
+            # like their square root
+            reach = 4.6 if t is leaves[0] else 27.0 if t is leaves[1] else 1.0
+            tol = math.sqrt(gy.numel()) * (step ** 2 / 6 * 2 * reach ** 3 + 4e-6 / step) + 1e-6 * n
+            assert abs(num - ana) <= tol, (act, tuple(t.shape), num, ana, tol)
+
+
+def test_shapes_without_rows_and_with_many_dimensions():
+    w = torch.randn(5, 3, device=DEV, requires_grad=True)
+    b = torch.randn(5, device=DEV, requires_grad=True)
+    x = torch.zeros(0, 3, device=DEV, requires_grad=True)
+    y = vq.linear(x, w, b, "silu")
+    assert y.shape == (0, 5)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.zeros(0, 5, device=DEV))
+    assert gx.shape == (0, 3) and not gw.any() and not gb.any()
+    (gb,) = torch.autograd.grad(vq.linear(x.detach(), w.detach(), b), b, torch.zeros(0, 5, device=DEV))
+    assert not gb.any()
+    v = torch.randn(2, 3, 4, 3, device=DEV)
+    assert vq.linear(v, w, b).shape == (2, 3, 4, 5)
+    assert torch.equal(vq.linear(v, w, b).view(24, 5), vq.linear(v.view(24, 3), w, b))
+    assert vq.linear(v[0, 0, 0], w, b).shape == (5,)
+    # other strides: transposed, expanded rows, transposed weight
+    vt = v.transpose(1, 2)
+    assert torch.equal(vq.linear(vt, w, b), vq.linear(vt.contiguous(), w, b))
+    e = torch.randn(1, 3, device=DEV).expand(70, 3)
+    assert torch.equal(vq.linear(e, w, b), vq.linear(e.contiguous(), w, b))
+    wt = torch.randn(3, 5, device=DEV).t()
+    assert torch.equal(vq.linear(v, wt, b), vq.linear(v, wt.contiguous(), b))
+
+
+def test_expanded_inputs_have_summed_gradients():
+    # autograd reduces what expand broadcast; grad_output itself may be expanded too (a sum's gradient)
+    w = torch.randn(66, 40, device=DEV, requires_grad=True)
+    row = torch.randn(40, device=DEV, requires_grad=True)
+    res = torch.randn(66, device=DEV, requires_grad=True)
+    y = vq.linear(row.expand(100, 40), w, activation="gelu", residual=res.expand(100, 66))
+    g = torch.autograd.grad(y.sum(), (row, w, res))
+    rd, wd = row.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    want = torch.autograd.grad(torch.nn.functional.gelu(rd.expand(100, 40) @ wd.t()).sum(), (rd, wd))
+    for a, b in zip(g, want):      # 100 equal terms, each within 1e-5 of the scale of the gradient
+        assert float((a.double() - b).abs().max()) <= 2e-5 * float(b.abs().max())
+    assert torch.equal(g[2], torch.full_like(g[2], 100.0))
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M", [5, 100])
+def test_nonfinite_rows_stay_among_themselves(M, kind):
+    K, N = 70, 66
+    x, w, b, r, gy = make(M, K, N, kind, True, True, False, 3)
+    clean = vq.linear(x, w, b, "silu", r)
+    x[2, 5] = float("nan")
+    x[4, 69] = float("inf")
+    y = vq.linear(x, w, b, "silu", r)
+    keep = [i for i in range(M) if i not in (2, 4)]
+    assert torch.equal(y[keep], clean[keep])
+    assert bool(y[2].isnan().all()) and not bool(y[4].isfinite().all())
+    # a weight row: one output column
+    x, w, b, r, gy = make(M, K, N, kind, True, True, False, 3)
+    w[7, 0] = float("nan")
+    y = vq.linear(x, w, b, "silu", r)
+    cols = [j for j in range(N) if j != 7]
+    assert torch.equal(y[:, cols], clean[:, cols]) and bool(y[:, 7].isnan().all())
+    # relu keeps a NaN, as max(p, 0) with a NaN does
+    assert bool(vq.linear(x, w, b, "relu")[:, 7].isnan().all())
+
+
+def test_half_precision_beyond_its_range():
+    # pre is kept in fp16: beyond its range it is infinite, and the slope there is its limit, not inf * 0
+    x = torch.full((20, 64), 200.0, device=DEV, dtype=torch.float16, requires_grad=True)
+    w = torch.full((8, 64), 100.0, device=DEV, dtype=torch.float16, requires_grad=True)
+    for act in ACTS[1:]:
+        y = vq.linear(x, w, activation=act)
+        (gx,) = torch.autograd.grad(y, x, torch.full_like(y, 2.0 ** -6))
+        assert bool((gx == 100.0 * 8 * 2.0 ** -6).all()), act
+        y = vq.linear(x, -w.detach(), activation=act)
+        (gx,) = torch.autograd.grad(y, x, torch.full_like(y, 2.0 ** -6))
+        assert bool((gx == 0).all()), act
+
+
+def test_nothing_outside_the_outputs_is_written():
+    # through the C interface, outputs in the middle of larger buffers
+    lib = _lib.load()
+    for M, K, N, dt, kind in ((3, 40, 50, 1, torch.bfloat16), (65, 72, 129, 1, torch.bfloat16), (130, 33, 70, 0, torch.float32),
+                              (300, 256, 520, 2, torch.float16), (40, 4096, 65, 1, torch.bfloat16)):
+        x, w, b, r, gy = make(M, K, N, kind, True, True, False, 1)
+        s = ops._stream(DEV)
+
+        def band(n):
+            buf = torch.full((n + 128,), 7.0, device=DEV, dtype=kind)
+            return buf, buf[64:64 + n]
+        (yb, y), (pb, p), (xb, gx), (wb, gw), (bb, gb) = (band(n) for n in (M * N, M * N, M * K, N * K, N))
+        work = [torch.empty(max(16, lib.vq_linear_work_bytes(q, M, K, N, dt)), dtype=torch.uint8, device=DEV) for q in range(3)]
+        P = ops._ptr
+        assert lib.vq_linear(P(x), K, P(w), K, P(b), P(r), N, dt, 2, M, K, N, P(y), P(p), P(work[0]), s) == 0
+        assert lib.vq_linear_dgrad(P(gy), P(w), K, dt, M, K, N, P(gx), P(work[1]), s) == 0
+        assert lib.vq_linear_wgrad(P(gy), P(x), K, dt, M, K, N, P(gw), P(gb), P(work[2]), s) == 0
+        torch.cuda.synchronize()
+        for buf in (yb, pb, xb, wb, bb):
+            assert bool((buf[:64] == 7).all()) and bool((buf[-64:] == 7).all())
+        assert torch.equal(y.view(M, N), vq.linear(x, w, b, "silu", r))
+        # the bias gradient alone comes from another kernel: the same sums up to their order
+        gb2 = torch.empty(N, device=DEV, dtype=kind)
+        assert lib.vq_linear_wgrad(P(gy), None, K, dt, M, K, N, None, P(gb2), P(work[2]), s) == 0
+        ref = gy.double().sum(0)
+        bound = (M + 1) * U * gy.double().abs().sum(0) + 1.01 * HALF[kind] * ref.abs() + TINY[kind]
+        close(gb, ref, bound, "bias gradient")
+        close(gb2, ref, bound, "bias gradient alone")
+
+
+def test_partial_gradients():
+    x, w, b, r, gy = make(200, 64, 96, torch.bfloat16, True, True, False, 8)
+    full = {}
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    out = vq.linear(x, w, b, "gelu", r)
+    for t, g in zip(leaves, torch.autograd.grad(out, leaves, gy)):
+        full[id(t)] = g
+    for chosen in ([0], [1], [0, 1], [0, 2], [3], [1, 3]):
+        for i, t in enumerate(leaves):
+            t.requires_grad_(i in chosen)
+        out = vq.linear(x, w, b, "gelu", r)
+        for i, g in zip(chosen, torch.autograd.grad(out, [leaves[i] for i in chosen], gy)):
+            assert torch.equal(g, full[id(leaves[i])])
+    for t in leaves:
+        t.requires_grad_(False)
+    b.requires_grad_()
+    (gb,) = torch.autograd.grad(vq.linear(x, w, b, "gelu", r), [b], gy)
+    # the sums of the same 200 rounded terms in another order, rounded to bf16
+    assert float((gb.float() - full[id(b)].float()).abs().max()) <= 2.0 ** -7 * float(full[id(b)].float().abs().max())
+    with pytest.raises(RuntimeError):      # differentiable once
+        x.requires_grad_()
+        (gx,) = torch.autograd.grad(vq.linear(x, w, b, "gelu").float().sum(), [x], create_graph=True)
+        torch.autograd.grad(gx.float().sum(), [x])
+
+
+def test_same_bits_on_every_run():
+    x, w, b, r, gy = make(3000, 520, 264, torch.bfloat16, True, True, False, 4)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    runs = []
+    for _ in range(3):
+        out = vq.linear(x, w, b, "silu", r)
+        runs.append([out.detach(), *torch.autograd.grad(out, leaves, gy)])
+    for other in runs[1:]:
+        assert all(torch.equal(a, c) for a, c in zip(runs[0], other))
+
+
+def test_large_offsets():
+    # inputs and outputs of more than 2^31 elements (4 GiB and more): rows at the start, in the middle and at the end
+    M, K, N = 2 ** 21 + 3, 1032, 1040
+    w = torch.randn(N, K, device=DEV).mul_(K ** -0.5).bfloat16()
+    b = torch.randn(N, device=DEV).bfloat16()
+    x = torch.empty(M, K, device=DEV, dtype=torch.bfloat16)
+    for part in x.split(2 ** 18):
+        part.copy_(torch.randn(part.shape, device=DEV))
+    y = vq.linear(x, w, b, "silu")
+    rows = torch.tensor([0, 1, 2 ** 20 - 1, 2 ** 20, M // 2, 2 ** 21 - 1, 2 ** 21, M - 2, M - 1], device=DEV)
+    want, _, _, ey, _ = forward64(x[rows], w, b, "silu", None)
+    close(y[rows], want, ey, "forward")
+    # weight gradient: a sum over all rows.  gy is one at chosen rows, zero elsewhere
+    gy = y.zero_()
+    gy[rows] = 1.0
+    w.requires_grad_()
+    xg = x.requires_grad_()
+    gx, gw = torch.autograd.grad(vq.linear(xg, w), [xg, w], gy)
+    want = x.detach()[rows].double().sum(0).expand(N, K)
+    bound = 10 * U * x.detach()[rows].double().abs().sum(0).expand(N, K) + HALF[torch.bfloat16] * 1.01 * want.abs() + 1e-30
+    close(gw, want, bound, "weight gradient")
+    wsum = w.detach().double().sum(0)
+    bound = (N + 1) * U * w.detach().double().abs().sum(0) + HALF[torch.bfloat16] * 1.01 * wsum.abs() + 1e-30
+    close(gx[rows], wsum.expand(len(rows), K), bound.expand(len(rows), K), "input gradient")
+    assert not bool(gx[rows[-1] - 2 - 5].any())
+
+
+def test_other_stream_and_layer():
+    layer = vq.Linear(72, 40, activation="gelu").to(DEV, torch.bfloat16)
+    x = torch.randn(33, 72, device=DEV).bfloat16()
+    r = torch.randn(33, 40, device=DEV).bfloat16()
+    want = layer(x, r)
+    assert torch.equal(want, vq.linear(x, layer.weight, layer.bias, "gelu", r))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [layer(x, r) for _ in range(4)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(want, o) for o in outs)
+    with torch.autocast("cuda", dtype=torch.float16):       # the tensors' types stay
+        assert torch.equal(layer(x, r), want)
+
+
+@pytest.mark.parametrize("M", [4, 700])
+def test_captured_and_replayed(M):
+    # forward and backward in two graphs with memory of their own, replayed in turn between eager work, on new inputs
+    kind, K, N = torch.bfloat16, 264, 136
+    w = torch.randn(N, K, device=DEV).mul_(0.06).to(kind).requires_grad_()
+    b = torch.randn(N, device=DEV).to(kind).requires_grad_()
+
+    def step(x, r, gy):
+        y = vq.linear(x, w, b, "gelu", r)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), gy))
+
+    def inputs(seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        return [torch.randn(*s, generator=g, device=DEV).to(kind) for s in ((M, K), (M, N), (M, N))]
+
+    graphs = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        held = [[t.requires_grad_(i == 0) for i, t in enumerate(inputs(k))] for k in range(2)]
+        step(*held[0])
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*held[k])
+        graphs.append((graph, held[k], out))
+    for n in range(3):
+        for k, (graph, ins, outs) in enumerate(graphs):
+            new = inputs(10 * n + k + 5)
+            with torch.no_grad():
+                for t, v in zip(ins, new):
+                    t.copy_(v)
+            graph.replay()
+            torch.cuda.synchronize()
+            want = step(new[0].requires_grad_(), *new[1:])
+            for o, e in zip(outs, want):
+                assert torch.equal(o, e)

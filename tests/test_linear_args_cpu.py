@@ -1,0 +1,179 @@
+"""Refusals of the linear layer, the gradient norm and clipping: wrong arguments end in an error before anything is
+launched, in Python and at the C interface.  Nothing here needs a GPU."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import vq_vae_amd as vq
+from vq_vae_amd import _lib
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def t(*shape, dtype=F32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("args, kwargs, error, says", [
+    ((t(2, 3), t(4, 3)), {}, RuntimeError, "GPU"),
+    ((t(2, 3), t(4, 3)), {"activation": "tanh"}, ValueError, "activation"),
+    ((t(2, 3), t(4, 5)), {}, ValueError, "in features"),
+    ((t(2, 3), t(3)), {}, ValueError, "weight"),
+    ((t(2, 3), t(0, 3)), {}, ValueError, "weight"),
+    ((t(2, 0), t(4, 0)), {}, ValueError, "weight"),
+    ((t(2, 3), t(4, 3, dtype=BF)), {}, TypeError, "share one type"),
+    ((t(2, 3), t(4, 3), t(4, dtype=BF)), {}, TypeError, "share one type"),
+    ((t(2, 3, dtype=torch.float64), t(4, 3, dtype=torch.float64)), {}, TypeError, "float64"),
+    ((t(2, 3), t(4, 3), t(3)), {}, ValueError, "bias"),
+    ((t(2, 3), t(4, 3), t(1, 4)), {}, ValueError, "bias"),
+    ((t(2, 3), t(4, 3)), {"residual": t(2, 3)}, ValueError, "residual"),
+    ((t(2, 3), t(4, 3)), {"residual": t(1, 4)}, ValueError, "residual"),        # nothing is broadcast
+    ((t(2, 3), t(4, 3)), {"residual": t(4)}, ValueError, "residual"),
+    ((t(()), t(4, 3)), {}, ValueError, "in features"),
+    ((np.zeros((2, 3)), t(4, 3)), {}, TypeError, "tensor"),
+    ((t(2, 3), None), {}, TypeError, "weight"),
+    ((torch.zeros(1, 1).expand(1, (1 << 20) + 1), torch.zeros(1, 1).expand(1, (1 << 20) + 1)), {}, ValueError, "up to"),
+])
+def test_linear_refuses(args, kwargs, error, says):
+    with pytest.raises(error, match=says):
+        vq.linear(*args, **kwargs)
+
+
+def test_layer_has_the_parameters_of_a_linear_layer():
+    a, b = vq.Linear(5, 7, activation="silu"), torch.nn.Linear(5, 7)
+    assert {k: v.shape for k, v in a.state_dict().items()} == {k: v.shape for k, v in b.state_dict().items()}
+    a.load_state_dict(b.state_dict())
+    assert "silu" in repr(a)
+    with pytest.raises(ValueError, match="activation"):
+        vq.Linear(5, 7, activation="sine")
+
+
+def test_gradient_functions_refuse():
+    g = [t(3), t(4)]
+    with pytest.raises(RuntimeError, match="GPU"):
+        vq.grad_norm(g)
+    with pytest.raises(RuntimeError, match="GPU"):
+        vq.clip_grads(g, 1.0)
+    for bad in (0, 3, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="norm_type"):
+            vq.grad_norm(g, bad)
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            vq.clip_grads(g, bad)
+    with pytest.raises(TypeError, match="float64"):
+        vq.grad_norm([t(3, dtype=torch.float64)])
+    with pytest.raises(TypeError, match="tensors"):
+        vq.grad_norm([t(3), None])
+    with pytest.raises(TypeError, match="dense"):
+        vq.grad_norm([t(3, 3).to_sparse()])
+    with pytest.raises(ValueError, match="one device"):
+        vq.grad_norm([t(3), torch.zeros(3, device="meta")])
+
+
+def test_clipping_refuses_shared_and_expanded_memory():
+    a = t(6, 4)
+    for bad in ([a, a], [a, a[2:3]], [a[:, :2], a[:, 1:3]], [a, a.t()], [a.view(-1)[:5], a.view(-1)[4:]]):
+        with pytest.raises(ValueError, match="share memory"):
+            vq.clip_grads(bad, 1.0)
+    with pytest.raises(ValueError, match="expanded"):
+        vq.clip_grads([t(1, 4).expand(3, 4)], 1.0)
+    with pytest.raises(ValueError, match="share memory"):
+        vq.clip_grads([a[0], a[1]], 1.0, out=[a[1], a[0]])
+    # neighbours in one buffer are apart
+    with pytest.raises(RuntimeError, match="GPU"):
+        vq.clip_grads([a[:3], a[3:]], 1.0)
+
+
+def test_clipping_refuses_wrong_outputs():
+    with pytest.raises(ValueError, match="1 gradients but 2"):
+        vq.clip_grads([t(3)], 1.0, out=[t(3), t(3)])
+    with pytest.raises(ValueError, match="shape"):
+        vq.clip_grads([t(3)], 1.0, out=[t(4)])
+    with pytest.raises(TypeError, match="same type or float32"):
+        vq.clip_grads([t(3)], 1.0, out=[t(3, dtype=BF)])
+    with pytest.raises(ValueError, match="requires a gradient"):
+        vq.clip_grads([t(3)], 1.0, out=[t(3).requires_grad_()])
+
+
+def test_nothing_to_clip():
+    assert float(vq.grad_norm([])) == 0.0
+    assert float(vq.clip_grads([], 1.0)) == 0.0
+    p = torch.nn.Parameter(t(3))
+    assert float(vq.clip_grad_norm_([p], 1.0)) == 0.0
+    with pytest.raises(ValueError, match="max_norm"):
+        vq.clip_grad_norm_([p], -1.0)
+
+
+INVALID, UNSUPPORTED, TOO_LARGE = 1, 2, 3
+
+
+def test_c_interface_checks_its_arguments():
+    lib = _lib.load()
+    p = ctypes.c_void_p(4096)                  # never followed: every call below ends at its checks
+    ok = (p, 8, p, 8, None, None, 0, 0, 0, 4, 8, 8, p, None, p, None)
+
+    def linear(**kw):
+        names = "x ldx W ldw bias residual ldr dtype act M K N y pre work stream".split()
+        return lib.vq_linear(*(kw.get(n, v) for n, v in zip(names, ok)))
+
+    for kw in ({"x": None}, {"W": None}, {"y": None}, {"M": -1}, {"K": 0}, {"N": 0}, {"dtype": 3}, {"dtype": -1}, {"act": 5},
+               {"act": -1}, {"ldx": 7}, {"ldw": 7}, {"residual": p, "ldr": 7}):
+        assert linear(**kw) == INVALID, kw
+    assert linear(K=(1 << 20) + 1, ldx=1 << 21, ldw=1 << 21) == UNSUPPORTED
+    assert linear(ldx=1 << 22) == UNSUPPORTED
+    assert linear(M=(1 << 31) + 1) == UNSUPPORTED
+    assert linear(M=0, x=None, y=None) == 0
+    assert lib.vq_linear_act_grad(p, p, 0, 0, 8, p, None) == INVALID      # no activation has no gradient to apply
+    assert lib.vq_linear_act_grad(None, p, 0, 1, 8, p, None) == INVALID
+    assert lib.vq_linear_act_grad(p, p, 0, 1, -1, p, None) == INVALID
+    assert lib.vq_linear_act_grad(None, None, 0, 1, 0, None, None) == 0
+    assert lib.vq_linear_dgrad(None, p, 8, 0, 4, 8, 8, p, p, None) == INVALID
+    assert lib.vq_linear_dgrad(p, p, 7, 0, 4, 8, 8, p, p, None) == INVALID
+    assert lib.vq_linear_dgrad(None, p, 8, 0, 0, 8, 8, None, p, None) == 0
+    assert lib.vq_linear_wgrad(p, p, 8, 0, 4, 8, 8, None, None, p, None) == INVALID
+    assert lib.vq_linear_wgrad(p, None, 8, 0, 4, 8, 8, p, None, p, None) == INVALID
+    assert lib.vq_linear_wgrad(p, p, 8, 0, 4, 8, 8, None, p, None, None) == INVALID     # the column sums need work
+    assert lib.vq_linear_wgrad(p, p, 8, 0, 4, 8, 8, p, p, None, None) == INVALID
+    # a split sum without its workspace
+    assert lib.vq_linear_work_bytes(2, 1 << 20, 64, 64, 1) > 0
+    assert lib.vq_linear_wgrad(p, p, 64, 1, 1 << 20, 64, 64, p, None, None, None) == INVALID
+    for bad in ((3, 4, 8, 8, 0), (0, -1, 8, 8, 0), (0, 4, 0, 8, 0), (0, 4, 8, 8, 7)):
+        assert lib.vq_linear_work_bytes(*bad) == 0
+
+
+class Ref(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("numel", ctypes.c_int64), ("src_type", ctypes.c_int32),
+                ("dst_type", ctypes.c_int32)]
+
+
+def test_c_interface_checks_the_tensor_list():
+    lib = _lib.load()
+    p = ctypes.c_void_p(4096)
+
+    def both(*refs, kind=2, max_norm=1.0, norm=p, work=p, n=None):
+        arr = (Ref * max(1, len(refs)))(*refs)
+        n = len(refs) if n is None else n
+        return (lib.vq_grad_norm(arr, n, kind, norm, work, None), lib.vq_clip_grads(arr, n, kind, max_norm, norm, work, None))
+
+    good = Ref(4096, 8192, 8, 0, 0)
+    assert both(good, kind=3) == (INVALID, INVALID)
+    assert both(good, kind=-1) == (INVALID, INVALID)
+    assert both(good, norm=None) == (INVALID, INVALID)
+    assert both(good, work=None) == (INVALID, INVALID)
+    assert both(good, work=ctypes.c_void_p(4100)) == (INVALID, INVALID)
+    assert both(good, n=-1) == (INVALID, INVALID)
+    assert both(Ref(None, 8192, 8, 0, 0)) == (INVALID, INVALID)
+    assert both(Ref(4096, 8192, -1, 0, 0)) == (INVALID, INVALID)
+    assert both(Ref(4096, 8192, 8, 3, 3)) == (INVALID, INVALID)
+    arr = (Ref * 1)(Ref(4096, None, 8, 0, 0))
+    assert lib.vq_clip_grads(arr, 1, 2, 1.0, p, p, None) == INVALID
+    arr = (Ref * 1)(Ref(4096, 8192, 8, 0, 1))          # fp32 into bf16
+    assert lib.vq_clip_grads(arr, 1, 2, 1.0, p, p, None) == INVALID
+    arr = (Ref * 1)(good)
+    assert lib.vq_clip_grads(arr, 1, 2, -1.0, p, p, None) == INVALID
+    assert lib.vq_clip_grads(arr, 1, 2, float("nan"), p, p, None) == INVALID
+    many = (Ref * 65537)()
+    assert lib.vq_grad_norm(many, 65537, 2, p, p, None) == TOO_LARGE
+    assert lib.vq_grad_norm_work_bytes(-1) == 0 and lib.vq_grad_norm_work_bytes(0) > 0

@@ -14,6 +14,11 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("VQ_VAE_AMD_LIB") or os.path.join(_PKG, "libvqhip.so")
 
 LAYOUT_ND, LAYOUT_NCHW = 0, 1
+F32, BF16, F16 = 0, 1, 2
+NORM_INF, NORM_1, NORM_2 = 0, 1, 2
+LINEAR_FORWARD, LINEAR_DGRAD, LINEAR_WGRAD = 0, 1, 2
+#: activation name -> VQ_ACT_*
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 #: every symbol include/vq_hip.h declares: name -> (restype, argtypes)
 SIGNATURES = {
@@ -83,6 +88,16 @@ SIGNATURES = {
     "vq_conv1x1_wgrad_work_bytes": (c_int64, [c_int64, c_int, c_int]),
     "vq_conv1x1_wgrad": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int64, c_void_p, c_void_p,
                                  c_void_p, c_void_p]),
+    "vq_linear_work_bytes": (c_int64, [c_int, c_int64, c_int, c_int, c_int]),
+    "vq_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64, c_int,
+                          c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "vq_linear_act_grad": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p]),
+    "vq_linear_dgrad": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "vq_linear_wgrad": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                c_void_p]),
+    "vq_grad_norm_work_bytes": (c_int64, [c_int]),
+    "vq_grad_norm": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "vq_clip_grads": (c_int, [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),
     "vq_reseed_stage_bytes": (c_size_t, [c_int, c_int]),
     "vq_reseed_codes": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int,
                                 c_float, c_float, ctypes.c_uint64, c_void_p, c_void_p]),

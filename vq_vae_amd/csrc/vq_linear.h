@@ -1,0 +1,616 @@
+// Matrix product with bias, activation and residual in its epilogue, and the products of its backward
+// pass (gfx950): shared device code of vq_linear_{f32,bf16,f16}.hip and vq_linear.hip.
+//
+// All three products are   C[i][j] = sum_r A(i, r) B(j, r)   with fp32 accumulation:
+//     forward          i = row, j = output channel, r = input channel    A = x,  B = W      both with r contiguous
+//     input gradient   i = row, j = input channel,  r = output channel   A = dp, B = W      B with j contiguous
+//     weight gradient  i = output channel, j = input channel, r = row    A = dp, B = x      both with i / j contiguous
+// An operand whose reduction index is contiguous is called r-major here, the other kind m-major.
+#pragma once
+#include "vq_common.h"
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct VqBf16 { uint16_t v; };   // element types of the templates: float, VqBf16, _Float16
+
+enum { VQL_C64 = 0, VQL_C128 = 1, VQL_C256 = 2 };
+
+struct VqLinearArgs {
+  const char* A;
+  const char* B;
+  int64_t lda, ldb;          // bytes between rows of the operand as it lies in memory
+  int64_t I;                 // rows of C
+  int J;                     // columns of C
+  int64_t R;                 // length of the sum
+  int64_t steps_per_split;   // 128-byte steps of the sum that one workgroup takes
+  int splits;
+  int64_t tiles_i;
+  int tiles_j;
+  void* out;                 // [I][J]
+  void* pre;                 // [I][J] or null: C + bias in T, what the activation's gradient needs
+  const void* bias;          // [J] or null
+  const char* res;           // [I][J] or null
+  int64_t ldr;               // bytes between rows of res
+  int act;
+  float* part;               // splits > 1: [splits][I][ldp] partial sums
+  int ldp;
+  float* asum;               // weight gradient: [splits][I] sums of A over r (the bias gradient), or null
+};
+
+// -------------------------------------------------------------------------------- element conversions
+template <typename T> struct VqElem;
+template <> struct VqElem<float> {
+  static __device__ __forceinline__ float to(float v) { return v; }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <> struct VqElem<VqBf16> {
+  static __device__ __forceinline__ float to(VqBf16 v) { return __uint_as_float((uint32_t)v.v << 16); }
+  static __device__ __forceinline__ VqBf16 from(float f) {
+    // the compiler's conversion: round to nearest, ties to even, NaN stays NaN (one instruction per pair)
+    return {__builtin_bit_cast(uint16_t, (__bf16)f)};
+  }
+};
+template <> struct VqElem<_Float16> {
+  static __device__ __forceinline__ float to(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 from(float f) { return (_Float16)f; }
+};
+
+// 16 bytes of T at any element-aligned address (the hardware takes unaligned 16-byte accesses)
+template <typename T>
+struct alignas(sizeof(T)) VqChunk {
+  T e[16 / sizeof(T)];
+};
+typedef u32x4 vql_u32x4_a2 __attribute__((aligned(2), may_alias));
+typedef u32x4 vql_u32x4_a4 __attribute__((aligned(4), may_alias));
+typedef u32x4 vql_u32x4_a16 __attribute__((may_alias));
+typedef f32x4 vql_f32x4 __attribute__((may_alias));
+#define VQL_LDS __attribute__((address_space(3)))
+typedef uint32_t vql_u32 __attribute__((may_alias));
+typedef uint16_t vql_u16 __attribute__((may_alias));
+template <typename T>
+__device__ __forceinline__ u32x4 vql_load16(const char* p) {
+  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const vql_u32x4_a4*>(p);
+  else return *reinterpret_cast<const vql_u32x4_a2*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void vql_store16(void* p, u32x4 v) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<vql_u32x4_a4*>(p) = v;
+  else *reinterpret_cast<vql_u32x4_a2*>(p) = v;
+}
+// `valid` of the 16 / sizeof(T) elements at p, the others zero
+template <typename T>
+__device__ __forceinline__ u32x4 vql_load16_part(const char* p, int64_t valid) {
+  constexpr int E = 16 / sizeof(T);
+  if (valid >= E) return vql_load16<T>(p);
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < E - 1; ++e)
+    if (e < valid) {
+      if constexpr (sizeof(T) == 4)
+        v[e] = *reinterpret_cast<const vql_u32*>(p + 4 * e);
+      else
+        v[e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(p + 2 * e) << (16 * (e & 1));
+    }
+  return v;
+}
+
+// -------------------------------------------------------------------------------- activations
+// erfc(z) for z >= 0: the Chebyshev fit of Numerical Recipes' erfcc (W. H. Press), relative error below 1.2e-7
+// everywhere; used where the result is rounded to 16 bits, together with the exponential it contains.
+__device__ __forceinline__ float vql_erfc_pos(float z) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.0f));
+  float q = 0.17087277f;
+  q = __builtin_fmaf(q, t, -0.82215223f);
+  q = __builtin_fmaf(q, t, 1.48851587f);
+  q = __builtin_fmaf(q, t, -1.13520398f);
+  q = __builtin_fmaf(q, t, 0.27886807f);
+  q = __builtin_fmaf(q, t, -0.18628806f);
+  q = __builtin_fmaf(q, t, 0.09678418f);
+  q = __builtin_fmaf(q, t, 0.37409196f);
+  q = __builtin_fmaf(q, t, 1.00002368f);
+  q = __builtin_fmaf(q, t, -1.26551223f);
+  return t * __expf(__builtin_fmaf(-z, z, q));
+}
+// FAST: 16-bit results. 1-ulp reciprocal and the hardware exponential, errors of some 1e-7 against a rounding of
+// 2^-9 or 2^-12; fp32 results take the library's functions and true divisions.
+template <bool FAST>
+__device__ __forceinline__ float vql_sigmoid(float p) {
+  if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __expf(-p));
+  return 1.0f / (1.0f + expf(-p));
+}
+template <bool FAST>
+__device__ __forceinline__ float vql_cdf(float p) {   // Phi(p)
+  if constexpr (FAST) {
+    const float half = 0.5f * vql_erfc_pos(fabsf(p) * 0.70710678f);
+    return p < 0.0f ? half : 1.0f - half;
+  }
+  return 0.5f * erfcf(-p * 0.70710678f);
+}
+template <bool FAST>
+__device__ __forceinline__ float vql_act(float p, int act) {
+  switch (act) {
+    case VQ_ACT_RELU: return p < 0.0f ? 0.0f : p;
+    case VQ_ACT_SILU: return p * vql_sigmoid<FAST>(p);
+    case VQ_ACT_GELU: return p * vql_cdf<FAST>(p);
+    case VQ_ACT_GELU_TANH: {
+      // (1 + tanh u) / 2 = sigmoid(2u)
+      const float u2 = 1.5957691216f * p * __builtin_fmaf(0.044715f * p, p, 1.0f);
+      return p * vql_sigmoid<FAST>(u2);
+    }
+    default: return p;
+  }
+}
+// act'(p).  Beyond |p| = 100 every derivative has its limit, 0 or 1; the clamp keeps inf * 0 out of it.
+template <bool FAST>
+__device__ __forceinline__ float vql_act_slope(float p0, int act) {
+  float p = p0 > 100.0f ? 100.0f : p0;
+  p = p < -100.0f ? -100.0f : p;   // NaN passes both
+  switch (act) {
+    case VQ_ACT_RELU: return p <= 0.0f ? 0.0f : 1.0f;
+    case VQ_ACT_SILU: {
+      const float s = vql_sigmoid<FAST>(p);
+      return s * __builtin_fmaf(p, 1.0f - s, 1.0f);
+    }
+    case VQ_ACT_GELU: {
+      const float g = FAST ? __expf(-0.5f * p * p) : expf(-0.5f * p * p);
+      return __builtin_fmaf(p * 0.3989422804f, g, vql_cdf<FAST>(p));
+    }
+    case VQ_ACT_GELU_TANH: {
+      const float p2 = p * p;
+      const float s = vql_sigmoid<FAST>(1.5957691216f * p * __builtin_fmaf(0.044715f, p2, 1.0f));
+      const float du2 = 1.5957691216f * __builtin_fmaf(0.134145f, p2, 1.0f);
+      return __builtin_fmaf(p * s * (1.0f - s), du2, s);
+    }
+    default: return 1.0f;
+  }
+}
+
+// -------------------------------------------------------------------------------- matrix core
+// One 16-byte fragment per lane of each operand.  16-bit types: lane l holds index l % 32, r = 8 (l / 32) + 0..7, one
+// 32x32x16 product.  fp32: r = 4 (l / 32) + 0..3, four 32x32x2 products (each pairs r = e with r = 4 + e, the same for
+// both operands).  D: lane l holds column l % 32 (of `b`), register g row 8 (g / 4) + 4 (l / 32) + g % 4 (of `a`).
+template <typename T>
+__device__ __forceinline__ f32x16 vql_mma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (__is_same(T, VqBf16)) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else if constexpr (__is_same(T, _Float16)) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else {
+    const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[e], fb[e], c, 0, 0, 0);
+    return c;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float vql_sum16(u32x4 v) {   // sum of the fragment's elements
+  float s = 0.0f;
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 f = __builtin_bit_cast(f32x4, v);
+    s = (f[0] + f[1]) + (f[2] + f[3]);
+  } else {
+    const VqChunk<T> c = __builtin_bit_cast(VqChunk<T>, v);
+    float q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = VqElem<T>::to(c.e[e]);
+    s = ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+  }
+  return s;
+}
+
+// -------------------------------------------------------------------------------- operand tiles in LDS
+// One step of the sum covers 128 bytes of r: 64 elements of 16 bits, 32 of 32 bits.
+// r-major tile of `B` indexes: B rows of 128 bytes, 16-byte piece c of row m in slot c ^ ((m >> 1) & 7): the 32 rows
+//   that a fragment read touches fall on all banks evenly.
+// m-major tile: one row of B elements per r, 16-byte piece c of row r in slot c ^ vql_mswz<T>(r): the rows that one
+//   transposing read (16 bits: r = 8h + 4t + 0..3 for both halves h) or one fp32 read (r = e and 4 + e) touches lie in
+//   different 64- or 128-byte segments.
+// The permutation is applied to the source address, so that the DMA, which writes LDS in lane order, needs no more.
+template <typename T>
+__device__ __forceinline__ int vql_mswz(int r) {
+  if constexpr (sizeof(T) == 2) return ((r & 3) | ((r >> 1) & 4)) << 2;
+  return ((r >> 2) & 1) << 3;
+}
+
+template <typename T, bool MMAJOR, int B, int NT, bool DMA>
+struct VqOperand {
+  static constexpr int ES = sizeof(T), E = 16 / ES, BK = 128 / ES;
+  static constexpr int BYTES = B * 128;
+  static constexpr int CPR = MMAJOR ? B / E : 8;       // 16-byte pieces per row of the tile
+  static constexpr int PER = BYTES / 16 / NT;          // pieces per thread
+  static constexpr int SWZ = MMAJOR ? CPR - 1 : 7;
+  static constexpr bool SUMS = MMAJOR;                 // only the weight gradient's A operand is summed
+  const char* base;      // m-major: column m0 of row 0; r-major: row m0
+  int64_t ld;            // bytes
+  int64_t M;             // indexes that exist from m0 on
+  uint32_t off[PER];     // this lane's byte offsets of a full step
+
+  __device__ __forceinline__ static void where(int n, int wave, int lane, int& row, int& piece) {
+    const int p = (wave * PER + n) * 64 + lane;
+    row = p / CPR;
+    piece = (p % CPR) ^ ((MMAJOR ? vql_mswz<T>(row) : (row >> 1)) & SWZ);
+  }
+  __device__ __forceinline__ void init(const char* src, int64_t ld_, int64_t m0, int64_t total, int wave, int lane) {
+    ld = ld_;
+    M = total - m0;
+    base = MMAJOR ? src + m0 * ES : src + m0 * ld_;
+    if constexpr (DMA) {
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        int row, piece;
+        where(n, wave, lane, row, piece);
+        if constexpr (MMAJOR) {   // pieces behind the last index repeat the last one: those outputs are not stored
+          const int last = (int)(M < B ? M : B) / E - 1;
+          off[n] = (uint32_t)(row * ld) + (piece < last ? piece : last) * 16;
+        } else {
+          const int last = (int)(M < B ? M : B) - 1;
+          off[n] = (uint32_t)((row < last ? row : last) * ld) + piece * 16;
+        }
+      }
+    }
+  }
+  // a whole step (all BK values of r exist), straight into LDS
+  __device__ __forceinline__ void dma(int64_t step, VQL_LDS char* lds, int wave) const {
+    const char* p = MMAJOR ? base + step * (BK * ld) : base + step * 128;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (VQL_LDS void*)(lds + (wave * PER + n) * 1024), 16, off[n], 0, 0, 0);
+  }
+  // any step, by way of registers: indexes and r that do not exist read as zero
+  __device__ __forceinline__ void fetch(int64_t step, int64_t R, int wave, int lane, u32x4 (&v)[PER]) const {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      int row, piece;
+      where(n, wave, lane, row, piece);
+      const int64_t r0 = step * BK;
+      int64_t valid;
+      const char* p;
+      if constexpr (MMAJOR) {
+        valid = r0 + row < R ? M - piece * E : 0;
+        p = base + (r0 + row) * ld + piece * 16;
+      } else {
+        valid = row < M ? R - r0 - piece * E : 0;
+        p = base + row * ld + r0 * ES + piece * 16;
+      }
+      v[n] = vql_load16_part<T>(p, valid);
+    }
+  }
+  __device__ __forceinline__ void commit(VQL_LDS char* lds, int wave, int lane, const u32x4 (&v)[PER]) const {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) *reinterpret_cast<VQL_LDS vql_u32x4_a16*>(lds + ((wave * PER + n) * 64 + lane) * 16) = v[n];
+  }
+  // fragment of indexes m .. m + 31 for the q-th quarter of the step
+  __device__ __forceinline__ static u32x4 frag(const VQL_LDS char* lds, int m, int q, int lane) {
+    const int h = lane >> 5;
+    if constexpr (!MMAJOR) {
+      const int row = m + (lane & 31);
+      return *reinterpret_cast<const VQL_LDS vql_u32x4_a16*>(lds + row * 128 + (((2 * q + h) ^ ((row >> 1) & 7)) * 16));
+    } else if constexpr (ES == 2) {
+      // transposing read: each group of 16 lanes names 4 rows (r) of 16 consecutive indexes, 8 bytes a lane, and lane i
+      // of the group receives index i of the four rows
+      const int s = lane & 15, col = m + ((lane >> 4) & 1) * 16 + (s & 3) * 4;
+      s16x4 half[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 16 * q + 8 * h + 4 * t + (s >> 2);
+        const int at = r * (B * 2) + ((((col >> 3) ^ (vql_mswz<T>(r) & SWZ)) * 16) | ((col & 4) * 2));
+        half[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((VQL_LDS s16x4*)(lds + at));
+      }
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      return __builtin_bit_cast(u32x4, (s16x8)__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      u32x4 v;
+      const int col = m + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 8 * q + 4 * h + e;
+        v[e] = *reinterpret_cast<const VQL_LDS vql_u32*>(lds + r * (B * 4) + ((((col >> 2) ^ (vql_mswz<T>(r) & SWZ)) * 16) | ((col & 3) * 4)));
+      }
+      return v;
+    }
+  }
+};
+
+// -------------------------------------------------------------------------------- epilogue of 16 / sizeof(T) columns
+// y = act(c + bias) + residual, rounded once; `pre` = c + bias rounded (kept for the activation's gradient).
+template <typename T>
+__device__ __forceinline__ void vql_epilogue(const VqLinearArgs& a, int64_t i, int j, const float* c, const float* bias) {
+  constexpr int E = 16 / sizeof(T);
+  constexpr bool FAST = sizeof(T) == 2;
+  const int n = a.J - j < E ? a.J - j : E;
+  float p[E], r[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) p[e] = c[e] + bias[e];
+  if (a.res) {
+    const VqChunk<T> rv = __builtin_bit_cast(VqChunk<T>, vql_load16_part<T>(a.res + i * a.ldr + (int64_t)j * sizeof(T), n));
+#pragma unroll
+    for (int e = 0; e < E; ++e) r[e] = VqElem<T>::to(rv.e[e]);
+  }
+  VqChunk<T> y, pv;
+#pragma unroll
+  for (int e = 0; e < E; ++e) pv.e[e] = VqElem<T>::from(p[e]);
+  if (a.act != VQ_ACT_NONE) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) p[e] = vql_act<FAST>(p[e], a.act);
+  }
+  if (a.res) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) p[e] += r[e];
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(p[e]);
+  T* yp = reinterpret_cast<T*>(a.out) + i * a.J + j;
+  T* pp = a.pre ? reinterpret_cast<T*>(a.pre) + i * a.J + j : nullptr;
+  if (n == E) {
+    vql_store16<T>(yp, __builtin_bit_cast(u32x4, y));
+    if (pp) vql_store16<T>(pp, __builtin_bit_cast(u32x4, pv));
+  } else {
+#pragma unroll
+    for (int e = 0; e < E - 1; ++e)
+      if (e < n) {
+        yp[e] = y.e[e];
+        if (pp) pp[e] = pv.e[e];
+      }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void vql_bias16(const VqLinearArgs& a, int j, float* bias) {
+  constexpr int E = 16 / sizeof(T);
+#pragma unroll
+  for (int e = 0; e < E; ++e) bias[e] = 0.0f;
+  if (a.bias && j < a.J) {
+    const VqChunk<T> b = __builtin_bit_cast(
+        VqChunk<T>, vql_load16_part<T>(reinterpret_cast<const char*>(a.bias) + (int64_t)j * sizeof(T), a.J - j));
+#pragma unroll
+    for (int e = 0; e < E; ++e) bias[e] = VqElem<T>::to(b.e[e]);
+  }
+}
+
+// -------------------------------------------------------------------------------- one step
+// The matrix work of one step on the tiles at `cur`.
+template <typename T, typename OA, typename OB, int TI, int TJ>
+__device__ __forceinline__ void vql_compute(const VQL_LDS char* cur, int wi, int wj, int lane, bool want_sum,
+                                            f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    u32x4 fa[TI], fb[TJ];
+#pragma unroll
+    for (int u = 0; u < TI; ++u) fa[u] = OA::frag(cur, (wi * TI + u) * 32, q, lane);
+#pragma unroll
+    for (int v = 0; v < TJ; ++v) fb[v] = OB::frag(cur + OA::BYTES, (wj * TJ + v) * 32, q, lane);
+#pragma unroll
+    for (int u = 0; u < TI; ++u)
+#pragma unroll
+      for (int v = 0; v < TJ; ++v) acc[u][v] = vql_mma<T>(fb[v], fa[u], acc[u][v]);
+    if (OA::SUMS && want_sum) {
+#pragma unroll
+      for (int u = 0; u < TI; ++u) asum[u] += vql_sum16<T>(fa[u]);
+    }
+  }
+}
+// The same with the DMA of the next step issued first.  __restrict__ (the two buffers are different ones) tells the
+// compiler that the fragment reads need not wait for the DMA.
+template <typename T, typename OA, typename OB, int TI, int TJ>
+__device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t next, bool more, VQL_LDS char* __restrict__ nxt,
+                                         const VQL_LDS char* __restrict__ cur, int wi, int wj, int wave, int lane,
+                                         bool want_sum, f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
+  if (more) {
+    oa.dma(next, nxt, wave);
+    ob.dma(next, nxt + OA::BYTES, wave);
+  }
+  vql_compute<T, OA, OB, TI, TJ>(cur, wi, wj, lane, want_sum, acc, asum);
+}
+
+// -------------------------------------------------------------------------------- the product
+namespace {   // the kernels of a translation unit are its own
+// A workgroup of WI x WJ waves owns a BI x BJ block of C (and, with splits, a range of the sum); a wave owns
+// (BI / WI) x (BJ / WJ) of it in 32x32 accumulator tiles.  Both operand tiles of a 128-byte step lie in one of two LDS
+// buffers, filled for the next step while the matrix cores work on this one: by DMA where rows start on 16 bytes,
+// else through registers.  One barrier a step.
+template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, bool DMA>
+__global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_product_kernel(VqLinearArgs a) {
+  constexpr int NT = WI * WJ * 64;
+  constexpr int TI = BI / WI / 32, TJ = BJ / WJ / 32;
+  constexpr int STAGE = (BI + BJ) * 128;
+  typedef VqOperand<T, AMM, BI, NT, DMA> OA;
+  typedef VqOperand<T, BMM, BJ, NT, DMA> OB;
+  extern __shared__ __attribute__((aligned(16))) char vql_lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = wave / WJ, wj = wave % WJ;
+
+  // Consecutive workgroups go to the 8 dies in turn: give each die a contiguous range of blocks, and walk the range in
+  // groups of 8 block rows, so that the blocks in flight on a die share their operands in its L2.
+  const int64_t per_split = a.tiles_i * a.tiles_j;
+  const int64_t total = per_split * a.splits;
+  const int64_t bid = blockIdx.x;
+  const int64_t q8 = total >> 3, r8 = total & 7, x8 = bid & 7;
+  int64_t id = x8 * q8 + (x8 < r8 ? x8 : r8) + (bid >> 3);
+  const int split = (int)(id / per_split);
+  id -= split * per_split;
+  const int64_t group = id / (8 * (int64_t)a.tiles_j);
+  const int64_t first = group * 8;
+  const int64_t gsz = a.tiles_i - first < 8 ? a.tiles_i - first : 8;
+  id -= group * 8 * a.tiles_j;
+  const int64_t ti0 = first + id % gsz;
+  const int tj0 = (int)(id / gsz);
+  const int64_t i0 = ti0 * BI;
+  const int64_t j0 = (int64_t)tj0 * BJ;
+
+  const int64_t steps = (a.R + OA::BK - 1) / OA::BK;
+  const int64_t full = a.R / OA::BK;
+  const int64_t s0 = split * a.steps_per_split;
+  const int64_t s1 = s0 + a.steps_per_split < steps ? s0 + a.steps_per_split : steps;
+
+  OA oa;
+  OB ob;
+  oa.init(a.A, a.lda, i0, a.I, wave, lane);
+  ob.init(a.B, a.ldb, j0, a.J, wave, lane);
+
+  f32x16 acc[TI][TJ];
+#pragma unroll
+  for (int u = 0; u < TI; ++u)
+#pragma unroll
+    for (int v = 0; v < TJ; ++v)
+#pragma unroll
+      for (int g = 0; g < 16; ++g) acc[u][v][g] = 0.0f;
+  const bool want_sum = AMM && a.asum && tj0 == 0 && wj == 0;
+  float asum[TI];
+#pragma unroll
+  for (int u = 0; u < TI; ++u) asum[u] = 0.0f;
+
+  auto by_registers = [&](int64_t s, VQL_LDS char* buf) {
+    u32x4 va[OA::PER], vb[OB::PER];
+    oa.fetch(s, a.R, wave, lane, va);
+    ob.fetch(s, a.R, wave, lane, vb);
+    oa.commit(buf, wave, lane, va);
+    ob.commit(buf + OA::BYTES, wave, lane, vb);
+  };
+  auto publish = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): this wave's DMA and LDS writes have landed
+    __syncthreads();
+  };
+  VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
+  if (s0 < s1) {
+    if (DMA && s0 < full) {
+      oa.dma(s0, lds, wave);
+      ob.dma(s0, lds + OA::BYTES, wave);
+    } else {
+      by_registers(s0, lds);
+    }
+  }
+  publish();
+  int cur = 0;
+  for (int64_t s = s0; s < s1; ++s) {
+    VQL_LDS char* buf = lds + cur * STAGE;
+    VQL_LDS char* nxt = lds + (cur ^ 1) * STAGE;
+    if constexpr (DMA) {
+      const bool more = s + 1 < s1 && s + 1 < full;
+      vql_step<T, OA, OB, TI, TJ>(oa, ob, s + 1, more, nxt, buf, wi, wj, wave, lane, want_sum, acc, asum);
+      if (s + 1 < s1 && s + 1 >= full) by_registers(s + 1, nxt);
+    } else {
+      u32x4 va[OA::PER], vb[OB::PER];
+      if (s + 1 < s1) {
+        oa.fetch(s + 1, a.R, wave, lane, va);
+        ob.fetch(s + 1, a.R, wave, lane, vb);
+      }
+      vql_compute<T, OA, OB, TI, TJ>(buf, wi, wj, lane, want_sum, acc, asum);
+      if (s + 1 < s1) {
+        oa.commit(nxt, wave, lane, va);
+        ob.commit(nxt + OA::BYTES, wave, lane, vb);
+      }
+    }
+    publish();
+    cur ^= 1;
+  }
+
+  if (AMM && want_sum) {
+#pragma unroll
+    for (int u = 0; u < TI; ++u) {
+      const float s = asum[u] + __shfl_xor(asum[u], 32);
+      const int64_t i = i0 + (wi * TI + u) * 32 + (lane & 31);
+      if (lane < 32 && i < a.I) a.asum[split * a.I + i] = s;
+    }
+  }
+
+  // The accumulators hold 4 consecutive columns of one row per lane; through LDS (this wave's own part, 32 rows at a
+  // time) they become 16-byte pieces of rows, so that loads and stores of the epilogue are whole lines.
+  constexpr int PITCH = TJ * 32 + 4;
+  float* st = reinterpret_cast<float*>(vql_lds) + wave * 32 * PITCH;
+  const int64_t jw = j0 + wj * TJ * 32;
+#pragma unroll
+  for (int u = 0; u < TI; ++u) {
+#pragma unroll
+    for (int v = 0; v < TJ; ++v)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 w = {acc[u][v][4 * g], acc[u][v][4 * g + 1], acc[u][v][4 * g + 2], acc[u][v][4 * g + 3]};
+        *reinterpret_cast<vql_f32x4*>(st + (lane & 31) * PITCH + v * 32 + 8 * g + 4 * (lane >> 5)) = w;
+      }
+    __builtin_amdgcn_wave_barrier();
+    const int64_t iw = i0 + (wi * TI + u) * 32;
+    if (a.splits > 1) {
+      constexpr int LPR = TJ * 8;
+#pragma unroll
+      for (int n = 0; n < 32 * LPR / 64; ++n) {
+        const int row = n * (64 / LPR) + lane / LPR, col = (lane % LPR) * 4;
+        const f32x4 w = *reinterpret_cast<const vql_f32x4*>(st + row * PITCH + col);
+        if (iw + row < a.I && jw + col < a.ldp)
+          *reinterpret_cast<vql_f32x4*>(a.part + ((int64_t)split * a.I + iw + row) * a.ldp + jw + col) = w;
+      }
+    } else {
+      constexpr int E = 16 / sizeof(T), LPR = TJ * 32 / E;
+      const int col = (lane % LPR) * E;
+      float bias[E];
+      vql_bias16<T>(a, (int)jw + col, bias);
+#pragma unroll
+      for (int n = 0; n < 32 * LPR / 64; ++n) {
+        const int row = n * (64 / LPR) + lane / LPR;
+        float c[E];
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          const f32x4 w = *reinterpret_cast<const vql_f32x4*>(st + row * PITCH + col + e);
+          c[e] = w[0]; c[e + 1] = w[1]; c[e + 2] = w[2]; c[e + 3] = w[3];
+        }
+        if (iw + row < a.I && jw + col < a.J) vql_epilogue<T>(a, iw + row, (int)jw + col, c, bias);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+}  // namespace
+
+// Launches the product of one element type: layout 0 = forward, 1 = input gradient, 2 = weight gradient.
+int vql_product_f32(const VqLinearArgs& a, int layout, int config, bool dma, hipStream_t s);
+int vql_product_bf16(const VqLinearArgs& a, int layout, int config, bool dma, hipStream_t s);
+int vql_product_f16(const VqLinearArgs& a, int layout, int config, bool dma, hipStream_t s);
+
+namespace {
+// One kernel of the family: its entry in the table of kernels with large LDS, and its launch.
+template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, bool DMA>
+struct VqProduct {
+  static constexpr int LDS = 2 * (BI + BJ) * 128;
+  static_assert(LDS >= WI * WJ * 32 * (BJ / WJ + 4) * 4, "the epilogue's staging fits the stage buffers");
+  static const void* address() { return reinterpret_cast<const void*>(&vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, DMA>); }
+  static inline VqLdsRegistrar registrar{address(), LDS};
+  static int launch(const VqLinearArgs& a, hipStream_t s) {
+    (void)&registrar;
+    const int rc = vq_lds_ensure(address(), LDS, nullptr);
+    if (rc != VQ_OK) return rc;
+    const int64_t blocks = a.tiles_i * a.tiles_j * a.splits;
+    hipLaunchKernelGGL((vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, DMA>), dim3((unsigned)blocks), dim3(WI * WJ * 64), LDS, s, a);
+    return vq_hip_status(hipGetLastError());
+  }
+};
+template <typename T, bool AMM, bool BMM>
+int vql_launch_layout(const VqLinearArgs& a, int config, bool dma, hipStream_t s) {
+  if (config == VQL_C256) return dma ? VqProduct<T, AMM, BMM, 256, 256, 2, 4, true>::launch(a, s) : VQ_ERR_INVALID_ARG;
+  if (config == VQL_C128)
+    return dma ? VqProduct<T, AMM, BMM, 128, 128, 2, 2, true>::launch(a, s) : VqProduct<T, AMM, BMM, 128, 128, 2, 2, false>::launch(a, s);
+  return dma ? VqProduct<T, AMM, BMM, 64, 64, 2, 2, true>::launch(a, s) : VqProduct<T, AMM, BMM, 64, 64, 2, 2, false>::launch(a, s);
+}
+template <typename T>
+int vql_product(const VqLinearArgs& a, int layout, int config, bool dma, hipStream_t s) {
+  if (layout == 0) return vql_launch_layout<T, false, false>(a, config, dma, s);
+  if (layout == 1) return vql_launch_layout<T, false, true>(a, config, dma, s);
+  return vql_launch_layout<T, true, true>(a, config, dma, s);
+}
+}  // namespace
+
+// The kernels of one element type (the compiler's host pass leaves kernels out that it meets only through VqProduct).
+#define VQL_KERNELS_OF(T, AMM, BMM)                                                       \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 256, 256, 2, 4, true>(VqLinearArgs);  \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, true>(VqLinearArgs);  \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, false>(VqLinearArgs); \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, true>(VqLinearArgs);    \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, false>(VqLinearArgs);
+#define VQL_KERNELS(T)           \
+  namespace {                    \
+  VQL_KERNELS_OF(T, false, false) \
+  VQL_KERNELS_OF(T, false, true) \
+  VQL_KERNELS_OF(T, true, true)  \
+  }

@@ -1,0 +1,417 @@
+// Entry points of the product with bias, activation and residual and of its backward pass, and their kernels beside
+// the tiled product of vq_linear.h: the product of a few rows, the join of a split sum, the activation's gradient and
+// column sums.
+#include <algorithm>
+
+#include "vq_linear.h"
+
+namespace {
+
+// ------------------------------------------------------------------------------ a few rows
+// Up to 16 rows: the product is bound by reading W once.  A workgroup owns 16 output channels, its waves share out the
+// sum; a wave reads W straight into the fragments of a 16x16 product (lane l: channel l % 16, 16 bytes at piece l / 16
+// of a 64-byte step, so consecutive steps of one channel are consecutive lines), eight steps in flight, with x, which
+// stays in the L2, in the other operand.  The waves' partial products are added in LDS in wave order.
+constexpr int ROWS_MAX = 16;
+constexpr int ROWS_UNROLL = 8;
+
+template <typename T>
+__device__ __forceinline__ f32x4 rows_mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (__is_same(T, VqBf16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else if constexpr (__is_same(T, _Float16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else {
+    const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[e], fb[e], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// One element of the epilogue (vql_epilogue does 16 bytes of them).
+template <typename T>
+__device__ __forceinline__ void epilogue_one(const VqLinearArgs& a, int64_t i, int j, float c) {
+  if (a.bias) c += VqElem<T>::to(reinterpret_cast<const T*>(a.bias)[j]);
+  if (a.pre) reinterpret_cast<T*>(a.pre)[i * a.J + j] = VqElem<T>::from(c);
+  c = vql_act<sizeof(T) == 2>(c, a.act);
+  if (a.res) c += VqElem<T>::to(reinterpret_cast<const T*>(a.res + i * a.ldr)[j]);
+  reinterpret_cast<T*>(a.out)[i * a.J + j] = VqElem<T>::from(c);
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void vql_rows_kernel(VqLinearArgs a) {
+  constexpr int E = 16 / sizeof(T), KS = 4 * E;   // elements of the sum per step
+  __shared__ float part[16][16 * 20];             // [wave][row][channel, padded]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int split = blockIdx.y;
+  const int sub = lane & 15, piece = lane >> 4;
+  const int64_t n = n0 + sub < a.J ? n0 + sub : a.J - 1;
+  const int64_t m = sub < a.I ? sub : a.I - 1;    // rows and channels that do not exist repeat the last one, unstored
+  const char* wp = a.B + n * a.ldb + piece * 16;
+  const char* xp = a.A + m * a.lda + piece * 16;
+  const int64_t steps = (a.R + KS - 1) / KS, full = a.R / KS;
+  // this workgroup's range of the sum, then this wave's
+  const int64_t g0 = split * a.steps_per_split;
+  const int64_t g1 = g0 + a.steps_per_split < steps ? g0 + a.steps_per_split : steps;
+  const int64_t per = (g1 - g0 + waves - 1) / waves;
+  int64_t s = g0 + wave * per;
+  const int64_t s1 = s + per < g1 ? s + per : g1;
+  const int64_t sf = s1 < full ? s1 : full;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (; s + ROWS_UNROLL <= sf; s += ROWS_UNROLL) {
+    u32x4 w[ROWS_UNROLL], x[ROWS_UNROLL];
+#pragma unroll
+    for (int u = 0; u < ROWS_UNROLL; ++u) w[u] = vql_load16<T>(wp + (s + u) * 64);
+#pragma unroll
+    for (int u = 0; u < ROWS_UNROLL; ++u) x[u] = vql_load16<T>(xp + (s + u) * 64);
+#pragma unroll
+    for (int u = 0; u < ROWS_UNROLL; ++u) acc = rows_mma<T>(w[u], x[u], acc);
+  }
+  for (; s < s1; ++s) {
+    const int64_t valid = a.R - s * KS - piece * E;
+    acc = rows_mma<T>(vql_load16_part<T>(wp + s * 64, valid), vql_load16_part<T>(xp + s * 64, valid), acc);
+  }
+  *reinterpret_cast<vql_f32x4*>(&part[wave][sub * 20 + 4 * piece]) = acc;   // row `sub`, channels 4 piece ..
+  __syncthreads();
+  for (int t = threadIdx.x; t < 256; t += blockDim.x) {
+    const int row = t >> 4, col = t & 15;
+    if (row >= a.I || n0 + col >= a.J) continue;
+    float c = 0.0f;
+    for (int w = 0; w < waves; ++w) c += part[w][row * 20 + col];
+    if (a.splits > 1) a.part[((int64_t)split * a.I + row) * a.ldp + n0 + col] = c;
+    else epilogue_one<T>(a, row, (int)(n0 + col), c);
+  }
+}
+
+// ------------------------------------------------------------------------------ join of a split sum
+// Adds the partial sums in split order (the same bits on every run) and applies the epilogue.
+template <typename T>
+__global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a) {
+  constexpr int E = 16 / sizeof(T);
+  const int64_t cols = (a.J + E - 1) / E;
+  const int64_t count = a.I * cols;
+  const int64_t size = a.I * a.ldp;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < count; t += (int64_t)gridDim.x * 256) {
+    const int64_t i = t / cols;
+    const int j = (int)(t - i * cols) * E;
+    float c[E], bias[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) c[e] = 0.0f;
+    const float* p = a.part + i * a.ldp + j;
+    for (int s = 0; s < a.splits; ++s, p += size) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const f32x4 v = *reinterpret_cast<const vql_f32x4*>(p + e);
+        c[e] += v[0]; c[e + 1] += v[1]; c[e + 2] += v[2]; c[e + 3] += v[3];
+      }
+    }
+    vql_bias16<T>(a, j, bias);
+    vql_epilogue<T>(a, i, j, c, bias);
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, int splits, int64_t n, T* out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float c = 0.0f;
+  for (int s = 0; s < splits; ++s) c += part[s * n + i];
+  out[i] = VqElem<T>::from(c);
+}
+
+// ------------------------------------------------------------------------------ activation's gradient
+// dp = gy * act'(pre), rounded to T: the operand of both products of the backward pass.
+template <typename T>
+__global__ __launch_bounds__(256) void vql_act_grad_kernel(const T* gy, const T* pre, int act, int64_t count, T* dp) {
+  constexpr int E = 16 / sizeof(T);
+  const int64_t vecs = count / E, stride = (int64_t)gridDim.x * 256;
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < vecs; v += stride) {
+    const VqChunk<T> g = __builtin_bit_cast(VqChunk<T>, vql_load16<T>(reinterpret_cast<const char*>(gy + v * E)));
+    const VqChunk<T> p = __builtin_bit_cast(VqChunk<T>, vql_load16<T>(reinterpret_cast<const char*>(pre + v * E)));
+    VqChunk<T> d;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      d.e[e] = VqElem<T>::from(VqElem<T>::to(g.e[e]) * vql_act_slope<sizeof(T) == 2>(VqElem<T>::to(p.e[e]), act));
+    vql_store16<T>(dp + v * E, __builtin_bit_cast(u32x4, d));
+  }
+  const int64_t at = vecs * E + (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at < count)
+    dp[at] = VqElem<T>::from(VqElem<T>::to(gy[at]) * vql_act_slope<sizeof(T) == 2>(VqElem<T>::to(pre[at]), act));
+}
+
+// ------------------------------------------------------------------------------ column sums
+// The bias gradient where no weight gradient is wanted (which carries it along): 64 columns and a range of rows per
+// workgroup, four rows at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void vql_colsum_kernel(const T* g, int64_t M, int N, int64_t rows_per, float* part) {
+  __shared__ float s[4][64];
+  const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  const int64_t m0 = blockIdx.y * rows_per, m1 = m0 + rows_per < M ? m0 + rows_per : M;
+  float sum = 0.0f;
+  if (col < N)
+    for (int64_t m = m0 + r; m < m1; m += 4) sum += VqElem<T>::to(g[m * N + col]);
+  s[r][c] = sum;
+  __syncthreads();
+  if (r == 0 && col < N) part[(int64_t)blockIdx.y * N + col] = (s[0][c] + s[1][c]) + (s[2][c] + s[3][c]);
+}
+
+// ------------------------------------------------------------------------------ choice of tile and split
+struct Plan {
+  bool rows;       // the few-rows kernel
+  int config;
+  int splits;
+  int64_t steps_per_split;
+  int64_t tiles_i;
+  int tiles_j;
+  int ldp;
+};
+
+constexpr int CUS = 256;
+
+size_t elem_size(int dtype) { return dtype == VQ_F32 ? 4 : 2; }
+
+// The cheapest of the three tiles, each with its best split of the sum, by a model of the launch: rounds of
+// workgroups x (steps of the sum x time of a step + what a workgroup pays once), plus the join of a split sum.
+// Times in microseconds, measured on an MI355X (step: 128 bytes of the sum).
+Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
+  const size_t es = elem_size(dtype);
+  Plan best{};
+  best.ldp = (J + 7) & ~7;
+  if (layout == 0 && I <= ROWS_MAX) {
+    best.rows = true;
+    const int64_t steps = (R * es + 63) / 64, groups = (J + 15) / 16;
+    // a workgroup's 16 waves take 8 steps each before a second round; the join costs more than 32 steps a wave
+    int64_t splits = 1;
+    if (groups * 4 <= CUS && steps > 16 * 32) splits = std::min<int64_t>((steps + 16 * 16 - 1) / (16 * 16), CUS / groups);
+    best.steps_per_split = (steps + splits - 1) / splits;
+    best.splits = (int)((steps + best.steps_per_split - 1) / best.steps_per_split);
+    return best;
+  }
+  static const struct { int tile, per_cu; double step16, step32, once; } cfg[3] = {
+      {64, 4, 0.30, 0.60, 2.0}, {128, 2, 0.50, 1.60, 3.0}, {256, 1, 0.90, 3.60, 6.0}};
+  const int64_t steps = (R * es + 127) / 128;
+  double best_t = 1e300;
+  for (int c = dma ? 2 : 1; c >= 0; --c) {
+    const int64_t ti = (I + cfg[c].tile - 1) / cfg[c].tile, tj = (J + cfg[c].tile - 1) / cfg[c].tile;
+    const int64_t slots = (int64_t)CUS * cfg[c].per_cu;
+    const double step = es == 2 ? cfg[c].step16 : cfg[c].step32;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 4, 2 * slots / std::max<int64_t>(1, ti * tj)));
+    for (int64_t s = 1; s <= most; s = s < 8 ? s + 1 : s + s / 8) {
+      const int64_t per = (steps + s - 1) / s, sp = steps ? (steps + per - 1) / per : 1;
+      const int64_t rounds = (ti * tj * sp + slots - 1) / slots;
+      double t = rounds * (per * step + cfg[c].once);
+      if (sp > 1) t += 4.0 + (double)I * J * 4 * (2 * sp + 1) / 4.0e6;   // partial sums written and read at 4 TB/s
+      if (t < best_t) {
+        best_t = t;
+        best.config = c;
+        best.splits = (int)sp;
+        best.steps_per_split = per;
+        best.tiles_i = ti;
+        best.tiles_j = (int)tj;
+      }
+    }
+  }
+  return best;
+}
+
+int64_t part_bytes(const Plan& p, int64_t I) {
+  return p.splits > 1 ? (int64_t)p.splits * I * p.ldp * 4 : 0;
+}
+// row slabs of vql_colsum_kernel
+int64_t colsum_slabs(int64_t M, int N) {
+  const int64_t groups = (N + 63) / 64;
+  return std::max<int64_t>(1, std::min<int64_t>((M + 63) / 64, std::max<int64_t>(1, 4 * CUS / groups)));
+}
+
+bool bad_sizes(int64_t M, int K, int N) { return M < 0 || K <= 0 || N <= 0; }
+bool known(int dtype) { return dtype == VQ_F32 || dtype == VQ_BF16 || dtype == VQ_F16; }
+constexpr int MAX_DIM = 1 << 20;
+constexpr int64_t MAX_ROWS = (int64_t)1 << 31;
+bool pitch_too_wide(int64_t ld, size_t es) { return ld * (int64_t)es > 0x7fffffff / 256 - 128; }
+
+int product(const VqLinearArgs& a, int layout, int dtype, int config, bool dma, hipStream_t s) {
+  if (dtype == VQ_F32) return vql_product_f32(a, layout, config, dma, s);
+  if (dtype == VQ_BF16) return vql_product_bf16(a, layout, config, dma, s);
+  return vql_product_f16(a, layout, config, dma, s);
+}
+
+template <template <typename> class F, typename... Args>
+int by_type(int dtype, Args&&... args) {
+  if (dtype == VQ_F32) return F<float>::run(args...);
+  if (dtype == VQ_BF16) return F<VqBf16>::run(args...);
+  return F<_Float16>::run(args...);
+}
+template <typename T> struct RunRows {
+  static int run(const VqLinearArgs& a, hipStream_t s) {
+    const int64_t steps = std::min<int64_t>(a.steps_per_split, (a.R * (int64_t)sizeof(T) + 63) / 64);
+    int waves = 1;
+    while (waves < 16 && waves * 2 < steps) waves *= 2;   // two steps or more a wave
+    if (waves < 4) waves = 4;                             // four waves write the 256 results
+    hipLaunchKernelGGL(vql_rows_kernel<T>, dim3((unsigned)((a.J + 15) / 16), (unsigned)a.splits), dim3(waves * 64), 0, s, a);
+    return vq_hip_status(hipGetLastError());
+  }
+};
+template <typename T> struct RunJoin {
+  static int run(const VqLinearArgs& a, hipStream_t s) {
+    constexpr int E = 16 / sizeof(T);
+    const int64_t blocks = std::min<int64_t>((a.I * ((a.J + E - 1) / E) + 255) / 256, 8192);
+    hipLaunchKernelGGL(vql_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    return vq_hip_status(hipGetLastError());
+  }
+};
+template <typename T> struct RunJoinSums {
+  static int run(const float* part, int splits, int64_t n, void* out, hipStream_t s) {
+    hipLaunchKernelGGL(vql_join_sums_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, splits, n,
+                       reinterpret_cast<T*>(out));
+    return vq_hip_status(hipGetLastError());
+  }
+};
+template <typename T> struct RunActGrad {
+  static int run(const void* gy, const void* pre, int act, int64_t count, void* dp, hipStream_t s) {
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((count / (16 / sizeof(T)) + 255) / 256, 16384));
+    hipLaunchKernelGGL(vql_act_grad_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, reinterpret_cast<const T*>(gy),
+                       reinterpret_cast<const T*>(pre), act, count, reinterpret_cast<T*>(dp));
+    return vq_hip_status(hipGetLastError());
+  }
+};
+template <typename T> struct RunColsum {
+  static int run(const void* g, int64_t M, int N, int64_t slabs, float* part, hipStream_t s) {
+    const int64_t per = (M + slabs - 1) / slabs;
+    hipLaunchKernelGGL(vql_colsum_kernel<T>, dim3((unsigned)((N + 63) / 64), (unsigned)slabs), dim3(256), 0, s,
+                       reinterpret_cast<const T*>(g), M, N, per, part);
+    return vq_hip_status(hipGetLastError());
+  }
+};
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Runs one of the three products with its epilogue; `gbias` (weight gradient) receives the sums of A.
+int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, void* work, hipStream_t s) {
+  const int64_t es = (int64_t)elem_size(dtype);
+  const int E = (int)(16 / es);
+  bool dma = aligned16(a.A) && aligned16(a.B) && a.lda % 16 == 0 && a.ldb % 16 == 0;
+  if (layout == 1 && a.J % E) dma = false;                 // a piece of an m-major operand must not pass its row's end
+  if (layout == 2 && (a.I % E || a.J % E)) dma = false;
+  const Plan p = make_plan(layout, a.I, a.J, a.R, dtype, dma);
+  a.splits = p.splits;
+  a.steps_per_split = p.steps_per_split;
+  a.tiles_i = p.tiles_i;
+  a.tiles_j = p.tiles_j;
+  a.ldp = p.ldp;
+  if (p.splits > 1) {
+    if (!work || !aligned16(work)) return VQ_ERR_INVALID_ARG;
+    a.part = reinterpret_cast<float*>(work);
+  }
+  if (p.rows) {
+    int rc = by_type<RunRows>(dtype, a, s);
+    if (rc == VQ_OK && a.splits > 1) rc = by_type<RunJoin>(dtype, a, s);
+    return rc;
+  }
+  if (p.tiles_i * p.tiles_j * p.splits >= (int64_t)1 << 23) return VQ_ERR_UNSUPPORTED;
+  if (gbias) {
+    if (!work) return VQ_ERR_INVALID_ARG;
+    a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p, a.I));
+  }
+  int rc = product(a, layout, dtype, p.config, dma, s);
+  if (rc == VQ_OK && a.splits > 1) rc = by_type<RunJoin>(dtype, a, s);
+  if (rc == VQ_OK && gbias) rc = by_type<RunJoinSums>(dtype, (const float*)a.asum, a.splits, a.I, gbias, s);
+  return rc;
+}
+
+int64_t product_work(int layout, int64_t I, int J, int64_t R, int dtype, bool sums) {
+  int64_t bytes = 0;
+  for (int dma = 0; dma < 2; ++dma) {
+    const Plan p = make_plan(layout, I, J, R, dtype, dma);
+    bytes = std::max(bytes, part_bytes(p, I) + (sums ? (int64_t)p.splits * I * 4 : 0));
+  }
+  return bytes;
+}
+
+}  // namespace
+
+extern "C" int64_t vq_linear_work_bytes(int pass, int64_t M, int K, int N, int dtype) {
+  if (bad_sizes(M, K, N) || K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || !known(dtype) || pass < 0 || pass > 2) return 0;
+  if (pass == VQ_LINEAR_FORWARD) return product_work(0, M, N, K, dtype, false);
+  if (pass == VQ_LINEAR_DGRAD) return product_work(1, M, K, N, dtype, false);
+  return std::max(product_work(2, N, K, M, dtype, true), colsum_slabs(M, N) * N * 4);
+}
+
+extern "C" int vq_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* residual,
+                         int64_t ldr, int dtype, int act, int64_t M, int K, int N, void* y, void* pre, void* work,
+                         void* stream) {
+  if (bad_sizes(M, K, N) || !known(dtype) || act < VQ_ACT_NONE || act > VQ_ACT_GELU_TANH) return VQ_ERR_INVALID_ARG;
+  if (ldx < K || ldw < K || (residual && ldr < N)) return VQ_ERR_INVALID_ARG;
+  if (M == 0) return VQ_OK;
+  if (!x || !W || !y) return VQ_ERR_INVALID_ARG;
+  const size_t es = elem_size(dtype);
+  if (K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || pitch_too_wide(ldx, es) || pitch_too_wide(ldw, es)) return VQ_ERR_UNSUPPORTED;
+  VqLinearArgs a{};
+  a.A = reinterpret_cast<const char*>(x);
+  a.B = reinterpret_cast<const char*>(W);
+  a.lda = ldx * es;
+  a.ldb = ldw * es;
+  a.I = M;
+  a.J = N;
+  a.R = K;
+  a.out = y;
+  a.pre = pre;
+  a.bias = bias;
+  a.res = reinterpret_cast<const char*>(residual);
+  a.ldr = ldr * es;
+  a.act = act;
+  return run_product(0, a, dtype, nullptr, work, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int vq_linear_act_grad(const void* gy, const void* pre, int dtype, int act, int64_t count, void* dp, void* stream) {
+  if (count < 0 || !known(dtype) || act <= VQ_ACT_NONE || act > VQ_ACT_GELU_TANH) return VQ_ERR_INVALID_ARG;
+  if (count == 0) return VQ_OK;
+  if (!gy || !pre || !dp) return VQ_ERR_INVALID_ARG;
+  return by_type<RunActGrad>(dtype, gy, pre, act, count, dp, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int vq_linear_dgrad(const void* dp, const void* W, int64_t ldw, int dtype, int64_t M, int K, int N, void* gx,
+                               void* work, void* stream) {
+  if (bad_sizes(M, K, N) || !known(dtype) || ldw < K) return VQ_ERR_INVALID_ARG;
+  if (M == 0) return VQ_OK;
+  if (!dp || !W || !gx) return VQ_ERR_INVALID_ARG;
+  const size_t es = elem_size(dtype);
+  if (K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || pitch_too_wide(N, es) || pitch_too_wide(ldw, es)) return VQ_ERR_UNSUPPORTED;
+  VqLinearArgs a{};
+  a.A = reinterpret_cast<const char*>(dp);
+  a.B = reinterpret_cast<const char*>(W);
+  a.lda = N * es;
+  a.ldb = ldw * es;
+  a.I = M;
+  a.J = K;
+  a.R = N;
+  a.out = gx;
+  return run_product(1, a, dtype, nullptr, work, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int vq_linear_wgrad(const void* dp, const void* x, int64_t ldx, int dtype, int64_t M, int K, int N, void* gW,
+                               void* gbias, void* work, void* stream) {
+  if (bad_sizes(M, K, N) || !known(dtype) || ldx < K || (!gW && !gbias)) return VQ_ERR_INVALID_ARG;
+  if (M > 0 && (!dp || (gW && !x))) return VQ_ERR_INVALID_ARG;
+  const size_t es = elem_size(dtype);
+  if (K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || pitch_too_wide(N, es) || pitch_too_wide(ldx, es)) return VQ_ERR_UNSUPPORTED;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (!gW) {
+    if (!work) return VQ_ERR_INVALID_ARG;
+    const int64_t slabs = colsum_slabs(M, N);
+    float* part = reinterpret_cast<float*>(work);
+    const int rc = by_type<RunColsum>(dtype, dp, M, N, slabs, part, s);
+    return rc != VQ_OK ? rc : by_type<RunJoinSums>(dtype, (const float*)part, (int)slabs, (int64_t)N, gbias, s);
+  }
+  VqLinearArgs a{};
+  a.A = reinterpret_cast<const char*>(dp);
+  a.B = reinterpret_cast<const char*>(x);
+  a.lda = N * es;
+  a.ldb = ldx * es;
+  a.I = N;
+  a.J = K;
+  a.R = M;
+  a.out = gW;
+  return run_product(2, a, dtype, gbias, work, s);
+}

@@ -1,0 +1,209 @@
+"""The global gradient norm over many tensors, and clipping by it.
+
+What a trainer does between ``backward`` and the optimizer's step (vqvae/vqgan_trainer.py:98-104 for the parameters of the
+model this quantizer sits in): a few launches over all gradients of a model instead of a few per tensor, nothing copied
+to the host.  GPU only.
+"""
+from __future__ import annotations
+
+import math
+from typing import Iterable, List, Optional, Sequence, Union
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import NORM_1, NORM_2, NORM_INF, check
+from .projection import DTYPES
+from .ops import _on_device, _ptr, _require_cuda, _stream
+
+_KINDS = {1.0: NORM_1, 2.0: NORM_2, math.inf: NORM_INF}
+
+
+def _kind(norm_type) -> int:
+    kind = _KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
+    return kind
+
+
+def _max_norm(max_norm) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    return max_norm
+
+
+def _list(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], name: str) -> List[torch.Tensor]:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be tensors, got {type(t).__name__}")
+    kinds = {(t.dtype, t.layout, t.device) for t in tensors}       # a model has a few, however many tensors it has
+    for dtype, layout, _ in kinds:
+        if layout is not torch.strided:
+            raise TypeError(f"{name} must be dense tensors, got {layout}")
+        if dtype not in DTYPES:
+            raise TypeError(f"{name} must be float32, bfloat16 or float16, got {dtype}")
+    devices = {device for _, _, device in kinds}
+    if len(devices) > 1:
+        raise ValueError(f"{name} must share one device, got {', '.join(sorted(map(str, devices)))}")
+    if len(tensors) > 65536:
+        raise ValueError(f"at most 65536 tensors in one call, got {len(tensors)}")
+    return tensors
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one run of memory, in whatever order (a transposed or channels_last tensor does)."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _refs(srcs: Sequence[torch.Tensor], dsts: Sequence[torch.Tensor]) -> np.ndarray:
+    """The vq_tensor_ref array of the C interface: four 64-bit words an entry."""
+    refs = np.empty((len(srcs), 4), np.int64)
+    refs[:, 0] = [t.data_ptr() for t in srcs]
+    refs[:, 2] = [t.numel() for t in srcs]
+    refs[:, 3] = [DTYPES[t.dtype] for t in srcs]
+    if dsts is srcs:
+        refs[:, 1] = refs[:, 0]
+        refs[:, 3] *= (1 << 32) + 1
+    else:
+        refs[:, 1] = [t.data_ptr() for t in dsts]
+        refs[:, 3] += [DTYPES[t.dtype] << 32 for t in dsts]
+    return refs
+
+
+def _refuse_overlap(tensors: Sequence[torch.Tensor]) -> None:
+    """Raises where two of the tensors share memory: a kernel over all of them would race with itself.  Tensors with gaps
+    (columns of one matrix) count from their first to their last element."""
+    runs = [(t.data_ptr(), t.numel() * t.element_size() if t.is_contiguous() else
+             (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()) for t in tensors if t.numel()]
+    runs.sort()
+    end = 0
+    for start, size in runs:
+        if start < end:
+            raise ValueError("gradients that are to be scaled share memory: each may be given once")
+        end = start + size
+
+
+def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all elements of all tensors together, a float32 scalar on their device.
+
+    grads: float32, bfloat16 and float16 tensors, mixed as they come, of any shape and strides, on one GPU.  norm_type: 1, 2
+    or inf.  Summed in 64 bits.  NaN and infinity come through as the formula has them.  No tensor at all: 0 (on the
+    host).  The same bits on every run; may be captured in a graph."""
+    kind = _kind(norm_type)
+    grads = _list(grads, "grads")
+    if not grads:
+        return torch.zeros(())
+    _require_cuda(grads[0], "grads")
+    lib = _lib.load()
+    device = grads[0].device
+    with _on_device(device):
+        flat = [t if _dense(t) else t.contiguous() for t in grads]
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        work = torch.empty(lib.vq_grad_norm_work_bytes(len(flat)), dtype=torch.uint8, device=device)
+        refs = _refs(flat, flat)
+        check(lib.vq_grad_norm(refs.ctypes.data, len(flat), kind, _ptr(norm), _ptr(work), _stream(device)), "vq_grad_norm")
+    return norm
+
+
+def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+               out: Union[torch.Tensor, Sequence[torch.Tensor], None] = None) -> torch.Tensor:
+    """Scales the gradients by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm`` (see :func:`grad_norm`), without a
+    word to the host.
+
+    In place, or into ``out``: one tensor per gradient, of its shape and either its type or float32 (an optimizer's
+    gradients beside 16-bit ones); ``grads`` are then only read.  Every result is rounded once.  An infinite norm scales by
+    0 and a NaN by NaN, as the formula has it.  A tensor given twice, tensors that share memory, and expanded tensors to
+    be written are refused.  The same bits on every run; may be captured in a graph."""
+    kind = _kind(norm_type)
+    max_norm = _max_norm(max_norm)
+    grads = _list(grads, "grads")
+    if out is not None:
+        out = _list(out, "out")
+        if len(out) != len(grads):
+            raise ValueError(f"{len(grads)} gradients but {len(out)} tensors in out")
+        for g, o in zip(grads, out):
+            if o.shape != g.shape:
+                raise ValueError(f"out has shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
+            if o.dtype != g.dtype and o.dtype != torch.float32:
+                raise TypeError(f"out is {o.dtype} for a {g.dtype} gradient: the same type or float32")
+            if o.device != g.device:
+                raise ValueError(f"out is on {o.device}, the gradients on {g.device}")
+            if o.requires_grad and o.is_leaf and torch.is_grad_enabled():
+                raise ValueError("out requires a gradient itself")
+    if not grads:
+        return torch.zeros(())
+    written = grads if out is None else out
+    for t in written:
+        if not t.is_contiguous() and t.numel() and any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
+            raise ValueError("an expanded tensor cannot be scaled: several of its elements are one")
+    _refuse_overlap(grads if out is None else [t for pair in zip(grads, out) for t in _apart(*pair)])
+    _require_cuda(grads[0], "grads")
+    device = grads[0].device
+    with torch.no_grad(), _on_device(device):
+        srcs, dsts, back = _dense_pairs(grads, written)
+        lib = _lib.load()
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        work = torch.empty(lib.vq_grad_norm_work_bytes(len(srcs)), dtype=torch.uint8, device=device)
+        refs = _refs(srcs, dsts)
+        check(lib.vq_clip_grads(refs.ctypes.data, len(srcs), kind, max_norm, _ptr(norm), _ptr(work), _stream(device)),
+              "vq_clip_grads")
+        for o, c in back:
+            o.copy_(c)
+        torch.autograd.graph.increment_version([t for t in dsts if not t.is_inference()])
+    return norm
+
+
+def _dense_pairs(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]):
+    """What the kernel reads and writes: dense runs of the same element order, the tensors themselves wherever they are
+    that, copies otherwise; and the copies to be brought back, as (tensor, copy)."""
+    if all(t.is_contiguous() for t in grads) and (written is grads or all(t.is_contiguous() for t in written)):
+        return grads, written, []
+    srcs, dsts, back = [], [], []
+    for g, o in zip(grads, written):
+        if _dense(g) and o.stride() == g.stride():
+            srcs.append(g)
+            dsts.append(o)
+            continue
+        c = g.contiguous()
+        srcs.append(c)
+        if o is g:
+            dsts.append(c)
+            back.append((o, c))
+        elif o.is_contiguous():
+            dsts.append(o)
+        else:
+            dsts.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
+            back.append((o, dsts[-1]))
+    return srcs, dsts, back
+
+
+def _apart(src: torch.Tensor, dst: torch.Tensor):
+    """The memory a pair touches: one run where it is scaled in place, two otherwise."""
+    return (dst,) if src.data_ptr() == dst.data_ptr() and src.dtype == dst.dtype else (src, dst)
+
+
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` on :func:`clip_grads`: scales the ``grad`` of every parameter in place and returns
+    the norm they had.  Parameters without a gradient are passed over.  ``error_if_nonfinite`` raises RuntimeError, before
+    anything is scaled, if the norm is not finite (this is the one case that waits for the GPU)."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    _kind(norm_type)
+    _max_norm(max_norm)
+    if error_if_nonfinite and grads:
+        norm = grad_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, "
+                               "so it cannot be clipped.")
+    return clip_grads(grads, max_norm, norm_type)

@@ -7,6 +7,7 @@ of the reference's ``EMAVectorQuantizer.forward`` (vqvae/ema_vector_quantizer.py
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from dataclasses import dataclass, field
 from typing import Optional
 
@@ -23,6 +24,13 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _on_device(device):
+    """Makes `device` the current one for a launch; nothing where it is already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
 
 
 def _require_cuda(t: torch.Tensor, name: str) -> None:

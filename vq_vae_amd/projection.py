@@ -1,0 +1,189 @@
+"""Linear layers with bias, activation and residual in one kernel, with their gradients.
+
+The quantizer sits between two projections (vqvae/custom_vqgan.py:50-51); a model over its codes consists of them.
+``linear`` computes ``act(x W^T + b) + residual`` on the matrix cores in fp32, bf16 or fp16: sums in fp32, one rounding
+per output, no tensor in between.  For one to sixteen rows (a token, a few sequences answered together) a kernel bound by
+reading the weights takes over.  GPU only, like everything here: there is no fallback.
+"""
+from __future__ import annotations
+
+import functools
+from typing import Optional
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from ._lib import ACTIVATIONS, LINEAR_DGRAD, LINEAR_FORWARD, LINEAR_WGRAD, check
+from .ops import _on_device, _ptr, _require_cuda, _stream
+
+DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+#: the widest distance between two rows that the kernels address (bytes)
+_MAX_PITCH = 0x7fffffff // 256 - 128
+
+
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(which: int, M: int, K: int, N: int, dtype: int) -> int:
+    return _lib.load().vq_linear_work_bytes(which, M, K, N, dtype)
+
+
+def _work(which: int, M: int, K: int, N: int, dtype: int, device) -> Optional[torch.Tensor]:
+    """Scratch of one call, out of torch's allocator: calls on different streams or in different graphs never share it."""
+    n = _work_bytes(which, M, K, N, dtype)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """t as a (rows, width) matrix whose rows are dense, at any distance from each other; copied only if it is not one."""
+    t = t if t.dim() == 2 else t.reshape(-1, width)
+    if t.stride(1) == 1 or width == 1:
+        pitch = t.stride(0)
+        if t.shape[0] <= 1 or width <= pitch <= _MAX_PITCH // t.element_size():
+            return t
+    return t.contiguous()
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements between the rows of what ``_rows`` returned (the width where there is only one row)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check(x, weight, bias, activation, residual) -> None:
+    given = [(t, name) for t, name in ((x, "input"), (weight, "weight"), (bias, "bias"), (residual, "residual"))
+             if not (t is None and name in ("bias", "residual"))]
+    for t, name in given:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t.dtype != x.dtype:
+            raise TypeError(f"{name} is {t.dtype}, the input {x.dtype}: all tensors of a linear layer share one type")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, the input on {x.device}")
+    if x.dtype not in DTYPES:
+        raise TypeError(f"linear takes float32, bfloat16 or float16 tensors, got {x.dtype}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"weight must be (out features, in features), both at least 1, got {tuple(weight.shape)}")
+    N, K = weight.shape
+    if max(N, K) > 1 << 20:
+        raise ValueError(f"linear takes up to {1 << 20} features, got {tuple(weight.shape)}")
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"input {tuple(x.shape)} does not end in the weight's {K} in features")
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"bias must have shape ({N},), got {tuple(bias.shape)}")
+    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
+        raise ValueError(f"residual must have the output's shape {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
+    _require_cuda(x, "input")
+
+
+def linear_forward(x, weight, bias=None, activation: str = "none", residual=None, want_pre: bool = False):
+    """``(y, pre)``: ``pre = x W^T + bias`` (None unless wanted) and ``y = act(pre) + residual``, without autograd.
+    Arguments as :func:`linear`, already checked."""
+    lib = _lib.load()
+    N, K = weight.shape
+    dt = DTYPES[x.dtype]
+    x2, w2 = _rows(x, K), _rows(weight, K)
+    M = x2.shape[0]
+    with _on_device(x.device):
+        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+        pre = torch.empty_like(y) if want_pre else None
+        b = None if bias is None else bias.contiguous()
+        r2 = None if residual is None else _rows(residual, N)
+        work = _work(LINEAR_FORWARD, M, K, N, dt, x.device)
+        check(lib.vq_linear(_ptr(x2), _pitch(x2), _ptr(w2), _pitch(w2), _ptr(b), _ptr(r2), 0 if r2 is None else _pitch(r2),
+                            dt, ACTIVATIONS[activation], M, K, N, _ptr(y), _ptr(pre), _ptr(work), _stream(x.device)),
+              "vq_linear")
+    return y, pre
+
+
+def linear_backward(grad, x, weight, pre, activation: str, want_x: bool, want_weight: bool, want_bias: bool):
+    """Gradients ``(input, weight, bias)`` of ``act(x W^T + b)`` for the output gradient ``grad`` (None where not
+    wanted); ``pre`` is what :func:`linear_forward` returned (None for activation "none")."""
+    lib = _lib.load()
+    N, K = weight.shape
+    dt = DTYPES[x.dtype]
+    g = grad.reshape(-1, N).contiguous()
+    M = g.shape[0]
+    gx = gw = gb = None
+    with _on_device(x.device):
+        s = _stream(x.device)
+        if activation != "none":
+            dp = torch.empty_like(g)
+            check(lib.vq_linear_act_grad(_ptr(g), _ptr(pre), dt, ACTIVATIONS[activation], g.numel(), _ptr(dp), s),
+                  "vq_linear_act_grad")
+        else:
+            dp = g
+        if want_x:
+            gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            w2 = _rows(weight, K)
+            work = _work(LINEAR_DGRAD, M, K, N, dt, x.device)
+            check(lib.vq_linear_dgrad(_ptr(dp), _ptr(w2), _pitch(w2), dt, M, K, N, _ptr(gx), _ptr(work), s),
+                  "vq_linear_dgrad")
+        if want_weight or want_bias:
+            x2 = _rows(x, K)
+            gw = torch.empty((N, K), dtype=x.dtype, device=x.device) if want_weight else None
+            gb = torch.empty((N,), dtype=x.dtype, device=x.device) if want_bias else None
+            work = _work(LINEAR_WGRAD, M, K, N, dt, x.device)
+            check(lib.vq_linear_wgrad(_ptr(dp), _ptr(x2), _pitch(x2), dt, M, K, N, _ptr(gw), _ptr(gb), _ptr(work), s),
+                  "vq_linear_wgrad")
+    return gx, gw, gb
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        ctx.activation = activation
+        want_pre = activation != "none" and any(ctx.needs_input_grad[:3])
+        y, pre = linear_forward(x, weight, bias, activation, residual, want_pre)
+        ctx.save_for_backward(x, weight, pre)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        gx = gw = gb = None
+        if any(need[:3]):
+            gx, gw, gb = linear_backward(grad, x, weight, pre, ctx.activation, *need[:3])
+        return gx, gw, gb, grad if need[3] else None, None
+
+
+def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+           residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(input @ weight.T + bias) + residual``.
+
+    input: (..., K); weight: (N, K); bias: (N,) or None; residual: (..., N) or None; the result is (..., N), dense.  One
+    element type for all of them: float32, bfloat16 or float16.  activation: "none", "relu", "silu", "gelu" (the exact
+    one, by the normal distribution function) or "gelu_tanh".  Rows at any distance from each other are read in place;
+    other strides are copied first.  Sums are fp32 and every output is rounded once; the result is the same bits on
+    every run.
+
+    Differentiable once in all four tensors.  For an activation the forward keeps ``input @ weight.T + bias`` in the
+    tensors' type, and the backward rounds the gradient behind the activation to it before the two products.
+    Under autocast the tensors keep their types.  May be captured in a graph, backward included (drop every eager autograd
+    graph over the same leaves before capturing, as torch asks for any backward under capture)."""
+    _check(input, weight, bias, activation, residual)
+    if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _LinearFn.apply(input, weight, bias, residual, activation)
+    return linear_forward(input, weight, bias, activation, residual)[0]
+
+
+class Linear(nn.Linear):
+    """``nn.Linear`` (same parameters, initialisation and state dict) on :func:`linear`, with the activation and an optional
+    residual in the same kernel: ``layer(x, residual)`` is ``act(x W^T + b) + residual``."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str = "none", device=None,
+                 dtype=None):
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        self.activation = activation
+
+    def forward(self, input: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return linear(input, self.weight, self.bias, self.activation, residual)
+
+    def extra_repr(self) -> str:
+        return f"{super().extra_repr()}, activation={self.activation}"
