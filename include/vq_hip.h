@@ -336,13 +336,14 @@ int vq_conv1x1_wgrad(const float* gy, const float* x, int layout, int64_t N, int
  * vq_linear_act_grad: dp = gy * act'(pre) for `count` elements, act other than VQ_ACT_NONE.  May run in place.
  * vq_linear_dgrad:    gx = dp W.
  * vq_linear_wgrad:    gW = dp^T x;  gbias[n] = sum_m dp[m][n].  One of the two may be NULL.
+ * vq_linear_backward: the three in one call, of those of gx, gW and gbias that are not NULL (for an empty gx give NULL).
  * Sums split over workgroups are added in a fixed order: the same bits on every run.
  * `work`: vq_linear_work_bytes(VQ_LINEAR_*, ...) bytes, 16-byte aligned, contents irrelevant before and after
  * the call; calls that may overlap need one each.
  */
 enum { VQ_F32 = 0, VQ_BF16 = 1, VQ_F16 = 2 };
 enum { VQ_ACT_NONE = 0, VQ_ACT_RELU = 1, VQ_ACT_SILU = 2, VQ_ACT_GELU = 3, VQ_ACT_GELU_TANH = 4 };
-enum { VQ_LINEAR_FORWARD = 0, VQ_LINEAR_DGRAD = 1, VQ_LINEAR_WGRAD = 2 };
+enum { VQ_LINEAR_FORWARD = 0, VQ_LINEAR_DGRAD = 1, VQ_LINEAR_WGRAD = 2, VQ_LINEAR_BACKWARD = 3 };
 int64_t vq_linear_work_bytes(int pass, int64_t M, int K, int N, int dtype);
 int vq_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* residual,
               int64_t ldr, int dtype, int act, int64_t M, int K, int N, void* y, void* pre, void* work, void* stream);
@@ -351,6 +352,8 @@ int vq_linear_dgrad(const void* dp, const void* W, int64_t ldw, int dtype, int64
                     void* stream);
 int vq_linear_wgrad(const void* dp, const void* x, int64_t ldx, int dtype, int64_t M, int K, int N, void* gW, void* gbias,
                     void* work, void* stream);
+int vq_linear_backward(const void* gy, const void* pre, const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype,
+                       int act, int64_t M, int K, int N, void* gx, void* gW, void* gbias, void* work, void* stream);
 
 /*
  * Global gradient norm over a list of tensors, and clipping by it: what stands between the gradients and the

@@ -81,6 +81,8 @@ def test_clipping_refuses_shared_and_expanded_memory():
         vq.clip_grads([t(1, 4).expand(3, 4)], 1.0)
     with pytest.raises(ValueError, match="share memory"):
         vq.clip_grads([a[0], a[1]], 1.0, out=[a[1], a[0]])
+    with pytest.raises(ValueError, match="share memory"):       # 16-bit gradients in the first half of their own fp32 output
+        vq.clip_grads([a.view(-1).view(BF)[:24]], 1.0, out=[a.view(-1)])
     # neighbours in one buffer are apart
     with pytest.raises(RuntimeError, match="GPU"):
         vq.clip_grads([a[:3], a[3:]], 1.0)
@@ -135,11 +137,13 @@ def test_c_interface_checks_its_arguments():
     assert lib.vq_linear_wgrad(p, p, 8, 0, 4, 8, 8, None, None, p, None) == INVALID
     assert lib.vq_linear_wgrad(p, None, 8, 0, 4, 8, 8, p, None, p, None) == INVALID
     assert lib.vq_linear_wgrad(p, p, 8, 0, 4, 8, 8, None, p, None, None) == INVALID     # the column sums need work
-    assert lib.vq_linear_wgrad(p, p, 8, 0, 4, 8, 8, p, p, None, None) == INVALID
+    back = (p, p, p, 8, p, 8, 0, 1, 4, 8, 8, p, p, p, p, None)
+    for at, v in ((0, None), (1, None), (3, 7), (5, 7), (6, 3), (7, 5), (8, -1), (9, 0), (10, 0), (14, None), (14, ctypes.c_void_p(4104))):
+        assert lib.vq_linear_backward(*(v if i == at else a for i, a in enumerate(back))) in (INVALID, ), (at, v)
     # a split sum without its workspace
     assert lib.vq_linear_work_bytes(2, 1 << 20, 64, 64, 1) > 0
     assert lib.vq_linear_wgrad(p, p, 64, 1, 1 << 20, 64, 64, p, None, None, None) == INVALID
-    for bad in ((3, 4, 8, 8, 0), (0, -1, 8, 8, 0), (0, 4, 0, 8, 0), (0, 4, 8, 8, 7)):
+    for bad in ((4, 4, 8, 8, 0), (-1, 4, 8, 8, 0), (0, -1, 8, 8, 0), (0, 4, 0, 8, 0), (0, 4, 8, 8, 7)):
         assert lib.vq_linear_work_bytes(*bad) == 0
 
 

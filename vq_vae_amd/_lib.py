@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("VQ_VAE_AMD_LIB") or os.path.join(_PKG, "libvqhip.so")
 LAYOUT_ND, LAYOUT_NCHW = 0, 1
 F32, BF16, F16 = 0, 1, 2
 NORM_INF, NORM_1, NORM_2 = 0, 1, 2
-LINEAR_FORWARD, LINEAR_DGRAD, LINEAR_WGRAD = 0, 1, 2
+LINEAR_FORWARD, LINEAR_DGRAD, LINEAR_WGRAD, LINEAR_BACKWARD = 0, 1, 2, 3
 #: activation name -> VQ_ACT_*
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
@@ -95,6 +95,8 @@ SIGNATURES = {
     "vq_linear_dgrad": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "vq_linear_wgrad": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                 c_void_p]),
+    "vq_linear_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int64, c_int,
+                                   c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "vq_grad_norm_work_bytes": (c_int64, [c_int]),
     "vq_grad_norm": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "vq_clip_grads": (c_int, [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),

@@ -36,7 +36,8 @@ struct VqLinearArgs {
   int act;
   float* part;               // splits > 1: [splits][I][ldp] partial sums
   int ldp;
-  float* asum;               // weight gradient: [splits][I] sums of A over r (the bias gradient), or null
+  float* asum;               // weight gradient: the sums of A over r (the bias gradient) of a split sum, [splits][I], or null
+  void* gbias;               // the same in T, where the sum is not split
 };
 
 // -------------------------------------------------------------------------------- element conversions
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     for (int v = 0; v < TJ; ++v)
 #pragma unroll
       for (int g = 0; g < 16; ++g) acc[u][v][g] = 0.0f;
-  const bool want_sum = AMM && a.asum && tj0 == 0 && wj == 0;
+  const bool want_sum = AMM && (a.asum || a.gbias) && tj0 == 0 && wj == 0;
   float asum[TI];
 #pragma unroll
   for (int u = 0; u < TI; ++u) asum[u] = 0.0f;
@@ -512,7 +513,10 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     for (int u = 0; u < TI; ++u) {
       const float s = asum[u] + __shfl_xor(asum[u], 32);
       const int64_t i = i0 + (wi * TI + u) * 32 + (lane & 31);
-      if (lane < 32 && i < a.I) a.asum[split * a.I + i] = s;
+      if (lane < 32 && i < a.I) {
+        if (a.splits > 1) a.asum[split * a.I + i] = s;
+        else reinterpret_cast<T*>(a.gbias)[i] = VqElem<T>::from(s);
+      }
     }
   }
 

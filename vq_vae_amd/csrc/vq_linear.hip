@@ -93,6 +93,13 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a) {
   const int64_t cols = (a.J + E - 1) / E;
   const int64_t count = a.I * cols;
   const int64_t size = a.I * a.ldp;
+  if (a.asum) {   // weight gradient: the bias gradient's partial sums too
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.I; i += (int64_t)gridDim.x * 256) {
+      float c = 0.0f;
+      for (int s = 0; s < a.splits; ++s) c += a.asum[s * a.I + i];
+      reinterpret_cast<T*>(a.gbias)[i] = VqElem<T>::from(c);
+    }
+  }
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < count; t += (int64_t)gridDim.x * 256) {
     const int64_t i = t / cols;
     const int j = (int)(t - i * cols) * E;
@@ -225,6 +232,9 @@ int64_t colsum_slabs(int64_t M, int N) {
   return std::max<int64_t>(1, std::min<int64_t>((M + 63) / 64, std::max<int64_t>(1, 4 * CUS / groups)));
 }
 
+// the activation's gradient, at the head of the backward pass's workspace
+int64_t dp_bytes(int64_t M, int N, int dtype) { return (M * N * (int64_t)elem_size(dtype) + 255) & ~(int64_t)255; }
+
 bool bad_sizes(int64_t M, int K, int N) { return M < 0 || K <= 0 || N <= 0; }
 bool known(int dtype) { return dtype == VQ_F32 || dtype == VQ_BF16 || dtype == VQ_F16; }
 constexpr int MAX_DIM = 1 << 20;
@@ -310,13 +320,10 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, void* work, 
     return rc;
   }
   if (p.tiles_i * p.tiles_j * p.splits >= (int64_t)1 << 23) return VQ_ERR_UNSUPPORTED;
-  if (gbias) {
-    if (!work) return VQ_ERR_INVALID_ARG;
-    a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p, a.I));
-  }
+  a.gbias = gbias;
+  if (gbias && p.splits > 1) a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p, a.I));
   int rc = product(a, layout, dtype, p.config, dma, s);
   if (rc == VQ_OK && a.splits > 1) rc = by_type<RunJoin>(dtype, a, s);
-  if (rc == VQ_OK && gbias) rc = by_type<RunJoinSums>(dtype, (const float*)a.asum, a.splits, a.I, gbias, s);
   return rc;
 }
 
@@ -324,7 +331,7 @@ int64_t product_work(int layout, int64_t I, int J, int64_t R, int dtype, bool su
   int64_t bytes = 0;
   for (int dma = 0; dma < 2; ++dma) {
     const Plan p = make_plan(layout, I, J, R, dtype, dma);
-    bytes = std::max(bytes, part_bytes(p, I) + (sums ? (int64_t)p.splits * I * 4 : 0));
+    bytes = std::max(bytes, part_bytes(p, I) + (sums && p.splits > 1 ? (int64_t)p.splits * I * 4 : 0));
   }
   return bytes;
 }
@@ -332,7 +339,11 @@ int64_t product_work(int layout, int64_t I, int J, int64_t R, int dtype, bool su
 }  // namespace
 
 extern "C" int64_t vq_linear_work_bytes(int pass, int64_t M, int K, int N, int dtype) {
-  if (bad_sizes(M, K, N) || K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || !known(dtype) || pass < 0 || pass > 2) return 0;
+  if (bad_sizes(M, K, N) || K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || !known(dtype)) return 0;
+  if (pass < VQ_LINEAR_FORWARD || pass > VQ_LINEAR_BACKWARD) return 0;
+  if (pass == VQ_LINEAR_BACKWARD)
+    return dp_bytes(M, N, dtype) + std::max(vq_linear_work_bytes(VQ_LINEAR_DGRAD, M, K, N, dtype),
+                                            vq_linear_work_bytes(VQ_LINEAR_WGRAD, M, K, N, dtype));
   if (pass == VQ_LINEAR_FORWARD) return product_work(0, M, N, K, dtype, false);
   if (pass == VQ_LINEAR_DGRAD) return product_work(1, M, K, N, dtype, false);
   return std::max(product_work(2, N, K, M, dtype, true), colsum_slabs(M, N) * N * 4);
@@ -414,4 +425,31 @@ extern "C" int vq_linear_wgrad(const void* dp, const void* x, int64_t ldx, int d
   a.R = M;
   a.out = gW;
   return run_product(2, a, dtype, gbias, work, s);
+}
+
+extern "C" int vq_linear_backward(const void* gy, const void* pre, const void* x, int64_t ldx, const void* W, int64_t ldw,
+                                  int dtype, int act, int64_t M, int K, int N, void* gx, void* gW, void* gbias, void* work,
+                                  void* stream) {
+  if (bad_sizes(M, K, N) || !known(dtype) || act < VQ_ACT_NONE || act > VQ_ACT_GELU_TANH) return VQ_ERR_INVALID_ARG;
+  // everything the three calls would refuse, before the first of them has launched anything
+  if (M > 0 && (!gy || (act != VQ_ACT_NONE && !pre))) return VQ_ERR_INVALID_ARG;
+  if ((gx && (!W || ldw < K)) || (gW && ((M > 0 && !x) || ldx < K))) return VQ_ERR_INVALID_ARG;
+  if (vq_linear_work_bytes(VQ_LINEAR_BACKWARD, M, K, N, dtype) > 0 && (!work || !aligned16(work))) return VQ_ERR_INVALID_ARG;
+  const size_t es = elem_size(dtype);
+  if (K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || pitch_too_wide(N, es) || (gx && pitch_too_wide(ldw, es)) ||
+      (gW && pitch_too_wide(ldx, es)))
+    return VQ_ERR_UNSUPPORTED;
+  const void* dp = gy;
+  if (act != VQ_ACT_NONE && M > 0) {
+    const int rc = vq_linear_act_grad(gy, pre, dtype, act, M * N, work, stream);
+    if (rc != VQ_OK) return rc;
+    dp = work;
+    work = reinterpret_cast<char*>(work) + dp_bytes(M, N, dtype);
+  }
+  if (gx) {
+    const int rc = vq_linear_dgrad(dp, W, ldw, dtype, M, K, N, gx, work, stream);
+    if (rc != VQ_OK) return rc;
+  }
+  if (gW || gbias) return vq_linear_wgrad(dp, x, ldx, dtype, M, K, N, gW, gbias, work, stream);
+  return VQ_OK;
 }

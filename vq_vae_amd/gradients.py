@@ -15,8 +15,9 @@ import torch
 from . import _lib
 from ._lib import NORM_1, NORM_2, NORM_INF, check
 from .projection import DTYPES
-from .ops import _on_device, _ptr, _require_cuda, _stream
+from .ops import _on_device, _raw_stream, _require_cuda
 
+_ITEM = np.array([4, 2, 2], np.int64)        # bytes of an element, by the C interface's types
 _KINDS = {1.0: NORM_1, 2.0: NORM_2, math.inf: NORM_INF}
 
 
@@ -80,17 +81,22 @@ def _refs(srcs: Sequence[torch.Tensor], dsts: Sequence[torch.Tensor]) -> np.ndar
     return refs
 
 
-def _refuse_overlap(tensors: Sequence[torch.Tensor]) -> None:
-    """Raises where two of the tensors share memory: a kernel over all of them would race with itself.  Tensors with gaps
-    (columns of one matrix) count from their first to their last element."""
-    runs = [(t.data_ptr(), t.numel() * t.element_size() if t.is_contiguous() else
-             (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()) for t in tensors if t.numel()]
-    runs.sort()
-    end = 0
-    for start, size in runs:
-        if start < end:
-            raise ValueError("gradients that are to be scaled share memory: each may be given once")
-        end = start + size
+def _refuse_overlap(start: np.ndarray, size: np.ndarray) -> None:
+    """Raises where two runs of memory overlap: a kernel over all of them would race with itself."""
+    some = size > 0
+    start, size = start[some], size[some]
+    order = start.argsort()
+    start, end = start[order], (start + size)[order]
+    if (end[:-1] > start[1:]).any():
+        raise ValueError("gradients that are to be scaled share memory: each may be given once")
+
+
+def _runs(refs: np.ndarray):
+    """Addresses and sizes of the memory that clipping touches: once for a tensor scaled in place."""
+    size = refs[:, 2]
+    apart = (refs[:, 0] != refs[:, 1]) | (refs[:, 3] & 0xff != refs[:, 3] >> 32)
+    return (np.concatenate((refs[apart, 0], refs[:, 1])),
+            np.concatenate((size[apart] * _ITEM[refs[apart, 3] & 0xff], size * _ITEM[refs[:, 3] >> 32])))
 
 
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
@@ -111,7 +117,7 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
         norm = torch.empty((), dtype=torch.float32, device=device)
         work = torch.empty(lib.vq_grad_norm_work_bytes(len(flat)), dtype=torch.uint8, device=device)
         refs = _refs(flat, flat)
-        check(lib.vq_grad_norm(refs.ctypes.data, len(flat), kind, _ptr(norm), _ptr(work), _stream(device)), "vq_grad_norm")
+        check(lib.vq_grad_norm(refs.ctypes.data, len(flat), kind, norm.data_ptr(), work.data_ptr(), _raw_stream(device)), "vq_grad_norm")
     return norm
 
 
@@ -143,31 +149,47 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     if not grads:
         return torch.zeros(())
     written = grads if out is None else out
-    for t in written:
-        if not t.is_contiguous() and t.numel() and any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
-            raise ValueError("an expanded tensor cannot be scaled: several of its elements are one")
-    _refuse_overlap(grads if out is None else [t for pair in zip(grads, out) for t in _apart(*pair)])
+    dense = all([t.is_contiguous() for t in grads]) and (out is None or all([t.is_contiguous() for t in out]))
+    if dense:
+        refs = _refs(grads, written)
+        _refuse_overlap(*_runs(refs))
+    else:
+        _refuse_strides(grads, written)
     _require_cuda(grads[0], "grads")
     device = grads[0].device
-    with torch.no_grad(), _on_device(device):
-        srcs, dsts, back = _dense_pairs(grads, written)
+    with _on_device(device):
+        dsts, back = written, ()
+        if not dense:
+            with torch.no_grad():
+                srcs, dsts, back = _dense_pairs(grads, written)
+            refs = _refs(srcs, dsts)
         lib = _lib.load()
         norm = torch.empty((), dtype=torch.float32, device=device)
-        work = torch.empty(lib.vq_grad_norm_work_bytes(len(srcs)), dtype=torch.uint8, device=device)
-        refs = _refs(srcs, dsts)
-        check(lib.vq_clip_grads(refs.ctypes.data, len(srcs), kind, max_norm, _ptr(norm), _ptr(work), _stream(device)),
-              "vq_clip_grads")
-        for o, c in back:
-            o.copy_(c)
+        work = torch.empty(lib.vq_grad_norm_work_bytes(len(grads)), dtype=torch.uint8, device=device)
+        check(lib.vq_clip_grads(refs.ctypes.data, len(grads), kind, max_norm, norm.data_ptr(), work.data_ptr(),
+                                _raw_stream(device)), "vq_clip_grads")
+        with torch.no_grad():
+            for o, c in back:
+                o.copy_(c)
         torch.autograd.graph.increment_version([t for t in dsts if not t.is_inference()])
     return norm
+
+
+def _refuse_strides(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]) -> None:
+    """Refusals of a list with tensors that are not contiguous.  One with gaps (columns of a matrix) counts from its first to
+    its last element."""
+    for t in written:
+        if t.numel() and any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
+            raise ValueError("an expanded tensor cannot be scaled: several of its elements are one")
+    tensors = list(written) + [g for g, o in zip(grads, written) if g.data_ptr() != o.data_ptr()]
+    _refuse_overlap(np.array([t.data_ptr() for t in tensors], np.int64),
+                    np.array([t.numel() and (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
+                              for t in tensors], np.int64))
 
 
 def _dense_pairs(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]):
     """What the kernel reads and writes: dense runs of the same element order, the tensors themselves wherever they are
     that, copies otherwise; and the copies to be brought back, as (tensor, copy)."""
-    if all(t.is_contiguous() for t in grads) and (written is grads or all(t.is_contiguous() for t in written)):
-        return grads, written, []
     srcs, dsts, back = [], [], []
     for g, o in zip(grads, written):
         if _dense(g) and o.stride() == g.stride():
@@ -185,11 +207,6 @@ def _dense_pairs(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor])
             dsts.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
             back.append((o, dsts[-1]))
     return srcs, dsts, back
-
-
-def _apart(src: torch.Tensor, dst: torch.Tensor):
-    """The memory a pair touches: one run where it is scaled in place, two otherwise."""
-    return (dst,) if src.data_ptr() == dst.data_ptr() and src.dtype == dst.dtype else (src, dst)
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,

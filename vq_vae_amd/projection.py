@@ -14,8 +14,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from ._lib import ACTIVATIONS, LINEAR_DGRAD, LINEAR_FORWARD, LINEAR_WGRAD, check
-from .ops import _on_device, _ptr, _require_cuda, _stream
+from ._lib import ACTIVATIONS, LINEAR_BACKWARD, LINEAR_FORWARD, check
+from .ops import _on_device, _raw_stream, _require_cuda
 
 DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -34,6 +34,10 @@ def _work(which: int, M: int, K: int, N: int, dtype: int, device) -> Optional[to
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
+def _address(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """t as a (rows, width) matrix whose rows are dense, at any distance from each other; copied only if it is not one."""
     t = t if t.dim() == 2 else t.reshape(-1, width)
@@ -50,9 +54,9 @@ def _pitch(t: torch.Tensor) -> int:
 
 
 def _check(x, weight, bias, activation, residual) -> None:
-    given = [(t, name) for t, name in ((x, "input"), (weight, "weight"), (bias, "bias"), (residual, "residual"))
-             if not (t is None and name in ("bias", "residual"))]
-    for t, name in given:
+    for t, name, optional in ((x, "input", False), (weight, "weight", False), (bias, "bias", True), (residual, "residual", True)):
+        if t is None and optional:
+            continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
         if t.dtype != x.dtype:
@@ -70,9 +74,9 @@ def _check(x, weight, bias, activation, residual) -> None:
         raise ValueError(f"linear takes up to {1 << 20} features, got {tuple(weight.shape)}")
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"input {tuple(x.shape)} does not end in the weight's {K} in features")
-    if bias is not None and tuple(bias.shape) != (N,):
+    if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias must have shape ({N},), got {tuple(bias.shape)}")
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
+    if residual is not None and residual.shape != (*x.shape[:-1], N):
         raise ValueError(f"residual must have the output's shape {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
     _require_cuda(x, "input")
 
@@ -80,53 +84,44 @@ def _check(x, weight, bias, activation, residual) -> None:
 def linear_forward(x, weight, bias=None, activation: str = "none", residual=None, want_pre: bool = False):
     """``(y, pre)``: ``pre = x W^T + bias`` (None unless wanted) and ``y = act(pre) + residual``, without autograd.
     Arguments as :func:`linear`, already checked."""
-    lib = _lib.load()
     N, K = weight.shape
     dt = DTYPES[x.dtype]
-    x2, w2 = _rows(x, K), _rows(weight, K)
-    M = x2.shape[0]
-    with _on_device(x.device):
-        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    device = x.device
+    with _on_device(device):
+        x2, w2 = _rows(x, K), _rows(weight, K)
+        M = x2.shape[0]
+        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=device)
         pre = torch.empty_like(y) if want_pre else None
         b = None if bias is None else bias.contiguous()
-        r2 = None if residual is None else _rows(residual, N)
-        work = _work(LINEAR_FORWARD, M, K, N, dt, x.device)
-        check(lib.vq_linear(_ptr(x2), _pitch(x2), _ptr(w2), _pitch(w2), _ptr(b), _ptr(r2), 0 if r2 is None else _pitch(r2),
-                            dt, ACTIVATIONS[activation], M, K, N, _ptr(y), _ptr(pre), _ptr(work), _stream(x.device)),
-              "vq_linear")
+        r2, ldr = None, 0
+        if residual is not None:
+            r2 = _rows(residual, N)
+            ldr = _pitch(r2)
+        work = _work(LINEAR_FORWARD, M, K, N, dt, device)
+        check(_lib.load().vq_linear(x2.data_ptr(), _pitch(x2), w2.data_ptr(), _pitch(w2), _address(b), _address(r2), ldr, dt,
+                                    ACTIVATIONS[activation], M, K, N, y.data_ptr(), _address(pre), _address(work),
+                                    _raw_stream(device)), "vq_linear")
     return y, pre
 
 
 def linear_backward(grad, x, weight, pre, activation: str, want_x: bool, want_weight: bool, want_bias: bool):
     """Gradients ``(input, weight, bias)`` of ``act(x W^T + b)`` for the output gradient ``grad`` (None where not
     wanted); ``pre`` is what :func:`linear_forward` returned (None for activation "none")."""
-    lib = _lib.load()
     N, K = weight.shape
     dt = DTYPES[x.dtype]
-    g = grad.reshape(-1, N).contiguous()
-    M = g.shape[0]
-    gx = gw = gb = None
-    with _on_device(x.device):
-        s = _stream(x.device)
-        if activation != "none":
-            dp = torch.empty_like(g)
-            check(lib.vq_linear_act_grad(_ptr(g), _ptr(pre), dt, ACTIVATIONS[activation], g.numel(), _ptr(dp), s),
-                  "vq_linear_act_grad")
-        else:
-            dp = g
-        if want_x:
-            gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            w2 = _rows(weight, K)
-            work = _work(LINEAR_DGRAD, M, K, N, dt, x.device)
-            check(lib.vq_linear_dgrad(_ptr(dp), _ptr(w2), _pitch(w2), dt, M, K, N, _ptr(gx), _ptr(work), s),
-                  "vq_linear_dgrad")
-        if want_weight or want_bias:
-            x2 = _rows(x, K)
-            gw = torch.empty((N, K), dtype=x.dtype, device=x.device) if want_weight else None
-            gb = torch.empty((N,), dtype=x.dtype, device=x.device) if want_bias else None
-            work = _work(LINEAR_WGRAD, M, K, N, dt, x.device)
-            check(lib.vq_linear_wgrad(_ptr(dp), _ptr(x2), _pitch(x2), dt, M, K, N, _ptr(gw), _ptr(gb), _ptr(work), s),
-                  "vq_linear_wgrad")
+    device = x.device
+    with _on_device(device):
+        g = grad.reshape(-1, N).contiguous()
+        M = g.shape[0]
+        x2, w2 = _rows(x, K), _rows(weight, K)
+        gx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_x else None
+        gw = torch.empty((N, K), dtype=x.dtype, device=device) if want_weight else None
+        gb = torch.empty((N,), dtype=x.dtype, device=device) if want_bias else None
+        work = _work(LINEAR_BACKWARD, M, K, N, dt, device)
+        check(_lib.load().vq_linear_backward(g.data_ptr(), _address(pre), x2.data_ptr(), _pitch(x2), w2.data_ptr(),
+                                             _pitch(w2), dt, ACTIVATIONS[activation], M, K, N, _address(gx) if M else None,
+                                             _address(gw), _address(gb), _address(work), _raw_stream(device)),
+              "vq_linear_backward")
     return gx, gw, gb
 
 
