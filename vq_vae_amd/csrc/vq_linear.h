@@ -143,6 +143,21 @@ __device__ __forceinline__ float vql_act(float p, int act) {
     default: return p;
   }
 }
+template <int ACT, bool FAST, int E>
+__device__ __forceinline__ void vql_act_each(float (&p)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) p[e] = vql_act<FAST>(p[e], ACT);
+}
+template <bool FAST, int E>
+__device__ __forceinline__ void vql_act_all(float (&p)[E], int act) {   // one branch for all of them
+  switch (act) {
+    case VQ_ACT_RELU: vql_act_each<VQ_ACT_RELU, FAST, E>(p); break;
+    case VQ_ACT_SILU: vql_act_each<VQ_ACT_SILU, FAST, E>(p); break;
+    case VQ_ACT_GELU: vql_act_each<VQ_ACT_GELU, FAST, E>(p); break;
+    case VQ_ACT_GELU_TANH: vql_act_each<VQ_ACT_GELU_TANH, FAST, E>(p); break;
+    default: break;
+  }
+}
 // act'(p).  Beyond |p| = 100 every derivative has its limit, 0 or 1; the clamp keeps inf * 0 out of it.
 template <bool FAST>
 __device__ __forceinline__ float vql_act_slope(float p0, int act) {
@@ -333,10 +348,7 @@ __device__ __forceinline__ void vql_epilogue(const VqLinearArgs& a, int64_t i, i
   VqChunk<T> y, pv;
 #pragma unroll
   for (int e = 0; e < E; ++e) pv.e[e] = VqElem<T>::from(p[e]);
-  if (a.act != VQ_ACT_NONE) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) p[e] = vql_act<FAST>(p[e], a.act);
-  }
+  vql_act_all<FAST, E>(p, a.act);
   if (a.res) {
 #pragma unroll
     for (int e = 0; e < E; ++e) p[e] += r[e];
@@ -371,47 +383,77 @@ __device__ __forceinline__ void vql_bias16(const VqLinearArgs& a, int j, float* 
 }
 
 // -------------------------------------------------------------------------------- one step
-// The matrix work of one step on the tiles at `cur`.
-template <typename T, typename OA, typename OB, int TI, int TJ>
-__device__ __forceinline__ void vql_compute(const VQL_LDS char* cur, int wi, int wj, int lane, bool want_sum,
-                                            f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
+template <int TI, int TJ>
+struct VqFrags {
+  u32x4 a[TI], b[TJ];
+};
+template <typename OA, typename OB, int TI, int TJ>
+__device__ __forceinline__ void vql_read(VqFrags<TI, TJ>& f, const VQL_LDS char* tile, int q, int wi, int wj, int lane) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    u32x4 fa[TI], fb[TJ];
+  for (int u = 0; u < TI; ++u) f.a[u] = OA::frag(tile, (wi * TI + u) * 32, q, lane);
 #pragma unroll
-    for (int u = 0; u < TI; ++u) fa[u] = OA::frag(cur, (wi * TI + u) * 32, q, lane);
+  for (int v = 0; v < TJ; ++v) f.b[v] = OB::frag(tile + OA::BYTES, (wj * TJ + v) * 32, q, lane);
+}
+template <typename T, bool SUMS, int TI, int TJ>
+__device__ __forceinline__ void vql_mul(const VqFrags<TI, TJ>& f, bool want_sum, f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
 #pragma unroll
-    for (int v = 0; v < TJ; ++v) fb[v] = OB::frag(cur + OA::BYTES, (wj * TJ + v) * 32, q, lane);
+  for (int u = 0; u < TI; ++u)
 #pragma unroll
-    for (int u = 0; u < TI; ++u)
+    for (int v = 0; v < TJ; ++v) acc[u][v] = vql_mma<T>(f.b[v], f.a[u], acc[u][v]);
+  if (SUMS && want_sum) {
 #pragma unroll
-      for (int v = 0; v < TJ; ++v) acc[u][v] = vql_mma<T>(fb[v], fa[u], acc[u][v]);
-    if (OA::SUMS && want_sum) {
-#pragma unroll
-      for (int u = 0; u < TI; ++u) asum[u] += vql_sum16<T>(fa[u]);
-    }
+    for (int u = 0; u < TI; ++u) asum[u] += vql_sum16<T>(f.a[u]);
   }
 }
-// The same with the DMA of the next step issued first.  __restrict__ (the two buffers are different ones) tells the
-// compiler that the fragment reads need not wait for the DMA.
-template <typename T, typename OA, typename OB, int TI, int TJ>
-__device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t next, bool more, VQL_LDS char* __restrict__ nxt,
-                                         const VQL_LDS char* __restrict__ cur, int wi, int wj, int wave, int lane,
-                                         bool want_sum, f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
-  if (more) {
-    oa.dma(next, nxt, wave);
-    ob.dma(next, nxt + OA::BYTES, wave);
+// Waits until at most `n` of this wave's DMA instructions are in flight and its LDS accesses are done, then for the
+// other waves.  A bare barrier: nothing else has to have landed.
+template <int N>
+__device__ __forceinline__ void vql_publish() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// One step of the sum: the tiles of this step at from + cur, those of the next at from + nxt.  In registers there are two
+// sets of fragments, one read while the other is multiplied, so that neither the LDS reads nor the barrier of a step leave
+// the matrix cores idle:
+//     q0 | read q1, multiply q0 | read q2, multiply q1 | read q3, multiply q2 | barrier, fill, read the next q0, multiply q3
+// `fly`: this wave's DMA instructions that may still be in flight behind those of the next step, or 0.  `into` and `from`
+// are the same memory; __restrict__ tells the compiler that a fragment read need not wait for the DMA in flight: the
+// barriers and the counted waits see to that.
+template <typename T, typename OA, typename OB, int TI, int TJ, int FLYING>
+__device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma_step, bool dma, bool more, bool counted,
+                                         VQL_LDS char* __restrict__ into, const VQL_LDS char* __restrict__ from, int cur, int nxt,
+                                         int wi, int wj, int wave, int lane, bool want_sum, VqFrags<TI, TJ> (&f)[2],
+                                         f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    vql_read<OA, OB, TI, TJ>(f[(q + 1) & 1], from + cur, q + 1, wi, wj, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    vql_mul<T, OA::SUMS, TI, TJ>(f[q & 1], want_sum, acc, asum);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  vql_compute<T, OA, OB, TI, TJ>(cur, wi, wj, lane, want_sum, acc, asum);
+  if (FLYING > 0 && counted) vql_publish<FLYING>();
+  else vql_publish<0>();
+  if (dma) {
+    oa.dma(dma_step, into + cur, wave);
+    ob.dma(dma_step, into + cur + OA::BYTES, wave);
+  }
+  if (more) vql_read<OA, OB, TI, TJ>(f[0], from + nxt, 0, wi, wj, lane);
+  __builtin_amdgcn_sched_barrier(0);
+  vql_mul<T, OA::SUMS, TI, TJ>(f[1], want_sum, acc, asum);
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // -------------------------------------------------------------------------------- the product
 namespace {   // the kernels of a translation unit are its own
 // A workgroup of WI x WJ waves owns a BI x BJ block of C (and, with splits, a range of the sum); a wave owns
-// (BI / WI) x (BJ / WJ) of it in 32x32 accumulator tiles.  Both operand tiles of a 128-byte step lie in one of two LDS
-// buffers, filled for the next step while the matrix cores work on this one: by DMA where rows start on 16 bytes,
-// else through registers.  One barrier a step.
-template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, bool DMA>
+// (BI / WI) x (BJ / WJ) of it in 32x32 accumulator tiles.  DMA: rows start on 16 bytes, so that the tiles go straight into
+// LDS; otherwise they go through registers.
+template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
 __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_product_kernel(VqLinearArgs a) {
   constexpr int NT = WI * WJ * 64;
   constexpr int TI = BI / WI / 32, TJ = BJ / WJ / 32;
@@ -463,49 +505,39 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
 #pragma unroll
   for (int u = 0; u < TI; ++u) asum[u] = 0.0f;
 
-  auto by_registers = [&](int64_t s, VQL_LDS char* buf) {
+  // The sum.  NS tile pairs lie in LDS; the one that a step has used up is filled for the step NS later, by DMA where that
+  // step is a whole one, through registers otherwise.
+  VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
+  auto by_registers = [&](int64_t s, int at) {
     u32x4 va[OA::PER], vb[OB::PER];
     oa.fetch(s, a.R, wave, lane, va);
     ob.fetch(s, a.R, wave, lane, vb);
-    oa.commit(buf, wave, lane, va);
-    ob.commit(buf + OA::BYTES, wave, lane, vb);
+    oa.commit(lds + at, wave, lane, va);
+    ob.commit(lds + at + OA::BYTES, wave, lane, vb);
   };
-  auto publish = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): this wave's DMA and LDS writes have landed
-    __syncthreads();
-  };
-  VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
   if (s0 < s1) {
-    if (DMA && s0 < full) {
-      oa.dma(s0, lds, wave);
-      ob.dma(s0, lds + OA::BYTES, wave);
-    } else {
-      by_registers(s0, lds);
-    }
-  }
-  publish();
-  int cur = 0;
-  for (int64_t s = s0; s < s1; ++s) {
-    VQL_LDS char* buf = lds + cur * STAGE;
-    VQL_LDS char* nxt = lds + (cur ^ 1) * STAGE;
-    if constexpr (DMA) {
-      const bool more = s + 1 < s1 && s + 1 < full;
-      vql_step<T, OA, OB, TI, TJ>(oa, ob, s + 1, more, nxt, buf, wi, wj, wave, lane, want_sum, acc, asum);
-      if (s + 1 < s1 && s + 1 >= full) by_registers(s + 1, nxt);
-    } else {
-      u32x4 va[OA::PER], vb[OB::PER];
-      if (s + 1 < s1) {
-        oa.fetch(s + 1, a.R, wave, lane, va);
-        ob.fetch(s + 1, a.R, wave, lane, vb);
-      }
-      vql_compute<T, OA, OB, TI, TJ>(buf, wi, wj, lane, want_sum, acc, asum);
-      if (s + 1 < s1) {
-        oa.commit(nxt, wave, lane, va);
-        ob.commit(nxt + OA::BYTES, wave, lane, vb);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      if (DMA && s0 + n < s1 && s0 + n < full) {
+        oa.dma(s0 + n, lds + n * STAGE, wave);
+        ob.dma(s0 + n, lds + n * STAGE + OA::BYTES, wave);
+      } else if (s0 + n < s1) {
+        by_registers(s0 + n, n * STAGE);
       }
     }
-    publish();
-    cur ^= 1;
+    vql_publish<0>();
+    VqFrags<TI, TJ> f[2];
+    vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
+    const int64_t last_dma = DMA ? (s1 < full ? s1 : full) : s0;      // steps from here on are filled through registers
+    int at = 0;
+    for (int64_t s = s0; s < s1; ++s) {
+      const int cur = at * STAGE;
+      at = at + 1 == NS ? 0 : at + 1;
+      vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(oa, ob, s + NS, s + NS < last_dma, s + 1 < s1,
+                                                                 s + NS - 1 < last_dma, lds, lds, cur, at * STAGE, wi, wj, wave,
+                                                                 lane, want_sum, f, acc, asum);
+      if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
+    }
   }
 
   if (AMM && want_sum) {
@@ -575,27 +607,27 @@ int vql_product_f16(const VqLinearArgs& a, int layout, int config, bool dma, hip
 
 namespace {
 // One kernel of the family: its entry in the table of kernels with large LDS, and its launch.
-template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, bool DMA>
+template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
 struct VqProduct {
-  static constexpr int LDS = 2 * (BI + BJ) * 128;
+  static constexpr int LDS = NS * (BI + BJ) * 128;
   static_assert(LDS >= WI * WJ * 32 * (BJ / WJ + 4) * 4, "the epilogue's staging fits the stage buffers");
-  static const void* address() { return reinterpret_cast<const void*>(&vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, DMA>); }
+  static const void* address() { return reinterpret_cast<const void*>(&vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, NS, DMA>); }
   static inline VqLdsRegistrar registrar{address(), LDS};
   static int launch(const VqLinearArgs& a, hipStream_t s) {
     (void)&registrar;
     const int rc = vq_lds_ensure(address(), LDS, nullptr);
     if (rc != VQ_OK) return rc;
     const int64_t blocks = a.tiles_i * a.tiles_j * a.splits;
-    hipLaunchKernelGGL((vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, DMA>), dim3((unsigned)blocks), dim3(WI * WJ * 64), LDS, s, a);
+    hipLaunchKernelGGL((vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, NS, DMA>), dim3((unsigned)blocks), dim3(WI * WJ * 64), LDS, s, a);
     return vq_hip_status(hipGetLastError());
   }
 };
 template <typename T, bool AMM, bool BMM>
 int vql_launch_layout(const VqLinearArgs& a, int config, bool dma, hipStream_t s) {
-  if (config == VQL_C256) return dma ? VqProduct<T, AMM, BMM, 256, 256, 2, 4, true>::launch(a, s) : VQ_ERR_INVALID_ARG;
+  if (config == VQL_C256) return dma ? VqProduct<T, AMM, BMM, 256, 256, 2, 4, 2, true>::launch(a, s) : VQ_ERR_INVALID_ARG;
   if (config == VQL_C128)
-    return dma ? VqProduct<T, AMM, BMM, 128, 128, 2, 2, true>::launch(a, s) : VqProduct<T, AMM, BMM, 128, 128, 2, 2, false>::launch(a, s);
-  return dma ? VqProduct<T, AMM, BMM, 64, 64, 2, 2, true>::launch(a, s) : VqProduct<T, AMM, BMM, 64, 64, 2, 2, false>::launch(a, s);
+    return dma ? VqProduct<T, AMM, BMM, 128, 128, 2, 2, 2, true>::launch(a, s) : VqProduct<T, AMM, BMM, 128, 128, 2, 2, 2, false>::launch(a, s);
+  return dma ? VqProduct<T, AMM, BMM, 64, 64, 2, 2, 3, true>::launch(a, s) : VqProduct<T, AMM, BMM, 64, 64, 2, 2, 2, false>::launch(a, s);
 }
 template <typename T>
 int vql_product(const VqLinearArgs& a, int layout, int config, bool dma, hipStream_t s) {
@@ -607,11 +639,11 @@ int vql_product(const VqLinearArgs& a, int layout, int config, bool dma, hipStre
 
 // The kernels of one element type (the compiler's host pass leaves kernels out that it meets only through VqProduct).
 #define VQL_KERNELS_OF(T, AMM, BMM)                                                       \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 256, 256, 2, 4, true>(VqLinearArgs);  \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, true>(VqLinearArgs);  \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, false>(VqLinearArgs); \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, true>(VqLinearArgs);    \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, false>(VqLinearArgs);
+  template __global__ void vql_product_kernel<T, AMM, BMM, 256, 256, 2, 4, 2, true>(VqLinearArgs);  \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, 2, true>(VqLinearArgs);  \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, 2, false>(VqLinearArgs); \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, 3, true>(VqLinearArgs);    \
+  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, 2, false>(VqLinearArgs);
 #define VQL_KERNELS(T)           \
   namespace {                    \
   VQL_KERNELS_OF(T, false, false) \
