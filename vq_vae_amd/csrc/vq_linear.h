@@ -26,6 +26,7 @@ struct VqLinearArgs {
   int64_t R;                 // length of the sum
   int64_t steps_per_split;   // 128-byte steps of the sum that one workgroup takes
   int splits;
+  int workgroups;            // that fit the device at a time (a multiple of 8): each takes every so many-th block
   int64_t tiles_i;
   int tiles_j;
   void* out;                 // [I][J]
@@ -218,8 +219,8 @@ __device__ __forceinline__ float vql_sum16(u32x4 v) {   // sum of the fragment's
 
 // -------------------------------------------------------------------------------- operand tiles in LDS
 // One step of the sum covers 128 bytes of r: 64 elements of 16 bits, 32 of 32 bits.
-// r-major tile of `B` indexes: B rows of 128 bytes, 16-byte piece c of row m in slot c ^ ((m >> 1) & 7): the 32 rows
-//   that a fragment read touches fall on all banks evenly.
+// r-major tile of `B` indexes: B rows of 128 bytes, 16-byte piece c of row m in slot c ^ (bits 1-3 of m; for the ordered
+//   operand bits 1, 2 and 4): the 16 rows that a fragment read touches at a time fall on all banks evenly.
 // m-major tile: one row of B elements per r, 16-byte piece c of row r in slot c ^ vql_mswz<T>(r): the rows that one
 //   transposing read (16 bits: r = 8h + 4t + 0..3 for both halves h) or one fp32 read (r = e and 4 + e) touches lie in
 //   different 64- or 128-byte segments.
@@ -230,7 +231,11 @@ __device__ __forceinline__ int vql_mswz(int r) {
   return ((r >> 2) & 1) << 3;
 }
 
-template <typename T, bool MMAJOR, int B, int NT, bool DMA>
+// Which index of a 32-block the lanes of the `b`-side operand hold: the matrix instruction leaves a lane the rows 8g + 4h + r
+// (g, r = 0..3) of its column, h = lane / 32; with this order they are the 16 consecutive indexes 16h + 4g + r.
+__device__ __forceinline__ int vql_order(int rho) { return ((rho & 4) << 2) | ((rho >> 1) & 12) | (rho & 3); }
+
+template <typename T, bool MMAJOR, int B, int NT, bool DMA, bool ORDERED>
 struct VqOperand {
   static constexpr int ES = sizeof(T), E = 16 / ES, BK = 128 / ES;
   static constexpr int BYTES = B * 128;
@@ -243,10 +248,11 @@ struct VqOperand {
   int64_t M;             // indexes that exist from m0 on
   uint32_t off[PER];     // this lane's byte offsets of a full step
 
+  __device__ __forceinline__ static int rswz(int row) { return ORDERED ? ((row >> 1) & 3) | ((row >> 2) & 4) : row >> 1; }
   __device__ __forceinline__ static void where(int n, int wave, int lane, int& row, int& piece) {
     const int p = (wave * PER + n) * 64 + lane;
     row = p / CPR;
-    piece = (p % CPR) ^ ((MMAJOR ? vql_mswz<T>(row) : (row >> 1)) & SWZ);
+    piece = (p % CPR) ^ ((MMAJOR ? vql_mswz<T>(row) : rswz(row)) & SWZ);
   }
   __device__ __forceinline__ void init(const char* src, int64_t ld_, int64_t m0, int64_t total, int wave, int lane) {
     ld = ld_;
@@ -302,12 +308,12 @@ struct VqOperand {
   __device__ __forceinline__ static u32x4 frag(const VQL_LDS char* lds, int m, int q, int lane) {
     const int h = lane >> 5;
     if constexpr (!MMAJOR) {
-      const int row = m + (lane & 31);
-      return *reinterpret_cast<const VQL_LDS vql_u32x4_a16*>(lds + row * 128 + (((2 * q + h) ^ ((row >> 1) & 7)) * 16));
+      const int rho = lane & 31, row = m + (ORDERED ? vql_order(rho) : rho);
+      return *reinterpret_cast<const VQL_LDS vql_u32x4_a16*>(lds + row * 128 + (((2 * q + h) ^ (rswz(row) & 7)) * 16));
     } else if constexpr (ES == 2) {
       // transposing read: each group of 16 lanes names 4 rows (r) of 16 consecutive indexes, 8 bytes a lane, and lane i
       // of the group receives index i of the four rows
-      const int s = lane & 15, col = m + ((lane >> 4) & 1) * 16 + (s & 3) * 4;
+      const int s = lane & 15, rho = (lane & 16) + (s & 3) * 4, col = m + (ORDERED ? vql_order(rho) : rho);
       s16x4 half[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -319,7 +325,7 @@ struct VqOperand {
       return __builtin_bit_cast(u32x4, (s16x8)__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       u32x4 v;
-      const int col = m + (lane & 31);
+      const int rho = lane & 31, col = m + (ORDERED ? vql_order(rho) : rho);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 8 * q + 4 * h + e;
@@ -330,59 +336,108 @@ struct VqOperand {
   }
 };
 
-// -------------------------------------------------------------------------------- epilogue of 16 / sizeof(T) columns
-// y = act(c + bias) + residual, rounded once; `pre` = c + bias rounded (kept for the activation's gradient).
+// -------------------------------------------------------------------------------- epilogue
+// y = act(c + bias) + residual, rounded once, for 16 / sizeof(T) columns from j on, `n` of which exist; `pre` = c + bias
+// rounded (kept for the activation's gradient); res: the residual's 16 bytes.
 template <typename T>
-__device__ __forceinline__ void vql_epilogue(const VqLinearArgs& a, int64_t i, int j, const float* c, const float* bias) {
+__device__ __forceinline__ void vql_finish(const VqLinearArgs& a, char* y_at, char* pre_at, int n, const float* c, const float* bias,
+                                           u32x4 res) {
   constexpr int E = 16 / sizeof(T);
-  constexpr bool FAST = sizeof(T) == 2;
-  const int n = a.J - j < E ? a.J - j : E;
-  float p[E], r[E];
+  float p[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) p[e] = c[e] + bias[e];
-  if (a.res) {
-    const VqChunk<T> rv = __builtin_bit_cast(VqChunk<T>, vql_load16_part<T>(a.res + i * a.ldr + (int64_t)j * sizeof(T), n));
-#pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = VqElem<T>::to(rv.e[e]);
-  }
   VqChunk<T> y, pv;
 #pragma unroll
   for (int e = 0; e < E; ++e) pv.e[e] = VqElem<T>::from(p[e]);
-  vql_act_all<FAST, E>(p, a.act);
+  vql_act_all<sizeof(T) == 2, E>(p, a.act);
   if (a.res) {
+    const VqChunk<T> r = __builtin_bit_cast(VqChunk<T>, res);
 #pragma unroll
-    for (int e = 0; e < E; ++e) p[e] += r[e];
+    for (int e = 0; e < E; ++e) p[e] += VqElem<T>::to(r.e[e]);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(p[e]);
-  T* yp = reinterpret_cast<T*>(a.out) + i * a.J + j;
-  T* pp = a.pre ? reinterpret_cast<T*>(a.pre) + i * a.J + j : nullptr;
-  if (n == E) {
-    vql_store16<T>(yp, __builtin_bit_cast(u32x4, y));
-    if (pp) vql_store16<T>(pp, __builtin_bit_cast(u32x4, pv));
+  if (n >= E) {
+    vql_store16<T>(y_at, __builtin_bit_cast(u32x4, y));
+    if (a.pre) vql_store16<T>(pre_at, __builtin_bit_cast(u32x4, pv));
   } else {
 #pragma unroll
     for (int e = 0; e < E - 1; ++e)
       if (e < n) {
-        yp[e] = y.e[e];
-        if (pp) pp[e] = pv.e[e];
+        reinterpret_cast<T*>(y_at)[e] = y.e[e];
+        if (a.pre) reinterpret_cast<T*>(pre_at)[e] = pv.e[e];
       }
   }
 }
-template <typename T>
-__device__ __forceinline__ void vql_bias16(const VqLinearArgs& a, int j, float* bias) {
+// bias[j .. j + W), zero where there is none
+template <typename T, int W>
+__device__ __forceinline__ void vql_bias(const VqLinearArgs& a, int64_t j, float (&bias)[W]) {
   constexpr int E = 16 / sizeof(T);
 #pragma unroll
-  for (int e = 0; e < E; ++e) bias[e] = 0.0f;
-  if (a.bias && j < a.J) {
-    const VqChunk<T> b = __builtin_bit_cast(
-        VqChunk<T>, vql_load16_part<T>(reinterpret_cast<const char*>(a.bias) + (int64_t)j * sizeof(T), a.J - j));
+  for (int e = 0; e < W; ++e) bias[e] = 0.0f;
+  if (a.bias) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) bias[e] = VqElem<T>::to(b.e[e]);
+    for (int k = 0; k < W / E; ++k) {
+      const VqChunk<T> b = __builtin_bit_cast(
+          VqChunk<T>, vql_load16_part<T>(reinterpret_cast<const char*>(a.bias) + (j + k * E) * (int64_t)sizeof(T), a.J - j - k * E));
+#pragma unroll
+      for (int e = 0; e < E; ++e) bias[k * E + e] = VqElem<T>::to(b.e[e]);
+    }
+  }
+}
+// The epilogue of a wave's part of a block: rows i .. i + 32 TI, columns j .. j + 32 TJ.  A lane holds 16 consecutive
+// columns of a row per tile, so that all of it is 16-byte accesses straight from the accumulators.  INSIDE: the whole part
+// exists.  The residual of the next row block is on its way while this one is worked on.
+template <typename T, int TI, int TJ, bool INSIDE>
+__device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int64_t j, int lane, const f32x16 (&acc)[TI][TJ]) {
+  constexpr int ES = sizeof(T), E = 16 / ES, PV = 16 / E;
+  const int lr = lane & 31, lc = 16 * (lane >> 5);
+  // one wave-uniform address per tensor and one 32-bit offset per lane
+  const int64_t pitch = (int64_t)a.J * ES, origin = i * pitch + j * ES;
+  char* const yb = reinterpret_cast<char*>(a.out) + origin;
+  char* const pb = reinterpret_cast<char*>(a.pre) + origin;
+  const char* const rb = a.res + i * a.ldr + j * ES;
+  const uint32_t yo = (uint32_t)(lr * (int)pitch + lc * ES), ro = (uint32_t)(lr * (int)a.ldr + lc * ES);
+#pragma unroll
+  for (int v = 0; v < TJ; ++v) {
+    const int left_v = (int)(a.J - j) - v * 32 - lc;
+    float bias[16];
+    vql_bias<T, 16>(a, j + v * 32 + lc, bias);
+    u32x4 res[2][PV];
+    auto load = [&](int u, u32x4 (&to)[PV]) {
+#pragma unroll
+      for (int k = 0; k < PV; ++k) {
+        const char* p = rb + (int64_t)u * 32 * a.ldr + (v * 32 + k * E) * ES + ro;
+        if (INSIDE) to[k] = vql_load16<T>(p);
+        else to[k] = vql_load16_part<T>(p, i + u * 32 + lr < a.I ? left_v - k * E : 0);
+      }
+    };
+    if (a.res) load(0, res[0]);
+#pragma unroll
+    for (int u = 0; u < TI; ++u) {
+      if (a.res && u + 1 < TI) load(u + 1, res[(u + 1) & 1]);
+#pragma unroll
+      for (int k = 0; k < PV; ++k) {
+        float c[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) c[e] = acc[u][v][k * E + e];
+        const int64_t step = (int64_t)u * 32 * pitch + (v * 32 + k * E) * ES;
+        const int left = left_v - k * E;
+        if (INSIDE || (i + u * 32 + lr < a.I && left > 0))
+          vql_finish<T>(a, yb + step + yo, pb + step + yo, INSIDE ? E : left < E ? left : E, c, bias + k * E, res[u & 1][k]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
 // -------------------------------------------------------------------------------- one step
+// The lane number as a value that the compiler knows nothing about: what is computed from it inside a loop stays there,
+// instead of taking up registers all through the kernel.
+__device__ __forceinline__ int vql_fresh(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 template <int TI, int TJ>
 struct VqFrags {
   u32x4 a[TI], b[TJ];
@@ -458,143 +513,143 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
   constexpr int NT = WI * WJ * 64;
   constexpr int TI = BI / WI / 32, TJ = BJ / WJ / 32;
   constexpr int STAGE = (BI + BJ) * 128;
-  typedef VqOperand<T, AMM, BI, NT, DMA> OA;
-  typedef VqOperand<T, BMM, BJ, NT, DMA> OB;
+  typedef VqOperand<T, AMM, BI, NT, DMA, false> OA;
+  typedef VqOperand<T, BMM, BJ, NT, DMA, true> OB;
   extern __shared__ __attribute__((aligned(16))) char vql_lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
 
-  // Consecutive workgroups go to the 8 dies in turn: give each die a contiguous range of blocks, and walk the range in
-  // groups of 8 block rows, so that the blocks in flight on a die share their operands in its L2.
-  const int64_t per_split = a.tiles_i * a.tiles_j;
-  const int64_t total = per_split * a.splits;
-  const int64_t bid = blockIdx.x;
-  const int64_t q8 = total >> 3, r8 = total & 7, x8 = bid & 7;
-  int64_t id = x8 * q8 + (x8 < r8 ? x8 : r8) + (bid >> 3);
-  const int split = (int)(id / per_split);
-  id -= split * per_split;
-  const int64_t group = id / (8 * (int64_t)a.tiles_j);
-  const int64_t first = group * 8;
-  const int64_t gsz = a.tiles_i - first < 8 ? a.tiles_i - first : 8;
-  id -= group * 8 * a.tiles_j;
-  const int64_t ti0 = first + id % gsz;
-  const int tj0 = (int)(id / gsz);
-  const int64_t i0 = ti0 * BI;
-  const int64_t j0 = (int64_t)tj0 * BJ;
-
+  const int64_t per_split = a.tiles_i * a.tiles_j, total = per_split * a.splits;
   const int64_t steps = (a.R + OA::BK - 1) / OA::BK;
   const int64_t full = a.R / OA::BK;
-  const int64_t s0 = split * a.steps_per_split;
-  const int64_t s1 = s0 + a.steps_per_split < steps ? s0 + a.steps_per_split : steps;
-
+  VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
   OA oa;
   OB ob;
-  oa.init(a.A, a.lda, i0, a.I, wave, lane);
-  ob.init(a.B, a.ldb, j0, a.J, wave, lane);
+  int split = 0, tj0 = 0;
+  int64_t i0 = 0, j0 = 0, s0 = 0, s1 = 0;
 
-  f32x16 acc[TI][TJ];
-#pragma unroll
-  for (int u = 0; u < TI; ++u)
-#pragma unroll
-    for (int v = 0; v < TJ; ++v)
-#pragma unroll
-      for (int g = 0; g < 16; ++g) acc[u][v][g] = 0.0f;
-  const bool want_sum = AMM && (a.asum || a.gbias) && tj0 == 0 && wj == 0;
-  float asum[TI];
-#pragma unroll
-  for (int u = 0; u < TI; ++u) asum[u] = 0.0f;
-
-  // The sum.  NS tile pairs lie in LDS; the one that a step has used up is filled for the step NS later, by DMA where that
-  // step is a whole one, through registers otherwise.
-  VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
-  auto by_registers = [&](int64_t s, int at) {
-    u32x4 va[OA::PER], vb[OB::PER];
-    oa.fetch(s, a.R, wave, lane, va);
-    ob.fetch(s, a.R, wave, lane, vb);
-    oa.commit(lds + at, wave, lane, va);
-    ob.commit(lds + at + OA::BYTES, wave, lane, vb);
+  // Consecutive workgroups go to the 8 dies in turn: give each die a contiguous range of blocks, and walk the range in
+  // groups of 8 block rows, so that the blocks in flight on a die share their operands in its L2.
+  auto choose = [&](int64_t n) {
+    const int64_t q8 = total >> 3, r8 = total & 7, x8 = n & 7;
+    int64_t id = x8 * q8 + (x8 < r8 ? x8 : r8) + (n >> 3);
+    split = (int)(id / per_split);
+    id -= split * per_split;
+    const int64_t group = id / (8 * (int64_t)a.tiles_j);
+    const int64_t first = group * 8;
+    const int64_t gsz = a.tiles_i - first < 8 ? a.tiles_i - first : 8;
+    id -= group * 8 * a.tiles_j;
+    i0 = (first + id % gsz) * BI;
+    tj0 = (int)(id / gsz);
+    j0 = (int64_t)tj0 * BJ;
+    s0 = split * a.steps_per_split;
+    s1 = s0 + a.steps_per_split < steps ? s0 + a.steps_per_split : steps;
+    const int l = vql_fresh(lane);
+    oa.init(a.A, a.lda, i0, a.I, wave, l);
+    ob.init(a.B, a.ldb, j0, a.J, wave, l);
   };
-  if (s0 < s1) {
+  auto by_registers = [&](int64_t s, int at) {
+    const int l = vql_fresh(lane);
+    u32x4 va[OA::PER], vb[OB::PER];
+    oa.fetch(s, a.R, wave, l, va);
+    ob.fetch(s, a.R, wave, l, vb);
+    oa.commit(lds + at, wave, l, va);
+    ob.commit(lds + at + OA::BYTES, wave, l, vb);
+  };
+  // NS tile pairs lie in LDS; the one that a step has used up is filled for the step NS later, by DMA where that step is a
+  // whole one, through registers otherwise.  The first NS steps: the whole ones early (under the epilogue of the block
+  // before, whose accumulators leave no registers for the others), the rest late.
+  auto begin_early = [&]() {
+    if constexpr (DMA) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      if (DMA && s0 + n < s1 && s0 + n < full) {
-        oa.dma(s0 + n, lds + n * STAGE, wave);
-        ob.dma(s0 + n, lds + n * STAGE + OA::BYTES, wave);
-      } else if (s0 + n < s1) {
-        by_registers(s0 + n, n * STAGE);
-      }
-    }
-    vql_publish<0>();
-    VqFrags<TI, TJ> f[2];
-    vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
-    const int64_t last_dma = DMA ? (s1 < full ? s1 : full) : s0;      // steps from here on are filled through registers
-    int at = 0;
-    for (int64_t s = s0; s < s1; ++s) {
-      const int cur = at * STAGE;
-      at = at + 1 == NS ? 0 : at + 1;
-      vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(oa, ob, s + NS, s + NS < last_dma, s + 1 < s1,
-                                                                 s + NS - 1 < last_dma, lds, lds, cur, at * STAGE, wi, wj, wave,
-                                                                 lane, want_sum, f, acc, asum);
-      if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
-    }
-  }
-
-  if (AMM && want_sum) {
-#pragma unroll
-    for (int u = 0; u < TI; ++u) {
-      const float s = asum[u] + __shfl_xor(asum[u], 32);
-      const int64_t i = i0 + (wi * TI + u) * 32 + (lane & 31);
-      if (lane < 32 && i < a.I) {
-        if (a.splits > 1) a.asum[split * a.I + i] = s;
-        else reinterpret_cast<T*>(a.gbias)[i] = VqElem<T>::from(s);
-      }
-    }
-  }
-
-  // The accumulators hold 4 consecutive columns of one row per lane; through LDS (this wave's own part, 32 rows at a
-  // time) they become 16-byte pieces of rows, so that loads and stores of the epilogue are whole lines.
-  constexpr int PITCH = TJ * 32 + 4;
-  float* st = reinterpret_cast<float*>(vql_lds) + wave * 32 * PITCH;
-  const int64_t jw = j0 + wj * TJ * 32;
-#pragma unroll
-  for (int u = 0; u < TI; ++u) {
-#pragma unroll
-    for (int v = 0; v < TJ; ++v)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 w = {acc[u][v][4 * g], acc[u][v][4 * g + 1], acc[u][v][4 * g + 2], acc[u][v][4 * g + 3]};
-        *reinterpret_cast<vql_f32x4*>(st + (lane & 31) * PITCH + v * 32 + 8 * g + 4 * (lane >> 5)) = w;
-      }
-    __builtin_amdgcn_wave_barrier();
-    const int64_t iw = i0 + (wi * TI + u) * 32;
-    if (a.splits > 1) {
-      constexpr int LPR = TJ * 8;
-#pragma unroll
-      for (int n = 0; n < 32 * LPR / 64; ++n) {
-        const int row = n * (64 / LPR) + lane / LPR, col = (lane % LPR) * 4;
-        const f32x4 w = *reinterpret_cast<const vql_f32x4*>(st + row * PITCH + col);
-        if (iw + row < a.I && jw + col < a.ldp)
-          *reinterpret_cast<vql_f32x4*>(a.part + ((int64_t)split * a.I + iw + row) * a.ldp + jw + col) = w;
-      }
-    } else {
-      constexpr int E = 16 / sizeof(T), LPR = TJ * 32 / E;
-      const int col = (lane % LPR) * E;
-      float bias[E];
-      vql_bias16<T>(a, (int)jw + col, bias);
-#pragma unroll
-      for (int n = 0; n < 32 * LPR / 64; ++n) {
-        const int row = n * (64 / LPR) + lane / LPR;
-        float c[E];
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const f32x4 w = *reinterpret_cast<const vql_f32x4*>(st + row * PITCH + col + e);
-          c[e] = w[0]; c[e + 1] = w[1]; c[e + 2] = w[2]; c[e + 3] = w[3];
+      for (int k = 0; k < NS; ++k)
+        if (s0 + k < s1 && s0 + k < full) {
+          oa.dma(s0 + k, lds + k * STAGE, wave);
+          ob.dma(s0 + k, lds + k * STAGE + OA::BYTES, wave);
         }
-        if (iw + row < a.I && jw + col < a.J) vql_epilogue<T>(a, iw + row, (int)jw + col, c, bias);
+    }
+  };
+  auto begin_late = [&]() {
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+      if (s0 + k < s1 && (!DMA || s0 + k >= full)) by_registers(s0 + k, k * STAGE);
+  };
+
+  int64_t n = blockIdx.x;
+  choose(n);
+  begin_early();
+  for (;;) {
+    begin_late();
+    f32x16 acc[TI][TJ];
+#pragma unroll
+    for (int u = 0; u < TI; ++u)
+#pragma unroll
+      for (int v = 0; v < TJ; ++v)
+#pragma unroll
+        for (int g = 0; g < 16; ++g) acc[u][v][g] = 0.0f;
+    const bool want_sum = AMM && (a.asum || a.gbias) && tj0 == 0 && wj == 0;
+    float asum[TI];
+#pragma unroll
+    for (int u = 0; u < TI; ++u) asum[u] = 0.0f;
+
+    if (s0 < s1) {
+      vql_publish<0>();
+      VqFrags<TI, TJ> f[2];
+      vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
+      const int64_t last_dma = DMA ? (s1 < full ? s1 : full) : s0;      // steps from here on are filled through registers
+      int at = 0;
+      for (int64_t s = s0; s < s1; ++s) {
+        const int cur = at * STAGE;
+        at = at + 1 == NS ? 0 : at + 1;
+        vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(oa, ob, s + NS, s + NS < last_dma, s + 1 < s1,
+                                                                   s + NS - 1 < last_dma, lds, lds, cur, at * STAGE, wi, wj,
+                                                                   wave, lane, want_sum, f, acc, asum);
+        if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
       }
     }
-    __builtin_amdgcn_wave_barrier();
+
+    // What this block needs from here on; its LDS buffers are free (every wave has passed the last step's barrier), so that
+    // the next block's first tiles are on their way under the epilogue.
+    const int64_t iw = i0 + wi * TI * 32, jw = j0 + wj * TJ * 32;
+    const bool inside = i0 + BI <= a.I && j0 + BJ <= a.J;
+    const int this_split = split;
+    n += gridDim.x;
+    const bool more = n < total;
+    if (more) {
+      choose(n);
+      begin_early();
+    }
+
+    if (AMM && want_sum) {
+#pragma unroll
+      for (int u = 0; u < TI; ++u) {
+        const float s = asum[u] + __shfl_xor(asum[u], 32);
+        const int64_t i = iw + u * 32 + (lane & 31);
+        if (lane < 32 && i < a.I) {
+          if (a.splits > 1) a.asum[this_split * a.I + i] = s;
+          else reinterpret_cast<T*>(a.gbias)[i] = VqElem<T>::from(s);
+        }
+      }
+    }
+    if (a.splits > 1) {
+      const int l = vql_fresh(lane);
+#pragma unroll
+      for (int u = 0; u < TI; ++u)
+#pragma unroll
+        for (int v = 0; v < TJ; ++v)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 w = {acc[u][v][4 * g], acc[u][v][4 * g + 1], acc[u][v][4 * g + 2], acc[u][v][4 * g + 3]};
+            const int64_t i = iw + u * 32 + (l & 31), j = jw + v * 32 + 16 * (l >> 5) + 4 * g;
+            if (i < a.I && j < a.ldp) *reinterpret_cast<vql_f32x4*>(a.part + ((int64_t)this_split * a.I + i) * a.ldp + j) = w;
+          }
+    } else if (inside) {
+      vql_write<T, TI, TJ, true>(a, iw, jw, vql_fresh(lane), acc);
+    } else {
+      vql_write<T, TI, TJ, false>(a, iw, jw, vql_fresh(lane), acc);
+    }
+    if (!more) break;
   }
 }
 
@@ -610,14 +665,14 @@ namespace {
 template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
 struct VqProduct {
   static constexpr int LDS = NS * (BI + BJ) * 128;
-  static_assert(LDS >= WI * WJ * 32 * (BJ / WJ + 4) * 4, "the epilogue's staging fits the stage buffers");
   static const void* address() { return reinterpret_cast<const void*>(&vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, NS, DMA>); }
   static inline VqLdsRegistrar registrar{address(), LDS};
   static int launch(const VqLinearArgs& a, hipStream_t s) {
     (void)&registrar;
     const int rc = vq_lds_ensure(address(), LDS, nullptr);
     if (rc != VQ_OK) return rc;
-    const int64_t blocks = a.tiles_i * a.tiles_j * a.splits;
+    const int64_t total = a.tiles_i * a.tiles_j * a.splits;
+    const int64_t blocks = total < a.workgroups ? total : a.workgroups;
     hipLaunchKernelGGL((vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, NS, DMA>), dim3((unsigned)blocks), dim3(WI * WJ * 64), LDS, s, a);
     return vq_hip_status(hipGetLastError());
   }

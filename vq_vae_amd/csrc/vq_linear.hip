@@ -29,7 +29,7 @@ __device__ __forceinline__ f32x4 rows_mma(u32x4 a, u32x4 b, f32x4 c) {
   }
 }
 
-// One element of the epilogue (vql_epilogue does 16 bytes of them).
+// One element of the epilogue (vql_finish does 16 bytes of them).
 template <typename T>
 __device__ __forceinline__ void epilogue_one(const VqLinearArgs& a, int64_t i, int j, float c) {
   if (a.bias) c += VqElem<T>::to(reinterpret_cast<const T*>(a.bias)[j]);
@@ -114,8 +114,12 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a) {
         c[e] += v[0]; c[e + 1] += v[1]; c[e + 2] += v[2]; c[e + 3] += v[3];
       }
     }
-    vql_bias16<T>(a, j, bias);
-    vql_epilogue<T>(a, i, j, c, bias);
+    vql_bias<T, E>(a, j, bias);
+    const int left = a.J - j < E ? a.J - j : E;
+    u32x4 res = {0, 0, 0, 0};
+    if (a.res) res = vql_load16_part<T>(a.res + i * a.ldr + (int64_t)j * sizeof(T), left);
+    const int64_t at = (i * a.J + j) * (int64_t)sizeof(T);
+    vql_finish<T>(a, reinterpret_cast<char*>(a.out) + at, reinterpret_cast<char*>(a.pre) + at, left, c, bias, res);
   }
 }
 template <typename T>
@@ -172,6 +176,7 @@ struct Plan {
   int64_t steps_per_split;
   int64_t tiles_i;
   int tiles_j;
+  int workgroups;
   int ldp;
 };
 
@@ -197,7 +202,7 @@ Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
     return best;
   }
   static const struct { int tile, per_cu; double step16, step32, once; } cfg[3] = {
-      {64, 4, 0.30, 0.60, 2.0}, {128, 2, 0.50, 1.60, 3.0}, {256, 1, 0.90, 3.60, 6.0}};
+      {64, 3, 0.30, 0.60, 2.0}, {128, 2, 0.50, 1.60, 3.0}, {256, 1, 0.90, 3.60, 6.0}};
   const int64_t steps = (R * es + 127) / 128;
   double best_t = 1e300;
   for (int c = dma ? 2 : 1; c >= 0; --c) {
@@ -217,6 +222,7 @@ Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
         best.steps_per_split = per;
         best.tiles_i = ti;
         best.tiles_j = (int)tj;
+        best.workgroups = (int)slots;
       }
     }
   }
@@ -309,6 +315,7 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, void* work, 
   a.steps_per_split = p.steps_per_split;
   a.tiles_i = p.tiles_i;
   a.tiles_j = p.tiles_j;
+  a.workgroups = p.workgroups;
   a.ldp = p.ldp;
   if (p.splits > 1) {
     if (!work || !aligned16(work)) return VQ_ERR_INVALID_ARG;
@@ -357,7 +364,9 @@ extern "C" int vq_linear(const void* x, int64_t ldx, const void* W, int64_t ldw,
   if (M == 0) return VQ_OK;
   if (!x || !W || !y) return VQ_ERR_INVALID_ARG;
   const size_t es = elem_size(dtype);
-  if (K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || pitch_too_wide(ldx, es) || pitch_too_wide(ldw, es)) return VQ_ERR_UNSUPPORTED;
+  if (K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || pitch_too_wide(ldx, es) || pitch_too_wide(ldw, es) ||
+      (residual && pitch_too_wide(ldr, es)))
+    return VQ_ERR_UNSUPPORTED;
   VqLinearArgs a{};
   a.A = reinterpret_cast<const char*>(x);
   a.B = reinterpret_cast<const char*>(W);
