@@ -273,13 +273,18 @@ struct VqOperand {
       }
     }
   }
-  // a whole step (all BK values of r exist), straight into LDS
-  __device__ __forceinline__ void dma(int64_t step, VQL_LDS char* lds, int wave) const {
+  // a whole step (all BK values of r exist), straight into LDS: piece n of this thread's PER
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(int64_t step) const {
     const char* p = MMAJOR ? base + step * (BK * ld) : base + step * 128;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
+  }
+  __device__ __forceinline__ void dma_piece(__amdgpu_buffer_rsrc_t rs, int n, VQL_LDS char* lds, int wave) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (VQL_LDS void*)(lds + (wave * PER + n) * 1024), 16, off[n], 0, 0, 0);
+  }
+  __device__ __forceinline__ void dma(int64_t step, VQL_LDS char* lds, int wave) const {
+    const __amdgpu_buffer_rsrc_t rs = source(step);
 #pragma unroll
-    for (int n = 0; n < PER; ++n)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (VQL_LDS void*)(lds + (wave * PER + n) * 1024), 16, off[n], 0, 0, 0);
+    for (int n = 0; n < PER; ++n) dma_piece(rs, n, lds, wave);
   }
   // any step, by way of registers: indexes and r that do not exist read as zero
   __device__ __forceinline__ void fetch(int64_t step, int64_t R, int wave, int lane, u32x4 (&v)[PER]) const {
@@ -450,15 +455,19 @@ __device__ __forceinline__ void vql_read(VqFrags<TI, TJ>& f, const VQL_LDS char*
   for (int v = 0; v < TJ; ++v) f.b[v] = OB::frag(tile + OA::BYTES, (wj * TJ + v) * 32, q, lane);
 }
 template <typename T, bool SUMS, int TI, int TJ>
+__device__ __forceinline__ void vql_add(const VqFrags<TI, TJ>& f, bool want_sum, float (&asum)[TI]) {
+  if (SUMS && want_sum) {
+#pragma unroll
+    for (int u = 0; u < TI; ++u) asum[u] += vql_sum16<T>(f.a[u]);
+  }
+}
+template <typename T, bool SUMS, int TI, int TJ>
 __device__ __forceinline__ void vql_mul(const VqFrags<TI, TJ>& f, bool want_sum, f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
 #pragma unroll
   for (int u = 0; u < TI; ++u)
 #pragma unroll
     for (int v = 0; v < TJ; ++v) acc[u][v] = vql_mma<T>(f.b[v], f.a[u], acc[u][v]);
-  if (SUMS && want_sum) {
-#pragma unroll
-    for (int u = 0; u < TI; ++u) asum[u] += vql_sum16<T>(f.a[u]);
-  }
+  vql_add<T, SUMS, TI, TJ>(f, want_sum, asum);
 }
 // Waits until at most `n` of this wave's DMA instructions are in flight and its LDS accesses are done, then for the
 // other waves.  A bare barrier: nothing else has to have landed.
@@ -493,14 +502,24 @@ __device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma
   }
   if (FLYING > 0 && counted) vql_publish<FLYING>();
   else vql_publish<0>();
-  if (dma) {
-    oa.dma(dma_step, into + cur, wave);
-    ob.dma(dma_step, into + cur + OA::BYTES, wave);
-  }
   if (more) vql_read<OA, OB, TI, TJ>(f[0], from + nxt, 0, wi, wj, lane);
   __builtin_amdgcn_sched_barrier(0);
-  vql_mul<T, OA::SUMS, TI, TJ>(f[1], want_sum, acc, asum);
-  __builtin_amdgcn_sched_barrier(0);
+  // the DMA instructions one by one between the products
+  const __amdgpu_buffer_rsrc_t ra = oa.source(dma_step), rb = ob.source(dma_step);
+  constexpr int PIECES = OA::PER + OB::PER, EACH = (PIECES + TI * TJ - 1) / (TI * TJ);
+#pragma unroll
+  for (int m = 0; m < TI * TJ; ++m) {
+    acc[m / TJ][m % TJ] = vql_mma<T>(f[1].b[m % TJ], f[1].a[m / TJ], acc[m / TJ][m % TJ]);
+    if (dma && m * EACH < PIECES) {
+#pragma unroll
+      for (int k = m * EACH; k < (m + 1) * EACH && k < PIECES; ++k) {
+        if (k < OA::PER) oa.dma_piece(ra, k, into + cur, wave);
+        else ob.dma_piece(rb, k - OA::PER, into + cur + OA::BYTES, wave);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  vql_add<T, OA::SUMS, TI, TJ>(f[1], want_sum, asum);
 }
 
 // -------------------------------------------------------------------------------- the product
