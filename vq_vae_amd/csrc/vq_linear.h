@@ -35,8 +35,7 @@ struct VqLinearArgs {
   const char* res;           // [I][J] or null
   int64_t ldr;               // bytes between rows of res
   int act;
-  float* part;               // splits > 1: [splits][I][ldp] partial sums
-  int ldp;
+  float* part;               // splits > 1: the partial sums, as the product kernel's registers lie
   float* asum;               // weight gradient: the sums of A over r (the bias gradient) of a split sum, [splits][I], or null
   void* gbias;               // the same in T, where the sum is not split
 };
@@ -95,6 +94,19 @@ __device__ __forceinline__ u32x4 vql_load16_part(const char* p, int64_t valid) {
       else
         v[e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(p + 2 * e) << (16 * (e & 1));
     }
+  return v;
+}
+
+// v moved down by `by` elements (0 .. all of them), zeros behind
+template <typename T>
+__device__ __forceinline__ u32x4 vql_shift(u32x4 v, int by) {
+  if constexpr (sizeof(T) == 2) {
+    if (by & 1) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    by >>= 1;
+  }
+  if (by & 1) v = u32x4{v[1], v[2], v[3], 0};
+  if (by & 2) v = u32x4{v[2], v[3], 0, 0};
+  if (by & 4) v = u32x4{0, 0, 0, 0};
   return v;
 }
 
@@ -245,7 +257,7 @@ struct VqOperand {
   static constexpr bool SUMS = MMAJOR;                 // only the weight gradient's A operand is summed
   const char* base;      // m-major: column m0 of row 0; r-major: row m0
   int64_t ld;            // bytes
-  int64_t M;             // indexes that exist from m0 on
+  int64_t M, total;      // indexes that exist from m0 on, and altogether
   uint32_t off[PER];     // this lane's byte offsets of a full step
 
   __device__ __forceinline__ static int rswz(int row) { return ORDERED ? ((row >> 1) & 3) | ((row >> 2) & 4) : row >> 1; }
@@ -254,9 +266,10 @@ struct VqOperand {
     row = p / CPR;
     piece = (p % CPR) ^ ((MMAJOR ? vql_mswz<T>(row) : rswz(row)) & SWZ);
   }
-  __device__ __forceinline__ void init(const char* src, int64_t ld_, int64_t m0, int64_t total, int wave, int lane) {
+  __device__ __forceinline__ void init(const char* src, int64_t ld_, int64_t m0, int64_t all, int wave, int lane) {
     ld = ld_;
-    M = total - m0;
+    total = all;
+    M = all - m0;
     base = MMAJOR ? src + m0 * ES : src + m0 * ld_;
     if constexpr (DMA) {
 #pragma unroll
@@ -286,23 +299,80 @@ struct VqOperand {
 #pragma unroll
     for (int n = 0; n < PER; ++n) dma_piece(rs, n, lds, wave);
   }
-  // any step, by way of registers: indexes and r that do not exist read as zero
+  // Any step, by way of registers.  All loads are 16 bytes and unconditional wherever the row has 16 bytes at all, so that
+  // they are on their way together: rows that do not exist read the last one instead, a piece that passes the end of its
+  // row is read from the row's last 16 bytes and shifted.  What must read as zero does (r behind the end); indexes that do
+  // not exist may hold anything finite or not: they reach only outputs that are not stored.
   __device__ __forceinline__ void fetch(int64_t step, int64_t R, int wave, int lane, u32x4 (&v)[PER]) const {
+    const int64_t r0 = step * BK;
+    const char* const tile = MMAJOR ? base + r0 * ld : base + r0 * ES;
+    const int rs = (int)(R - r0 < BK ? R - r0 : BK), ms = (int)(M < B ? M : B);      // r and indexes that exist in the tile
+    const int pitch = (int)ld;
+    if (rs == BK && (!MMAJOR || ms == B)) {
 #pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        int row, piece;
+        where(n, wave, lane, row, piece);
+        if (!MMAJOR) row = row < ms ? row : ms - 1;
+        v[n] = vql_load16<T>(tile + (uint32_t)(row * pitch + piece * 16));
+      }
+    } else if ((MMAJOR ? total : R) >= E) {
+      // a piece that passes the end of its row: from where the row's last 16 bytes start
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        int row, piece;
+        where(n, wave, lane, row, piece);
+        const int last = (MMAJOR ? ms : rs) - E, at = piece * E < last ? piece * E : last;
+        row = row < (MMAJOR ? rs : ms) ? row : (MMAJOR ? rs : ms) - 1;
+        v[n] = vql_load16<T>(tile + (row * pitch + at * ES));
+      }
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        int row, piece;
+        where(n, wave, lane, row, piece);
+        const int over = piece * E - (MMAJOR ? ms : rs) + E;
+        v[n] = vql_shift<T>(v[n], (MMAJOR && row >= rs) || over > E ? E : over > 0 ? over : 0);
+      }
+    } else {   // rows of less than 16 bytes
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        int row, piece;
+        where(n, wave, lane, row, piece);
+        v[n] = fetch_part(tile, row, piece, rs, ms);
+      }
+    }
+  }
+  // one piece, element by element
+  __device__ __forceinline__ u32x4 fetch_part(const char* tile, int row, int piece, int rs, int ms) const {
+    const bool exists = row < (MMAJOR ? rs : ms);
+    const int have = exists ? (MMAJOR ? ms : rs) - piece * E : 0;
+    const char* p = tile + (uint32_t)(exists ? row * (int)ld + piece * 16 : 0);
+    u32x4 v = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int e = (have < E ? have : E) - 1; e >= 0; --e) {   // from the last element on, each moving the others up
+      if constexpr (ES == 4) {
+        v = u32x4{*reinterpret_cast<const vql_u32*>(p + 4 * e), v[0], v[1], v[2]};
+      } else {
+        const uint32_t x = *reinterpret_cast<const vql_u16*>(p + 2 * e);
+        v = u32x4{v[0] << 16 | x, v[1] << 16 | v[0] >> 16, v[2] << 16 | v[1] >> 16, v[3] << 16 | v[2] >> 16};
+      }
+    }
+    return v;
+  }
+  // a step that is not a whole one, into LDS piece by piece: once in a sum, and with few registers
+  __device__ __forceinline__ void fill_part(int64_t step, int64_t R, VQL_LDS char* lds, int wave, int lane) const {
+    const int64_t r0 = step * BK;
+    const char* const tile = MMAJOR ? base + r0 * ld : base + r0 * ES;
+    const int rs = (int)(R - r0 < BK ? R - r0 : BK), ms = (int)(M < B ? M : B);
+#pragma unroll 1
     for (int n = 0; n < PER; ++n) {
       int row, piece;
       where(n, wave, lane, row, piece);
-      const int64_t r0 = step * BK;
-      int64_t valid;
-      const char* p;
-      if constexpr (MMAJOR) {
-        valid = r0 + row < R ? M - piece * E : 0;
-        p = base + (r0 + row) * ld + piece * 16;
-      } else {
-        valid = row < M ? R - r0 - piece * E : 0;
-        p = base + row * ld + r0 * ES + piece * 16;
-      }
-      v[n] = vql_load16_part<T>(p, valid);
+      const int have = row < (MMAJOR ? rs : ms) ? (MMAJOR ? ms : rs) - piece * E : 0;
+      u32x4 v;
+      if (have >= E) v = vql_load16<T>(tile + (uint32_t)(row * (int)ld + piece * 16));
+      else v = fetch_part(tile, row, piece, rs, ms);
+      *reinterpret_cast<VQL_LDS vql_u32x4_a16*>(lds + ((wave * PER + n) * 64 + lane) * 16) = v;
     }
   }
   __device__ __forceinline__ void commit(VQL_LDS char* lds, int wave, int lane, const u32x4 (&v)[PER]) const {
@@ -388,6 +458,23 @@ __device__ __forceinline__ void vql_bias(const VqLinearArgs& a, int64_t j, float
 #pragma unroll
       for (int e = 0; e < E; ++e) bias[k * E + e] = VqElem<T>::to(b.e[e]);
     }
+  }
+}
+// The epilogue of 16 columns cv .. cv + 15 of row r out of the values that one lane holds of one tile; what does not exist
+// is left out.
+template <typename T>
+__device__ __forceinline__ void vql_write16(const VqLinearArgs& a, int64_t r, int64_t cv, const float (&c)[16]) {
+  constexpr int ES = sizeof(T), E = 16 / ES, PV = 16 / E;
+  float bias[16];
+  vql_bias<T, 16>(a, cv, bias);
+#pragma unroll
+  for (int k = 0; k < PV; ++k) {
+    const int64_t left = a.J - cv - k * E, at = (r * a.J + cv + k * E) * ES;
+    if (r >= a.I || left <= 0) continue;
+    u32x4 res = {0, 0, 0, 0};
+    if (a.res) res = vql_load16_part<T>(a.res + r * a.ldr + (cv + k * E) * ES, left);
+    vql_finish<T>(a, reinterpret_cast<char*>(a.out) + at, reinterpret_cast<char*>(a.pre) + at, left < E ? (int)left : E, c + k * E,
+                  bias + k * E, res);
   }
 }
 // The epilogue of a wave's part of a block: rows i .. i + 32 TI, columns j .. j + 32 TJ.  A lane holds 16 consecutive
@@ -489,12 +576,33 @@ __device__ __forceinline__ void vql_publish() {
 // are the same memory; __restrict__ tells the compiler that a fragment read need not wait for the DMA in flight: the
 // barriers and the counted waits see to that.
 template <typename T, typename OA, typename OB, int TI, int TJ, int FLYING>
-__device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma_step, bool dma, bool more, bool counted,
-                                         VQL_LDS char* __restrict__ into, const VQL_LDS char* __restrict__ from, int cur, int nxt,
+__device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma_step, bool dma, bool pending, bool more, bool counted,
+                                         VQL_LDS char* __restrict__ into, const VQL_LDS char* __restrict__ from, int cur, int nxt, int prev,
                                          int wi, int wj, int wave, int lane, bool want_sum, VqFrags<TI, TJ> (&f)[2],
                                          f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
+  constexpr int PIECES = OA::PER + OB::PER, FIRST = PIECES / 2, PROD = TI * TJ;
+  auto piece = [&](__amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int k, VQL_LDS char* to) {
+    if (k < OA::PER) oa.dma_piece(ra, k, to, wave);
+    else ob.dma_piece(rb, k - OA::PER, to + OA::BYTES, wave);
+  };
+  {
+    vql_read<OA, OB, TI, TJ>(f[1], from + cur, 1, wi, wj, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    const __amdgpu_buffer_rsrc_t ra = oa.source(dma_step - 1), rb = ob.source(dma_step - 1);
+    constexpr int N = PIECES - FIRST, EACH = (N + PROD - 1) / PROD;
 #pragma unroll
-  for (int q = 0; q < 3; ++q) {
+    for (int m = 0; m < PROD; ++m) {
+      acc[m / TJ][m % TJ] = vql_mma<T>(f[0].b[m % TJ], f[0].a[m / TJ], acc[m / TJ][m % TJ]);
+      if (pending && m * EACH < N) {
+#pragma unroll
+        for (int k = m * EACH; k < (m + 1) * EACH && k < N; ++k) piece(ra, rb, FIRST + k, into + prev);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    vql_add<T, OA::SUMS, TI, TJ>(f[0], want_sum, asum);
+  }
+#pragma unroll
+  for (int q = 1; q < 3; ++q) {
     vql_read<OA, OB, TI, TJ>(f[(q + 1) & 1], from + cur, q + 1, wi, wj, lane);
     __builtin_amdgcn_sched_barrier(0);
     vql_mul<T, OA::SUMS, TI, TJ>(f[q & 1], want_sum, acc, asum);
@@ -506,16 +614,13 @@ __device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma
   __builtin_amdgcn_sched_barrier(0);
   // the DMA instructions one by one between the products
   const __amdgpu_buffer_rsrc_t ra = oa.source(dma_step), rb = ob.source(dma_step);
-  constexpr int PIECES = OA::PER + OB::PER, EACH = (PIECES + TI * TJ - 1) / (TI * TJ);
+  constexpr int EACH = (FIRST + PROD - 1) / PROD;
 #pragma unroll
   for (int m = 0; m < TI * TJ; ++m) {
     acc[m / TJ][m % TJ] = vql_mma<T>(f[1].b[m % TJ], f[1].a[m / TJ], acc[m / TJ][m % TJ]);
-    if (dma && m * EACH < PIECES) {
+    if (dma && m * EACH < FIRST) {
 #pragma unroll
-      for (int k = m * EACH; k < (m + 1) * EACH && k < PIECES; ++k) {
-        if (k < OA::PER) oa.dma_piece(ra, k, into + cur, wave);
-        else ob.dma_piece(rb, k - OA::PER, into + cur + OA::BYTES, wave);
-      }
+      for (int k = m * EACH; k < (m + 1) * EACH && k < FIRST; ++k) piece(ra, rb, k, into + cur);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -570,11 +675,8 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
   };
   auto by_registers = [&](int64_t s, int at) {
     const int l = vql_fresh(lane);
-    u32x4 va[OA::PER], vb[OB::PER];
-    oa.fetch(s, a.R, wave, l, va);
-    ob.fetch(s, a.R, wave, l, vb);
-    oa.commit(lds + at, wave, l, va);
-    ob.commit(lds + at + OA::BYTES, wave, l, vb);
+    oa.fill_part(s, a.R, lds + at, wave, l);
+    ob.fill_part(s, a.R, lds + at + OA::BYTES, wave, l);
   };
   // NS tile pairs lie in LDS; the one that a step has used up is filled for the step NS later, by DMA where that step is a
   // whole one, through registers otherwise.  The first NS steps: the whole ones early (under the epilogue of the block
@@ -590,9 +692,11 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     }
   };
   auto begin_late = [&]() {
-#pragma unroll
-    for (int k = 0; k < NS; ++k)
-      if (s0 + k < s1 && (!DMA || s0 + k >= full)) by_registers(s0 + k, k * STAGE);
+    if constexpr (DMA) {
+#pragma unroll 1
+      for (int k = 0; k < NS; ++k)
+        if (s0 + k < s1 && s0 + k >= full) by_registers(s0 + k, k * STAGE);
+    }
   };
 
   int64_t n = blockIdx.x;
@@ -613,18 +717,56 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     for (int u = 0; u < TI; ++u) asum[u] = 0.0f;
 
     if (s0 < s1) {
-      vql_publish<0>();
       VqFrags<TI, TJ> f[2];
-      vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
-      const int64_t last_dma = DMA ? (s1 < full ? s1 : full) : s0;      // steps from here on are filled through registers
-      int at = 0;
-      for (int64_t s = s0; s < s1; ++s) {
-        const int cur = at * STAGE;
-        at = at + 1 == NS ? 0 : at + 1;
-        vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(oa, ob, s + NS, s + NS < last_dma, s + 1 < s1,
-                                                                   s + NS - 1 < last_dma, lds, lds, cur, at * STAGE, wi, wj,
-                                                                   wave, lane, want_sum, f, acc, asum);
-        if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
+      if constexpr (DMA) {
+        const int64_t last_dma = s1 < full ? s1 : full;      // steps from here on are filled through registers
+        if (s0 + NS <= last_dma) vql_publish<(NS - 1) * (OA::PER + OB::PER)>();
+        else vql_publish<0>();
+        vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
+        int at = 0;
+        for (int64_t s = s0; s < s1; ++s) {
+          const int cur = at * STAGE, prev = at == 0 ? (NS - 1) * STAGE : cur - STAGE;
+          at = at + 1 == NS ? 0 : at + 1;
+          vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(
+              oa, ob, s + NS, s + NS < last_dma, s > s0 && s + NS - 1 < last_dma, s + 1 < s1, s + NS - 1 < last_dma, lds, lds,
+              cur, at * STAGE, prev, wi, wj, wave, lane, want_sum, f, acc, asum);
+          if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
+        }
+      } else {
+        // the same steps with two buffers; the tiles of the next step wait in registers while this one is worked on
+        u32x4 va[OA::PER], vb[OB::PER];
+        auto fetch = [&](int64_t s) {
+          const int l = vql_fresh(lane);
+          oa.fetch(s, a.R, wave, l, va);
+          ob.fetch(s, a.R, wave, l, vb);
+        };
+        fetch(s0);
+        oa.commit(lds, wave, lane, va);
+        ob.commit(lds + OA::BYTES, wave, lane, vb);
+        if (s0 + 1 < s1) fetch(s0 + 1);
+        vql_publish<63>();
+        vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
+        int cur = 0;
+        for (int64_t s = s0; s < s1; ++s) {
+#pragma unroll
+          for (int q = 0; q < 3; ++q) {
+            vql_read<OA, OB, TI, TJ>(f[(q + 1) & 1], lds + cur, q + 1, wi, wj, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            vql_mul<T, OA::SUMS, TI, TJ>(f[q & 1], want_sum, acc, asum);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          cur ^= STAGE;
+          if (s + 1 < s1) {
+            oa.commit(lds + cur, wave, lane, va);
+            ob.commit(lds + cur + OA::BYTES, wave, lane, vb);
+          }
+          vql_publish<63>();
+          if (s + 2 < s1) fetch(s + 2);
+          if (s + 1 < s1) vql_read<OA, OB, TI, TJ>(f[0], lds + cur, 0, wi, wj, lane);
+          __builtin_amdgcn_sched_barrier(0);
+          vql_mul<T, OA::SUMS, TI, TJ>(f[1], want_sum, acc, asum);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
 
@@ -632,7 +774,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     // the next block's first tiles are on their way under the epilogue.
     const int64_t iw = i0 + wi * TI * 32, jw = j0 + wj * TJ * 32;
     const bool inside = i0 + BI <= a.I && j0 + BJ <= a.J;
-    const int this_split = split;
+    const int64_t this_split = split, this_block = i0 / BI * a.tiles_j + tj0;
     n += gridDim.x;
     const bool more = n < total;
     if (more) {
@@ -652,7 +794,8 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
       }
     }
     if (a.splits > 1) {
-      const int l = vql_fresh(lane);
+      // as the registers lie, 1 KiB an instruction: [split][block][wave][32x32 tile][4 groups of 4 columns][lane][4]
+      float* to = a.part + ((this_split * per_split + this_block) * WI * WJ + wave) * (TI * TJ * 1024) + vql_fresh(lane) * 4;
 #pragma unroll
       for (int u = 0; u < TI; ++u)
 #pragma unroll
@@ -660,8 +803,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const f32x4 w = {acc[u][v][4 * g], acc[u][v][4 * g + 1], acc[u][v][4 * g + 2], acc[u][v][4 * g + 3]};
-            const int64_t i = iw + u * 32 + (l & 31), j = jw + v * 32 + 16 * (l >> 5) + 4 * g;
-            if (i < a.I && j < a.ldp) *reinterpret_cast<vql_f32x4*>(a.part + ((int64_t)this_split * a.I + i) * a.ldp + j) = w;
+            *reinterpret_cast<vql_f32x4*>(to + ((u * TJ + v) * 4 + g) * 256) = w;
           }
     } else if (inside) {
       vql_write<T, TI, TJ, true>(a, iw, jw, vql_fresh(lane), acc);

@@ -45,19 +45,15 @@ __global__ __launch_bounds__(1024) void vql_rows_kernel(VqLinearArgs a) {
   __shared__ float part[16][16 * 20];             // [wave][row][channel, padded]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int split = blockIdx.y;
   const int sub = lane & 15, piece = lane >> 4;
   const int64_t n = n0 + sub < a.J ? n0 + sub : a.J - 1;
   const int64_t m = sub < a.I ? sub : a.I - 1;    // rows and channels that do not exist repeat the last one, unstored
   const char* wp = a.B + n * a.ldb + piece * 16;
   const char* xp = a.A + m * a.lda + piece * 16;
   const int64_t steps = (a.R + KS - 1) / KS, full = a.R / KS;
-  // this workgroup's range of the sum, then this wave's
-  const int64_t g0 = split * a.steps_per_split;
-  const int64_t g1 = g0 + a.steps_per_split < steps ? g0 + a.steps_per_split : steps;
-  const int64_t per = (g1 - g0 + waves - 1) / waves;
-  int64_t s = g0 + wave * per;
-  const int64_t s1 = s + per < g1 ? s + per : g1;
+  const int64_t per = (steps + waves - 1) / waves;   // this wave's range of the sum
+  int64_t s = wave * per;
+  const int64_t s1 = s + per < steps ? s + per : steps;
   const int64_t sf = s1 < full ? s1 : full;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   for (; s + ROWS_UNROLL <= sf; s += ROWS_UNROLL) {
@@ -80,19 +76,17 @@ __global__ __launch_bounds__(1024) void vql_rows_kernel(VqLinearArgs a) {
     if (row >= a.I || n0 + col >= a.J) continue;
     float c = 0.0f;
     for (int w = 0; w < waves; ++w) c += part[w][row * 20 + col];
-    if (a.splits > 1) a.part[((int64_t)split * a.I + row) * a.ldp + n0 + col] = c;
-    else epilogue_one<T>(a, row, (int)(n0 + col), c);
+    epilogue_one<T>(a, row, (int)(n0 + col), c);
   }
 }
 
 // ------------------------------------------------------------------------------ join of a split sum
-// Adds the partial sums in split order (the same bits on every run) and applies the epilogue.
+// Adds the partial sums and applies the epilogue: a workgroup per 32x32 tile, a lane per 16 columns of a row as in the
+// product kernel; wave k adds the splits k, k + 4, .., then the four sums are added in order (the same bits on every run).
 template <typename T>
-__global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a) {
-  constexpr int E = 16 / sizeof(T);
-  const int64_t cols = (a.J + E - 1) / E;
-  const int64_t count = a.I * cols;
-  const int64_t size = a.I * a.ldp;
+__global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a, int tile, int waves_j, int tiles_u, int tiles_v) {
+  __shared__ f32x4 sums[3][4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (a.asum) {   // weight gradient: the bias gradient's partial sums too
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.I; i += (int64_t)gridDim.x * 256) {
       float c = 0.0f;
@@ -100,27 +94,30 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a) {
       reinterpret_cast<T*>(a.gbias)[i] = VqElem<T>::from(c);
     }
   }
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < count; t += (int64_t)gridDim.x * 256) {
-    const int64_t i = t / cols;
-    const int j = (int)(t - i * cols) * E;
-    float c[E], bias[E];
+  const int per_block = tile * tile / 1024;                 // 32x32 tiles of a block
+  const int64_t block = blockIdx.x / per_block, blocks = a.tiles_i * a.tiles_j;
+  const int sub = blockIdx.x % per_block;
+  const int w = sub / (tiles_u * tiles_v), u = sub / tiles_v % tiles_u, v = sub % tiles_v;
+  const int64_t r = block / a.tiles_j * tile + ((w / waves_j) * tiles_u + u) * 32 + (lane & 31);
+  const int64_t cv = block % a.tiles_j * tile + ((w % waves_j) * tiles_v + v) * 32 + 16 * (lane >> 5);
+  f32x4 c[4] = {};
+  const float* p = a.part + (block * per_block + sub) * 1024 + lane * 4;
+  for (int s = wave; s < a.splits; s += 4)
 #pragma unroll
-    for (int e = 0; e < E; ++e) c[e] = 0.0f;
-    const float* p = a.part + i * a.ldp + j;
-    for (int s = 0; s < a.splits; ++s, p += size) {
+    for (int g = 0; g < 4; ++g) c[g] += *reinterpret_cast<const vql_f32x4*>(p + s * blocks * per_block * 1024 + g * 256);
+  if (wave > 0)
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const f32x4 v = *reinterpret_cast<const vql_f32x4*>(p + e);
-        c[e] += v[0]; c[e + 1] += v[1]; c[e + 2] += v[2]; c[e + 3] += v[3];
-      }
-    }
-    vql_bias<T, E>(a, j, bias);
-    const int left = a.J - j < E ? a.J - j : E;
-    u32x4 res = {0, 0, 0, 0};
-    if (a.res) res = vql_load16_part<T>(a.res + i * a.ldr + (int64_t)j * sizeof(T), left);
-    const int64_t at = (i * a.J + j) * (int64_t)sizeof(T);
-    vql_finish<T>(a, reinterpret_cast<char*>(a.out) + at, reinterpret_cast<char*>(a.pre) + at, left, c, bias, res);
+    for (int g = 0; g < 4; ++g) sums[wave - 1][g][lane] = c[g];
+  __syncthreads();
+  if (wave > 0) return;
+  float all[16];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 t = ((c[g] + sums[0][g][lane]) + sums[1][g][lane]) + sums[2][g][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) all[4 * g + e] = t[e];
   }
+  vql_write16<T>(a, r, cv, all);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, int splits, int64_t n, T* out) {
@@ -177,7 +174,6 @@ struct Plan {
   int64_t tiles_i;
   int tiles_j;
   int workgroups;
-  int ldp;
 };
 
 constexpr int CUS = 256;
@@ -190,15 +186,11 @@ size_t elem_size(int dtype) { return dtype == VQ_F32 ? 4 : 2; }
 Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
   const size_t es = elem_size(dtype);
   Plan best{};
-  best.ldp = (J + 7) & ~7;
-  if (layout == 0 && I <= ROWS_MAX) {
+  // Few rows: the kernel that reads W once, with 16 channels to a workgroup.  A sum of more than 32 KiB a channel over few
+  // channels leaves most of the device idle there: the tiled kernel splits it.
+  if (layout == 0 && I <= ROWS_MAX && ((J + 15) / 16 * 4 > CUS || R * es <= 32768)) {
     best.rows = true;
-    const int64_t steps = (R * es + 63) / 64, groups = (J + 15) / 16;
-    // a workgroup's 16 waves take 8 steps each before a second round; the join costs more than 32 steps a wave
-    int64_t splits = 1;
-    if (groups * 4 <= CUS && steps > 16 * 32) splits = std::min<int64_t>((steps + 16 * 16 - 1) / (16 * 16), CUS / groups);
-    best.steps_per_split = (steps + splits - 1) / splits;
-    best.splits = (int)((steps + best.steps_per_split - 1) / best.steps_per_split);
+    best.splits = 1;
     return best;
   }
   static const struct { int tile, per_cu; double step16, step32, once; } cfg[3] = {
@@ -229,8 +221,9 @@ Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
   return best;
 }
 
-int64_t part_bytes(const Plan& p, int64_t I) {
-  return p.splits > 1 ? (int64_t)p.splits * I * p.ldp * 4 : 0;
+constexpr int TILE[3] = {64, 128, 256};
+int64_t part_bytes(const Plan& p) {
+  return p.splits > 1 ? p.splits * p.tiles_i * p.tiles_j * TILE[p.config] * TILE[p.config] * 4 : 0;
 }
 // row slabs of vql_colsum_kernel
 int64_t colsum_slabs(int64_t M, int N) {
@@ -261,19 +254,20 @@ int by_type(int dtype, Args&&... args) {
 }
 template <typename T> struct RunRows {
   static int run(const VqLinearArgs& a, hipStream_t s) {
-    const int64_t steps = std::min<int64_t>(a.steps_per_split, (a.R * (int64_t)sizeof(T) + 63) / 64);
+    const int64_t steps = (a.R * (int64_t)sizeof(T) + 63) / 64;
     int waves = 1;
     while (waves < 16 && waves * 2 < steps) waves *= 2;   // two steps or more a wave
     if (waves < 4) waves = 4;                             // four waves write the 256 results
-    hipLaunchKernelGGL(vql_rows_kernel<T>, dim3((unsigned)((a.J + 15) / 16), (unsigned)a.splits), dim3(waves * 64), 0, s, a);
+    hipLaunchKernelGGL(vql_rows_kernel<T>, dim3((unsigned)((a.J + 15) / 16)), dim3(waves * 64), 0, s, a);
     return vq_hip_status(hipGetLastError());
   }
 };
 template <typename T> struct RunJoin {
-  static int run(const VqLinearArgs& a, hipStream_t s) {
-    constexpr int E = 16 / sizeof(T);
-    const int64_t blocks = std::min<int64_t>((a.I * ((a.J + E - 1) / E) + 255) / 256, 8192);
-    hipLaunchKernelGGL(vql_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+  static int run(const VqLinearArgs& a, int config, hipStream_t s) {
+    const int tile = TILE[config], waves_j = config == VQL_C256 ? 4 : 2;
+    const int tiles_u = config == VQL_C256 ? 4 : tile / 64, tiles_v = config == VQL_C256 ? 2 : tile / 64;
+    const int64_t blocks = a.tiles_i * a.tiles_j * tile * tile / 1024;
+    hipLaunchKernelGGL(vql_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a, tile, waves_j, tiles_u, tiles_v);
     return vq_hip_status(hipGetLastError());
   }
 };
@@ -316,21 +310,16 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, void* work, 
   a.tiles_i = p.tiles_i;
   a.tiles_j = p.tiles_j;
   a.workgroups = p.workgroups;
-  a.ldp = p.ldp;
   if (p.splits > 1) {
     if (!work || !aligned16(work)) return VQ_ERR_INVALID_ARG;
     a.part = reinterpret_cast<float*>(work);
   }
-  if (p.rows) {
-    int rc = by_type<RunRows>(dtype, a, s);
-    if (rc == VQ_OK && a.splits > 1) rc = by_type<RunJoin>(dtype, a, s);
-    return rc;
-  }
+  if (p.rows) return by_type<RunRows>(dtype, a, s);
   if (p.tiles_i * p.tiles_j * p.splits >= (int64_t)1 << 23) return VQ_ERR_UNSUPPORTED;
   a.gbias = gbias;
-  if (gbias && p.splits > 1) a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p, a.I));
+  if (gbias && p.splits > 1) a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p));
   int rc = product(a, layout, dtype, p.config, dma, s);
-  if (rc == VQ_OK && a.splits > 1) rc = by_type<RunJoin>(dtype, a, s);
+  if (rc == VQ_OK && a.splits > 1) rc = by_type<RunJoin>(dtype, a, p.config, s);
   return rc;
 }
 
@@ -338,7 +327,7 @@ int64_t product_work(int layout, int64_t I, int J, int64_t R, int dtype, bool su
   int64_t bytes = 0;
   for (int dma = 0; dma < 2; ++dma) {
     const Plan p = make_plan(layout, I, J, R, dtype, dma);
-    bytes = std::max(bytes, part_bytes(p, I) + (sums && p.splits > 1 ? (int64_t)p.splits * I * 4 : 0));
+    bytes = std::max(bytes, part_bytes(p) + (sums && p.splits > 1 ? (int64_t)p.splits * I * 4 : 0));
   }
   return bytes;
 }
