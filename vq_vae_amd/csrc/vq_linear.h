@@ -15,7 +15,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct VqBf16 { uint16_t v; };   // element types of the templates: float, VqBf16, _Float16
 
-enum { VQL_C64 = 0, VQL_C128 = 1, VQL_C256 = 2 };
+// tiles of the product kernel
+enum { VQL_C64 = 0, VQL_C128 = 1, VQL_C256 = 2, VQL_CONFIGS = 3 };
 
 struct VqLinearArgs {
   const char* A;
@@ -24,7 +25,7 @@ struct VqLinearArgs {
   int64_t I;                 // rows of C
   int J;                     // columns of C
   int64_t R;                 // length of the sum
-  int64_t steps_per_split;   // 128-byte steps of the sum that one workgroup takes
+  int steps_per_split;       // 128-byte steps of the sum that one workgroup takes
   int splits;
   int workgroups;            // that fit the device at a time (a multiple of 8): each takes every so many-th block
   int64_t tiles_i;
@@ -112,7 +113,7 @@ __device__ __forceinline__ u32x4 vql_shift(u32x4 v, int by) {
 
 // -------------------------------------------------------------------------------- activations
 // erfc(z) for z >= 0: the Chebyshev fit of Numerical Recipes' erfcc (W. H. Press), relative error below 1.2e-7
-// everywhere; used where the result is rounded to 16 bits, together with the exponential it contains.
+// everywhere, and a dozen instructions without a branch.
 __device__ __forceinline__ float vql_erfc_pos(float z) {
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.0f));
   float q = 0.17087277f;
@@ -134,20 +135,18 @@ __device__ __forceinline__ float vql_sigmoid(float p) {
   if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __expf(-p));
   return 1.0f / (1.0f + expf(-p));
 }
-template <bool FAST>
-__device__ __forceinline__ float vql_cdf(float p) {   // Phi(p)
-  if constexpr (FAST) {
-    const float half = 0.5f * vql_erfc_pos(fabsf(p) * 0.70710678f);
-    return p < 0.0f ? half : 1.0f - half;
-  }
-  return 0.5f * erfcf(-p * 0.70710678f);
+// Phi(p), for every type: the library's erfcf takes the branches of all its ranges in a wave with mixed arguments, and the fit
+// is off by 2^-23 of the value, times 1 + p^2 / 2 in the tails, where the exponent's own rounding shows
+__device__ __forceinline__ float vql_cdf(float p) {
+  const float half = 0.5f * vql_erfc_pos(fabsf(p) * 0.70710678f);
+  return p < 0.0f ? half : 1.0f - half;
 }
 template <bool FAST>
 __device__ __forceinline__ float vql_act(float p, int act) {
   switch (act) {
     case VQ_ACT_RELU: return p < 0.0f ? 0.0f : p;
     case VQ_ACT_SILU: return p * vql_sigmoid<FAST>(p);
-    case VQ_ACT_GELU: return p * vql_cdf<FAST>(p);
+    case VQ_ACT_GELU: return p * vql_cdf(p);
     case VQ_ACT_GELU_TANH: {
       // (1 + tanh u) / 2 = sigmoid(2u)
       const float u2 = 1.5957691216f * p * __builtin_fmaf(0.044715f * p, p, 1.0f);
@@ -184,7 +183,7 @@ __device__ __forceinline__ float vql_act_slope(float p0, int act) {
     }
     case VQ_ACT_GELU: {
       const float g = FAST ? __expf(-0.5f * p * p) : expf(-0.5f * p * p);
-      return __builtin_fmaf(p * 0.3989422804f, g, vql_cdf<FAST>(p));
+      return __builtin_fmaf(p * 0.3989422804f, g, vql_cdf(p));
     }
     case VQ_ACT_GELU_TANH: {
       const float p2 = p * p;
@@ -287,14 +286,14 @@ struct VqOperand {
     }
   }
   // a whole step (all BK values of r exist), straight into LDS: piece n of this thread's PER
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(int64_t step) const {
-    const char* p = MMAJOR ? base + step * (BK * ld) : base + step * 128;
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(int step) const {
+    const char* p = MMAJOR ? base + step * (BK * ld) : base + step * (int64_t)128;
     return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
   }
   __device__ __forceinline__ void dma_piece(__amdgpu_buffer_rsrc_t rs, int n, VQL_LDS char* lds, int wave) const {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (VQL_LDS void*)(lds + (wave * PER + n) * 1024), 16, off[n], 0, 0, 0);
   }
-  __device__ __forceinline__ void dma(int64_t step, VQL_LDS char* lds, int wave) const {
+  __device__ __forceinline__ void dma(int step, VQL_LDS char* lds, int wave) const {
     const __amdgpu_buffer_rsrc_t rs = source(step);
 #pragma unroll
     for (int n = 0; n < PER; ++n) dma_piece(rs, n, lds, wave);
@@ -303,8 +302,8 @@ struct VqOperand {
   // they are on their way together: rows that do not exist read the last one instead, a piece that passes the end of its
   // row is read from the row's last 16 bytes and shifted.  What must read as zero does (r behind the end); indexes that do
   // not exist may hold anything finite or not: they reach only outputs that are not stored.
-  __device__ __forceinline__ void fetch(int64_t step, int64_t R, int wave, int lane, u32x4 (&v)[PER]) const {
-    const int64_t r0 = step * BK;
+  __device__ __forceinline__ void fetch(int step, int64_t R, int wave, int lane, u32x4 (&v)[PER]) const {
+    const int64_t r0 = (int64_t)step * BK;
     const char* const tile = MMAJOR ? base + r0 * ld : base + r0 * ES;
     const int rs = (int)(R - r0 < BK ? R - r0 : BK), ms = (int)(M < B ? M : B);      // r and indexes that exist in the tile
     const int pitch = (int)ld;
@@ -360,8 +359,8 @@ struct VqOperand {
     return v;
   }
   // a step that is not a whole one, into LDS piece by piece: once in a sum, and with few registers
-  __device__ __forceinline__ void fill_part(int64_t step, int64_t R, VQL_LDS char* lds, int wave, int lane) const {
-    const int64_t r0 = step * BK;
+  __device__ __forceinline__ void fill_part(int step, int64_t R, VQL_LDS char* lds, int wave, int lane) const {
+    const int64_t r0 = (int64_t)step * BK;
     const char* const tile = MMAJOR ? base + r0 * ld : base + r0 * ES;
     const int rs = (int)(R - r0 < BK ? R - r0 : BK), ms = (int)(M < B ? M : B);
 #pragma unroll 1
@@ -556,12 +555,23 @@ __device__ __forceinline__ void vql_mul(const VqFrags<TI, TJ>& f, bool want_sum,
     for (int v = 0; v < TJ; ++v) acc[u][v] = vql_mma<T>(f.b[v], f.a[u], acc[u][v]);
   vql_add<T, SUMS, TI, TJ>(f, want_sum, asum);
 }
-// Waits until at most `n` of this wave's DMA instructions are in flight and its LDS accesses are done, then for the
-// other waves.  A bare barrier: nothing else has to have landed.
+// Waits until this wave's LDS accesses are done and at most N of its DMA instructions are in flight (`counted`; else
+// none), then for the other waves.  A bare barrier: nothing else has to have landed.
 template <int N>
-__device__ __forceinline__ void vql_publish() {
+__device__ __forceinline__ void vql_publish(bool counted) {
   __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+  __builtin_amdgcn_s_waitcnt(0xC07F);                                        // lgkmcnt(0)
+  if (N > 0 && counted) __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));   // vmcnt(N)
+  else __builtin_amdgcn_s_waitcnt(0x0F70);                                   // vmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// the same for waves that fill LDS through registers: loads may be in flight
+__device__ __forceinline__ void vql_publish_lds() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xC07F);
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
@@ -576,7 +586,7 @@ __device__ __forceinline__ void vql_publish() {
 // are the same memory; __restrict__ tells the compiler that a fragment read need not wait for the DMA in flight: the
 // barriers and the counted waits see to that.
 template <typename T, typename OA, typename OB, int TI, int TJ, int FLYING>
-__device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma_step, bool dma, bool pending, bool more, bool counted,
+__device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int dma_step, bool dma, bool pending, bool more, bool counted,
                                          VQL_LDS char* __restrict__ into, const VQL_LDS char* __restrict__ from, int cur, int nxt, int prev,
                                          int wi, int wj, int wave, int lane, bool want_sum, VqFrags<TI, TJ> (&f)[2],
                                          f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
@@ -608,8 +618,7 @@ __device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma
     vql_mul<T, OA::SUMS, TI, TJ>(f[q & 1], want_sum, acc, asum);
     __builtin_amdgcn_sched_barrier(0);
   }
-  if (FLYING > 0 && counted) vql_publish<FLYING>();
-  else vql_publish<0>();
+  vql_publish<FLYING>(counted);
   if (more) vql_read<OA, OB, TI, TJ>(f[0], from + nxt, 0, wi, wj, lane);
   __builtin_amdgcn_sched_barrier(0);
   // the DMA instructions one by one between the products
@@ -625,6 +634,49 @@ __device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int64_t dma
     __builtin_amdgcn_sched_barrier(0);
   }
   vql_add<T, OA::SUMS, TI, TJ>(f[1], want_sum, asum);
+}
+
+// Two steps of the sum for the 64x64 tile, whose quarters have one product a wave (32 cycles, the latency of an LDS read is
+// some 150): the fragments of the whole next step are read while this one is multiplied.  A step takes 0.30 us instead of
+// 0.34 with one workgroup on a CU; with four products a quarter (tile 128) it takes 0.80 instead of 0.72, the reads delaying
+// the first product, so that tile reads a quarter ahead.  f[0] holds step s on entry, and step s + 2 on return.
+template <typename T, typename OA, typename OB, int TI, int TJ, int NS>
+__device__ __forceinline__ void vql_two_steps(const OA& oa, const OB& ob, int s, int s1, int last_dma, int64_t R,
+                                              VQL_LDS char* __restrict__ into, const VQL_LDS char* __restrict__ from, int& at,
+                                              int wi, int wj, int wave, int lane, bool want_sum, VqFrags<TI, TJ> (&f)[2][4],
+                                              f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
+  constexpr int PIECES = OA::PER + OB::PER, STAGE = OA::BYTES + OB::BYTES;
+#pragma unroll
+  for (int half = 0; half < 2; ++half, ++s) {
+    if (s >= s1) break;
+    const int cur = at * STAGE;
+    at = at + 1 == NS ? 0 : at + 1;
+    vql_publish<(NS - 2) * PIECES>(s + NS <= last_dma);   // all of the steps on their way (to s + NS - 1) but those behind s + 1
+    if (s + 1 < s1) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vql_read<OA, OB, TI, TJ>(f[half ^ 1][q], from + at * STAGE, q, wi, wj, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const bool dma = s + NS < last_dma;
+    const __amdgpu_buffer_rsrc_t ra = oa.source(s + NS), rb = ob.source(s + NS);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      vql_mul<T, OA::SUMS, TI, TJ>(f[half][q], want_sum, acc, asum);
+      if (dma) {   // a quarter of the DMA instructions behind each quarter's products
+#pragma unroll
+        for (int k = q * PIECES / 4; k < (q + 1) * PIECES / 4; ++k) {
+          if (k < OA::PER) oa.dma_piece(ra, k, into + cur, wave);
+          else ob.dma_piece(rb, k - OA::PER, into + cur + OA::BYTES, wave);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!dma && s + NS < s1) {   // a step that is not a whole one
+      const int l = vql_fresh(lane);
+      oa.fill_part(s + NS, R, into + cur, wave, l);
+      ob.fill_part(s + NS, R, into + cur + OA::BYTES, wave, l);
+    }
+  }
 }
 
 // -------------------------------------------------------------------------------- the product
@@ -645,13 +697,13 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
   const int wi = wave / WJ, wj = wave % WJ;
 
   const int64_t per_split = a.tiles_i * a.tiles_j, total = per_split * a.splits;
-  const int64_t steps = (a.R + OA::BK - 1) / OA::BK;
-  const int64_t full = a.R / OA::BK;
+  const int steps = (int)((a.R + OA::BK - 1) / OA::BK), full = (int)(a.R / OA::BK);
   VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
   OA oa;
   OB ob;
   int split = 0, tj0 = 0;
-  int64_t i0 = 0, j0 = 0, s0 = 0, s1 = 0;
+  int64_t i0 = 0, j0 = 0;
+  int s0 = 0, s1 = 0;
 
   // Consecutive workgroups go to the 8 dies in turn: give each die a contiguous range of blocks, and walk the range in
   // groups of 8 block rows, so that the blocks in flight on a die share their operands in its L2.
@@ -668,12 +720,12 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     tj0 = (int)(id / gsz);
     j0 = (int64_t)tj0 * BJ;
     s0 = split * a.steps_per_split;
-    s1 = s0 + a.steps_per_split < steps ? s0 + a.steps_per_split : steps;
+    s1 = steps - s0 < a.steps_per_split ? steps : s0 + a.steps_per_split;
     const int l = vql_fresh(lane);
     oa.init(a.A, a.lda, i0, a.I, wave, l);
     ob.init(a.B, a.ldb, j0, a.J, wave, l);
   };
-  auto by_registers = [&](int64_t s, int at) {
+  auto by_registers = [&](int s, int at) {
     const int l = vql_fresh(lane);
     oa.fill_part(s, a.R, lds + at, wave, l);
     ob.fill_part(s, a.R, lds + at + OA::BYTES, wave, l);
@@ -717,25 +769,33 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     for (int u = 0; u < TI; ++u) asum[u] = 0.0f;
 
     if (s0 < s1) {
-      VqFrags<TI, TJ> f[2];
       if constexpr (DMA) {
-        const int64_t last_dma = s1 < full ? s1 : full;      // steps from here on are filled through registers
-        if (s0 + NS <= last_dma) vql_publish<(NS - 1) * (OA::PER + OB::PER)>();
-        else vql_publish<0>();
-        vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
+        const int last_dma = s1 < full ? s1 : full;      // steps from here on are filled through registers
+        vql_publish<(NS - 1) * (OA::PER + OB::PER)>(s0 + NS <= last_dma);
         int at = 0;
-        for (int64_t s = s0; s < s1; ++s) {
-          const int cur = at * STAGE, prev = at == 0 ? (NS - 1) * STAGE : cur - STAGE;
-          at = at + 1 == NS ? 0 : at + 1;
-          vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(
-              oa, ob, s + NS, s + NS < last_dma, s > s0 && s + NS - 1 < last_dma, s + 1 < s1, s + NS - 1 < last_dma, lds, lds,
-              cur, at * STAGE, prev, wi, wj, wave, lane, want_sum, f, acc, asum);
-          if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
+        if constexpr (TI * TJ == 1) {
+          VqFrags<TI, TJ> f[2][4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) vql_read<OA, OB, TI, TJ>(f[0][q], lds, q, wi, wj, lane);
+          for (int s = s0; s < s1; s += 2)
+            vql_two_steps<T, OA, OB, TI, TJ, NS>(oa, ob, s, s1, last_dma, a.R, lds, lds, at, wi, wj, wave, lane, want_sum, f, acc, asum);
+        } else {
+          VqFrags<TI, TJ> f[2];
+          vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
+          for (int s = s0; s < s1; ++s) {
+            const int cur = at * STAGE, prev = at == 0 ? (NS - 1) * STAGE : cur - STAGE;
+            at = at + 1 == NS ? 0 : at + 1;
+            vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(
+                oa, ob, s + NS, s + NS < last_dma, s > s0 && s + NS - 1 < last_dma, s + 1 < s1, s + NS - 1 < last_dma, lds, lds,
+                cur, at * STAGE, prev, wi, wj, wave, lane, want_sum, f, acc, asum);
+            if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
+          }
         }
       } else {
         // the same steps with two buffers; the tiles of the next step wait in registers while this one is worked on
+        VqFrags<TI, TJ> f[2];
         u32x4 va[OA::PER], vb[OB::PER];
-        auto fetch = [&](int64_t s) {
+        auto fetch = [&](int s) {
           const int l = vql_fresh(lane);
           oa.fetch(s, a.R, wave, l, va);
           ob.fetch(s, a.R, wave, l, vb);
@@ -744,10 +804,10 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
         oa.commit(lds, wave, lane, va);
         ob.commit(lds + OA::BYTES, wave, lane, vb);
         if (s0 + 1 < s1) fetch(s0 + 1);
-        vql_publish<63>();
+        vql_publish_lds();
         vql_read<OA, OB, TI, TJ>(f[0], lds, 0, wi, wj, lane);
         int cur = 0;
-        for (int64_t s = s0; s < s1; ++s) {
+        for (int s = s0; s < s1; ++s) {
 #pragma unroll
           for (int q = 0; q < 3; ++q) {
             vql_read<OA, OB, TI, TJ>(f[(q + 1) & 1], lds + cur, q + 1, wi, wj, lane);
@@ -760,7 +820,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
             oa.commit(lds + cur, wave, lane, va);
             ob.commit(lds + cur + OA::BYTES, wave, lane, vb);
           }
-          vql_publish<63>();
+          vql_publish_lds();
           if (s + 2 < s1) fetch(s + 2);
           if (s + 1 < s1) vql_read<OA, OB, TI, TJ>(f[0], lds + cur, 0, wi, wj, lane);
           __builtin_amdgcn_sched_barrier(0);

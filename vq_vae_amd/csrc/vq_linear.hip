@@ -180,9 +180,20 @@ constexpr int CUS = 256;
 
 size_t elem_size(int dtype) { return dtype == VQ_F32 ? 4 : 2; }
 
-// The cheapest of the three tiles, each with its best split of the sum, by a model of the launch: rounds of
-// workgroups x (steps of the sum x time of a step + what a workgroup pays once), plus the join of a split sum.
-// Times in microseconds, measured on an MI355X (step: 128 bytes of the sum).
+// What a block of each tile costs: microseconds of a 128-byte step of the sum with 1, 2, 3 workgroups on a CU, and what a
+// workgroup pays once (start, first tiles, epilogue); 16-bit and 32-bit types, tiles filled by DMA and through registers.
+// Measured on an MI355X, 256 workgroups for each one on a CU, sums of 8 and of 32 steps.
+struct Cost {
+  int tile, per_cu;
+  struct { float step[3], once; } of[2][2];   // [dma][32 bits]
+};
+const Cost COST[VQL_CONFIGS] = {
+    {64, 3, {{{{0.90f, 1.17f, 1.38f}, 4.2f}, {{1.17f, 1.65f, 2.05f}, 6.0f}}, {{{0.32f, 0.45f, 0.60f}, 4.4f}, {{0.65f, 1.07f, 1.45f}, 6.5f}}}},
+    {128, 2, {{{{1.70f, 2.05f}, 8.0f}, {{2.95f, 4.60f}, 12.0f}}, {{{0.75f, 0.95f}, 6.5f}, {{2.00f, 3.72f}, 13.5f}}}},
+    {256, 1, {{}, {{{1.55f}, 12.5f}, {{7.15f}, 27.0f}}}},
+};
+// The cheapest tile with its best split of the sum: rounds of workgroups x (steps x time of a step + once), the last round
+// with as many on a CU as are left, and the join of a split sum (a launch, the partial sums written and read at 4 TB/s).
 Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
   const size_t es = elem_size(dtype);
   Plan best{};
@@ -193,20 +204,21 @@ Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
     best.splits = 1;
     return best;
   }
-  static const struct { int tile, per_cu; double step16, step32, once; } cfg[3] = {
-      {64, 3, 0.30, 0.60, 2.0}, {128, 2, 0.50, 1.60, 3.0}, {256, 1, 0.90, 3.60, 6.0}};
   const int64_t steps = (R * es + 127) / 128;
   double best_t = 1e300;
-  for (int c = dma ? 2 : 1; c >= 0; --c) {
-    const int64_t ti = (I + cfg[c].tile - 1) / cfg[c].tile, tj = (J + cfg[c].tile - 1) / cfg[c].tile;
-    const int64_t slots = (int64_t)CUS * cfg[c].per_cu;
-    const double step = es == 2 ? cfg[c].step16 : cfg[c].step32;
+  for (int c = 0; c < VQL_CONFIGS; ++c) {
+    const Cost& cost = COST[c];
+    const auto& of = cost.of[dma][es == 4];
+    if (of.once == 0.0f) continue;
+    const int64_t ti = (I + cost.tile - 1) / cost.tile, tj = (J + cost.tile - 1) / cost.tile;
+    const int64_t slots = (int64_t)CUS * cost.per_cu;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 4, 2 * slots / std::max<int64_t>(1, ti * tj)));
     for (int64_t s = 1; s <= most; s = s < 8 ? s + 1 : s + s / 8) {
       const int64_t per = (steps + s - 1) / s, sp = steps ? (steps + per - 1) / per : 1;
-      const int64_t rounds = (ti * tj * sp + slots - 1) / slots;
-      double t = rounds * (per * step + cfg[c].once);
-      if (sp > 1) t += 4.0 + (double)I * J * 4 * (2 * sp + 1) / 4.0e6;   // partial sums written and read at 4 TB/s
+      const int64_t blocks = ti * tj * sp, rounds = blocks / slots, rest = blocks % slots;
+      double t = rounds * (per * of.step[cost.per_cu - 1] + of.once);
+      if (rest) t += per * of.step[(rest - 1) / CUS] + of.once;
+      if (sp > 1) t += 3.0 + (double)ti * tj * cost.tile * cost.tile * 8 * sp / 4.0e6;
       if (t < best_t) {
         best_t = t;
         best.config = c;
@@ -221,9 +233,8 @@ Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
   return best;
 }
 
-constexpr int TILE[3] = {64, 128, 256};
 int64_t part_bytes(const Plan& p) {
-  return p.splits > 1 ? p.splits * p.tiles_i * p.tiles_j * TILE[p.config] * TILE[p.config] * 4 : 0;
+  return p.splits > 1 ? p.splits * p.tiles_i * p.tiles_j * COST[p.config].tile * COST[p.config].tile * 4 : 0;
 }
 // row slabs of vql_colsum_kernel
 int64_t colsum_slabs(int64_t M, int N) {
@@ -264,7 +275,7 @@ template <typename T> struct RunRows {
 };
 template <typename T> struct RunJoin {
   static int run(const VqLinearArgs& a, int config, hipStream_t s) {
-    const int tile = TILE[config], waves_j = config == VQL_C256 ? 4 : 2;
+    const int tile = COST[config].tile, waves_j = config == VQL_C256 ? 4 : 2;
     const int tiles_u = config == VQL_C256 ? 4 : tile / 64, tiles_v = config == VQL_C256 ? 2 : tile / 64;
     const int64_t blocks = a.tiles_i * a.tiles_j * tile * tile / 1024;
     hipLaunchKernelGGL(vql_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a, tile, waves_j, tiles_u, tiles_v);
@@ -306,7 +317,7 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, void* work, 
   if (layout == 2 && (a.I % E || a.J % E)) dma = false;
   const Plan p = make_plan(layout, a.I, a.J, a.R, dtype, dma);
   a.splits = p.splits;
-  a.steps_per_split = p.steps_per_split;
+  a.steps_per_split = (int)p.steps_per_split;
   a.tiles_i = p.tiles_i;
   a.tiles_j = p.tiles_j;
   a.workgroups = p.workgroups;
