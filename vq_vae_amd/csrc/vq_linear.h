@@ -568,6 +568,23 @@ __device__ __forceinline__ void vql_publish(bool counted) {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
+// The same behind an epilogue, whose stores are younger than the DMA of the next block's first tiles: `young` of them
+// need not have landed either (0, S, 2 S or P; vmcnt counts to 63).
+template <int N, int S, int P>
+__device__ __forceinline__ void vql_publish_young(bool counted, int young) {
+  constexpr auto code = [](int n) constexpr { return 0x0F70 | ((n < 63 ? n : 63) & 15) | (((n < 63 ? n : 63) >> 4) << 14); };
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  if (!counted) __builtin_amdgcn_s_waitcnt(0x0F70);
+  else if (young == S) __builtin_amdgcn_s_waitcnt(code(N + S));
+  else if (young == 2 * S) __builtin_amdgcn_s_waitcnt(code(N + 2 * S));
+  else if (young == P) __builtin_amdgcn_s_waitcnt(code(N + P));
+  else __builtin_amdgcn_s_waitcnt(code(N));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
 // the same for waves that fill LDS through registers: loads may be in flight
 __device__ __forceinline__ void vql_publish_lds() {
   __builtin_amdgcn_sched_barrier(0);
@@ -585,8 +602,9 @@ __device__ __forceinline__ void vql_publish_lds() {
 // `fly`: this wave's DMA instructions that may still be in flight behind those of the next step, or 0.  `into` and `from`
 // are the same memory; __restrict__ tells the compiler that a fragment read need not wait for the DMA in flight: the
 // barriers and the counted waits see to that.
-template <typename T, typename OA, typename OB, int TI, int TJ, int FLYING>
+template <typename T, typename OA, typename OB, int TI, int TJ, int FLYING, int S, int P>
 __device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int dma_step, bool dma, bool pending, bool more, bool counted,
+                                         int young,
                                          VQL_LDS char* __restrict__ into, const VQL_LDS char* __restrict__ from, int cur, int nxt, int prev,
                                          int wi, int wj, int wave, int lane, bool want_sum, VqFrags<TI, TJ> (&f)[2],
                                          f32x16 (&acc)[TI][TJ], float (&asum)[TI]) {
@@ -618,7 +636,7 @@ __device__ __forceinline__ void vql_step(const OA& oa, const OB& ob, int dma_ste
     vql_mul<T, OA::SUMS, TI, TJ>(f[q & 1], want_sum, acc, asum);
     __builtin_amdgcn_sched_barrier(0);
   }
-  vql_publish<FLYING>(counted);
+  vql_publish_young<FLYING, S, P>(counted, young);
   if (more) vql_read<OA, OB, TI, TJ>(f[0], from + nxt, 0, wi, wj, lane);
   __builtin_amdgcn_sched_barrier(0);
   // the DMA instructions one by one between the products
@@ -751,6 +769,9 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     }
   };
 
+  // stores of a wave's epilogue: of one tensor, where the whole block exists, and of a partial sum
+  constexpr int S = TI * TJ * (16 * (int)sizeof(T) / 16), P = TI * TJ * 4;
+  int young = 0;
   int64_t n = blockIdx.x;
   choose(n);
   begin_early();
@@ -771,7 +792,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     if (s0 < s1) {
       if constexpr (DMA) {
         const int last_dma = s1 < full ? s1 : full;      // steps from here on are filled through registers
-        vql_publish<(NS - 1) * (OA::PER + OB::PER)>(s0 + NS <= last_dma);
+        vql_publish_young<(NS - 1) * (OA::PER + OB::PER), S, P>(s0 + NS <= last_dma, young);
         int at = 0;
         if constexpr (TI * TJ == 1) {
           VqFrags<TI, TJ> f[2][4];
@@ -785,8 +806,9 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
           for (int s = s0; s < s1; ++s) {
             const int cur = at * STAGE, prev = at == 0 ? (NS - 1) * STAGE : cur - STAGE;
             at = at + 1 == NS ? 0 : at + 1;
-            vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER)>(
-                oa, ob, s + NS, s + NS < last_dma, s > s0 && s + NS - 1 < last_dma, s + 1 < s1, s + NS - 1 < last_dma, lds, lds,
+            vql_step<T, OA, OB, TI, TJ, (NS - 2) * (OA::PER + OB::PER), S, P>(
+                oa, ob, s + NS, s + NS < last_dma, s > s0 && s + NS - 1 < last_dma, s + 1 < s1, s + NS - 1 < last_dma,
+                s == s0 ? young : 0, lds, lds,
                 cur, at * STAGE, prev, wi, wj, wave, lane, want_sum, f, acc, asum);
             if (s + NS < s1 && s + NS >= last_dma) by_registers(s + NS, cur);
           }
@@ -870,6 +892,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     } else {
       vql_write<T, TI, TJ, false>(a, iw, jw, vql_fresh(lane), acc);
     }
+    young = a.splits > 1 ? P : inside ? (a.pre ? 2 * S : S) : 0;
     if (!more) break;
   }
 }
