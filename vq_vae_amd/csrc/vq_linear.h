@@ -81,6 +81,15 @@ __device__ __forceinline__ void vql_store16(void* p, u32x4 v) {
   if constexpr (sizeof(T) == 4) *reinterpret_cast<vql_u32x4_a4*>(p) = v;
   else *reinterpret_cast<vql_u32x4_a2*>(p) = v;
 }
+// The same, and past the caches if `stream`: outputs of the product are not read again by it, and keep its operands out of the
+// L2 otherwise (64 Ki x 1024 -> 1024 bf16 143 -> 130 us, 64 Ki x 64 -> 1024 42 -> 37).  Only for accesses that fill 64-byte
+// runs: with rows of 6766 bytes, whose runs straddle the lines, the same kernel took 103 us instead of 64.
+template <typename T>
+__device__ __forceinline__ void vql_stream16(bool stream, void* p, u32x4 v) {
+  if (!stream) vql_store16<T>(p, v);
+  else if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(v, reinterpret_cast<vql_u32x4_a4*>(p));
+  else __builtin_nontemporal_store(v, reinterpret_cast<vql_u32x4_a2*>(p));
+}
 // `valid` of the 16 / sizeof(T) elements at p, the others zero
 template <typename T>
 __device__ __forceinline__ u32x4 vql_load16_part(const char* p, int64_t valid) {
@@ -109,6 +118,19 @@ __device__ __forceinline__ u32x4 vql_shift(u32x4 v, int by) {
   if (by & 2) v = u32x4{v[2], v[3], 0, 0};
   if (by & 4) v = u32x4{0, 0, 0, 0};
   return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void vql_store16_part(char* p, u32x4 v, int64_t valid) {
+  constexpr int E = 16 / sizeof(T);
+  if (valid >= E) {
+    vql_store16<T>(p, v);
+  } else {
+    const VqChunk<T> c = __builtin_bit_cast(VqChunk<T>, v);
+#pragma unroll
+    for (int e = 0; e < E - 1; ++e)
+      if (e < valid) reinterpret_cast<T*>(p)[e] = c.e[e];
+  }
 }
 
 // -------------------------------------------------------------------------------- activations
@@ -230,8 +252,8 @@ __device__ __forceinline__ float vql_sum16(u32x4 v) {   // sum of the fragment's
 
 // -------------------------------------------------------------------------------- operand tiles in LDS
 // One step of the sum covers 128 bytes of r: 64 elements of 16 bits, 32 of 32 bits.
-// r-major tile of `B` indexes: B rows of 128 bytes, 16-byte piece c of row m in slot c ^ (bits 1-3 of m; for the ordered
-//   operand bits 1, 2 and 4): the 16 rows that a fragment read touches at a time fall on all banks evenly.
+// r-major tile of `B` indexes: B rows of 128 bytes, 16-byte piece c of row m in slot c ^ (bits 1-3 of m): the 16 rows that a
+//   fragment read touches at a time fall on all banks evenly.
 // m-major tile: one row of B elements per r, 16-byte piece c of row r in slot c ^ vql_mswz<T>(r): the rows that one
 //   transposing read (16 bits: r = 8h + 4t + 0..3 for both halves h) or one fp32 read (r = e and 4 + e) touches lie in
 //   different 64- or 128-byte segments.
@@ -243,8 +265,9 @@ __device__ __forceinline__ int vql_mswz(int r) {
 }
 
 // Which index of a 32-block the lanes of the `b`-side operand hold: the matrix instruction leaves a lane the rows 8g + 4h + r
-// (g, r = 0..3) of its column, h = lane / 32; with this order they are the 16 consecutive indexes 16h + 4g + r.
-__device__ __forceinline__ int vql_order(int rho) { return ((rho & 4) << 2) | ((rho >> 1) & 12) | (rho & 3); }
+// (g, r = 0..3) of its column, h = lane / 32; with this order they are the indexes 16 (g / 2) + 8h + 4 (g % 2) + r: two runs
+// of eight, one for each half of the 32, in which the lanes of the two halves take turns.
+__device__ __forceinline__ int vql_order(int rho) { return (rho & 19) | ((rho & 4) << 1) | ((rho & 8) >> 1); }
 
 template <typename T, bool MMAJOR, int B, int NT, bool DMA, bool ORDERED>
 struct VqOperand {
@@ -259,11 +282,10 @@ struct VqOperand {
   int64_t M, total;      // indexes that exist from m0 on, and altogether
   uint32_t off[PER];     // this lane's byte offsets of a full step
 
-  __device__ __forceinline__ static int rswz(int row) { return ORDERED ? ((row >> 1) & 3) | ((row >> 2) & 4) : row >> 1; }
   __device__ __forceinline__ static void where(int n, int wave, int lane, int& row, int& piece) {
     const int p = (wave * PER + n) * 64 + lane;
     row = p / CPR;
-    piece = (p % CPR) ^ ((MMAJOR ? vql_mswz<T>(row) : rswz(row)) & SWZ);
+    piece = (p % CPR) ^ ((MMAJOR ? vql_mswz<T>(row) : (row >> 1)) & SWZ);
   }
   __device__ __forceinline__ void init(const char* src, int64_t ld_, int64_t m0, int64_t all, int wave, int lane) {
     ld = ld_;
@@ -383,7 +405,7 @@ struct VqOperand {
     const int h = lane >> 5;
     if constexpr (!MMAJOR) {
       const int rho = lane & 31, row = m + (ORDERED ? vql_order(rho) : rho);
-      return *reinterpret_cast<const VQL_LDS vql_u32x4_a16*>(lds + row * 128 + (((2 * q + h) ^ (rswz(row) & 7)) * 16));
+      return *reinterpret_cast<const VQL_LDS vql_u32x4_a16*>(lds + row * 128 + (((2 * q + h) ^ ((row >> 1) & 7)) * 16));
     } else if constexpr (ES == 2) {
       // transposing read: each group of 16 lanes names 4 rows (r) of 16 consecutive indexes, 8 bytes a lane, and lane i
       // of the group receives index i of the four rows
@@ -411,18 +433,20 @@ struct VqOperand {
 };
 
 // -------------------------------------------------------------------------------- epilogue
-// y = act(c + bias) + residual, rounded once, for 16 / sizeof(T) columns from j on, `n` of which exist; `pre` = c + bias
-// rounded (kept for the activation's gradient); res: the residual's 16 bytes.
+// out = act(c + bias) + residual, rounded once, for 16 / sizeof(T) columns; pre = c + bias rounded (kept for the activation's
+// gradient); res: the residual's 16 bytes.
 template <typename T>
-__device__ __forceinline__ void vql_finish(const VqLinearArgs& a, char* y_at, char* pre_at, int n, const float* c, const float* bias,
-                                           u32x4 res) {
+__device__ __forceinline__ void vql_finish(const VqLinearArgs& a, const float* c, const float* bias, u32x4 res, u32x4& out, u32x4& pre) {
   constexpr int E = 16 / sizeof(T);
   float p[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) p[e] = c[e] + bias[e];
-  VqChunk<T> y, pv;
+  VqChunk<T> y;
+  if (a.pre) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) pv.e[e] = VqElem<T>::from(p[e]);
+    for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(p[e]);
+    pre = __builtin_bit_cast(u32x4, y);
+  }
   vql_act_all<sizeof(T) == 2, E>(p, a.act);
   if (a.res) {
     const VqChunk<T> r = __builtin_bit_cast(VqChunk<T>, res);
@@ -431,17 +455,7 @@ __device__ __forceinline__ void vql_finish(const VqLinearArgs& a, char* y_at, ch
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(p[e]);
-  if (n >= E) {
-    vql_store16<T>(y_at, __builtin_bit_cast(u32x4, y));
-    if (a.pre) vql_store16<T>(pre_at, __builtin_bit_cast(u32x4, pv));
-  } else {
-#pragma unroll
-    for (int e = 0; e < E - 1; ++e)
-      if (e < n) {
-        reinterpret_cast<T*>(y_at)[e] = y.e[e];
-        if (a.pre) reinterpret_cast<T*>(pre_at)[e] = pv.e[e];
-      }
-  }
+  out = __builtin_bit_cast(u32x4, y);
 }
 // bias[j .. j + W), zero where there is none
 template <typename T, int W>
@@ -459,48 +473,85 @@ __device__ __forceinline__ void vql_bias(const VqLinearArgs& a, int64_t j, float
     }
   }
 }
-// The epilogue of 16 columns cv .. cv + 15 of row r out of the values that one lane holds of one tile; what does not exist
-// is left out.
+// First column, within a 32x32 tile, of the k-th 16 bytes that a lane of half h holds of its row (see vql_order).
 template <typename T>
-__device__ __forceinline__ void vql_write16(const VqLinearArgs& a, int64_t r, int64_t cv, const float (&c)[16]) {
-  constexpr int ES = sizeof(T), E = 16 / ES, PV = 16 / E;
-  float bias[16];
-  vql_bias<T, 16>(a, cv, bias);
+__device__ __forceinline__ int vql_piece(int k, int h) {
+  return sizeof(T) == 2 ? 16 * k + 8 * h : 16 * (k >> 1) + 8 * h + 4 * (k & 1);
+}
+// The epilogue of what one lane holds of one tile: row r, the columns of its pieces from cv on.  What does not exist is
+// left out.
+template <typename T, typename C>
+__device__ __forceinline__ void vql_write_lane(const VqLinearArgs& a, int64_t r, int64_t cv, int h, const C& c) {
+  constexpr int ES = sizeof(T), E = 16 / ES;
 #pragma unroll
-  for (int k = 0; k < PV; ++k) {
-    const int64_t left = a.J - cv - k * E, at = (r * a.J + cv + k * E) * ES;
+  for (int k = 0; k < 16 / E; ++k) {
+    const int64_t col = cv + vql_piece<T>(k, h), left = a.J - col, at = (r * a.J + col) * ES;
     if (r >= a.I || left <= 0) continue;
-    u32x4 res = {0, 0, 0, 0};
-    if (a.res) res = vql_load16_part<T>(a.res + r * a.ldr + (cv + k * E) * ES, left);
-    vql_finish<T>(a, reinterpret_cast<char*>(a.out) + at, reinterpret_cast<char*>(a.pre) + at, left < E ? (int)left : E, c + k * E,
-                  bias + k * E, res);
+    float bias[E], v[E];
+    vql_bias<T, E>(a, col, bias);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = c[k * E + e];
+    u32x4 res = {0, 0, 0, 0}, y, pre;
+    if (a.res) res = vql_load16_part<T>(a.res + r * a.ldr + col * ES, left);
+    vql_finish<T>(a, v, bias, res, y, pre);
+    vql_store16_part<T>(reinterpret_cast<char*>(a.out) + at, y, left);
+    if (a.pre) vql_store16_part<T>(reinterpret_cast<char*>(a.pre) + at, pre, left);
   }
 }
-// The epilogue of a wave's part of a block: rows i .. i + 32 TI, columns j .. j + 32 TJ.  A lane holds 16 consecutive
-// columns of a row per tile, so that all of it is 16-byte accesses straight from the accumulators.  INSIDE: the whole part
-// exists.  The residual of the next row block is on its way while this one is worked on.
-template <typename T, int TI, int TJ, bool INSIDE>
-__device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int64_t j, int lane, const f32x16 (&acc)[TI][TJ]) {
+// Exchanges 16-lane rows: a lane with bit 4 clear keeps p and gets its neighbour's (lane + 16) p as q, one with bit 4 set keeps
+// q and gets its neighbour's q as p.  Its own inverse.
+__device__ __forceinline__ void vql_swap16(u32x4& p, u32x4& q) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto both = __builtin_amdgcn_permlane16_swap(p[e], q[e], false, false);
+    p[e] = both[0];
+    q[e] = both[1];
+  }
+}
+// The bias of a wave's part of a block as vql_write takes it, zero where there is none; asked for early, since nothing else of
+// the epilogue waits for memory.
+template <typename T, int TJ>
+__device__ __forceinline__ void vql_ask_bias(const VqLinearArgs& a, int64_t j, int h, u32x4 (&bias_of)[TJ][16 * sizeof(T) / 16]) {
+  const char* p = reinterpret_cast<const char*>(a.bias) + j * (int64_t)sizeof(T);
+#pragma unroll
+  for (int v = 0; v < TJ; ++v)
+#pragma unroll
+    for (int k = 0; k < (int)(16 * sizeof(T) / 16); ++k)
+      bias_of[v][k] = a.bias ? vql_load16<T>(p + (v * 32 + vql_piece<T>(k, h)) * (int)sizeof(T)) : u32x4{0, 0, 0, 0};
+}
+// The epilogue of a wave's part of a block: rows i .. i + 32 TI, columns j .. j + 32 TJ, all of which exist.  A lane holds 32
+// or 64 bytes of one row in pieces of 16; exchanging every other piece with the lane 16 away makes one access of the wave 64
+// consecutive bytes of 16 rows instead of twice 16 bytes of 32 rows (64 Ki x 256 -> 1024 bf16: 52 instead of 59 us: the L2 takes
+// a request per line and instruction).  The residual of the next row block is on its way while this one is worked on.
+template <typename T, int TI, int TJ>
+__device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int64_t j, int lane, const u32x4 (&bias_of)[TJ][16 * sizeof(T) / 16],
+                                          const f32x16 (&acc)[TI][TJ]) {
   constexpr int ES = sizeof(T), E = 16 / ES, PV = 16 / E;
-  const int lr = lane & 31, lc = 16 * (lane >> 5);
-  // one wave-uniform address per tensor and one 32-bit offset per lane
+  const int h = lane >> 5;
+  // One wave-uniform address per tensor and one 32-bit offset per lane: row lane % 16, and the first or second piece of a pair.
   const int64_t pitch = (int64_t)a.J * ES, origin = i * pitch + j * ES;
   char* const yb = reinterpret_cast<char*>(a.out) + origin;
   char* const pb = reinterpret_cast<char*>(a.pre) + origin;
   const char* const rb = a.res + i * a.ldr + j * ES;
-  const uint32_t yo = (uint32_t)(lr * (int)pitch + lc * ES), ro = (uint32_t)(lr * (int)a.ldr + lc * ES);
+  const bool stream = ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.pre) | pitch) & 63) == 0;
+  const int lc = vql_piece<T>((lane >> 4) & 1, h) * ES;
+  const uint32_t yo = (uint32_t)((lane & 15) * (int)pitch + lc), ro = (uint32_t)((lane & 15) * (int)a.ldr + lc);
 #pragma unroll
   for (int v = 0; v < TJ; ++v) {
-    const int left_v = (int)(a.J - j) - v * 32 - lc;
-    float bias[16];
-    vql_bias<T, 16>(a, j + v * 32 + lc, bias);
+    float bias[PV][E];
+#pragma unroll
+    for (int k = 0; k < PV; ++k) {
+      const VqChunk<T> b = __builtin_bit_cast(VqChunk<T>, bias_of[v][k]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) bias[k][e] = VqElem<T>::to(b.e[e]);
+    }
     u32x4 res[2][PV];
     auto load = [&](int u, u32x4 (&to)[PV]) {
 #pragma unroll
-      for (int k = 0; k < PV; ++k) {
-        const char* p = rb + (int64_t)u * 32 * a.ldr + (v * 32 + k * E) * ES + ro;
-        if (INSIDE) to[k] = vql_load16<T>(p);
-        else to[k] = vql_load16_part<T>(p, i + u * 32 + lr < a.I ? left_v - k * E : 0);
+      for (int k = 0; k < PV; k += 2) {
+        const char* p = rb + (int64_t)u * 32 * a.ldr + (v * 32 + 8 * k) * ES + ro;
+        to[k] = vql_load16<T>(p);
+        to[k + 1] = vql_load16<T>(p + 16 * a.ldr);
       }
     };
     if (a.res) load(0, res[0]);
@@ -508,14 +559,25 @@ __device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int6
     for (int u = 0; u < TI; ++u) {
       if (a.res && u + 1 < TI) load(u + 1, res[(u + 1) & 1]);
 #pragma unroll
-      for (int k = 0; k < PV; ++k) {
-        float c[E];
+      for (int k = 0; k < PV; k += 2) {
+        u32x4 y[2], pre[2];
+        if (a.res) vql_swap16(res[u & 1][k], res[u & 1][k + 1]);
 #pragma unroll
-        for (int e = 0; e < E; ++e) c[e] = acc[u][v][k * E + e];
-        const int64_t step = (int64_t)u * 32 * pitch + (v * 32 + k * E) * ES;
-        const int left = left_v - k * E;
-        if (INSIDE || (i + u * 32 + lr < a.I && left > 0))
-          vql_finish<T>(a, yb + step + yo, pb + step + yo, INSIDE ? E : left < E ? left : E, c, bias + k * E, res[u & 1][k]);
+        for (int w = 0; w < 2; ++w) {
+          float c[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) c[e] = acc[u][v][(k + w) * E + e];
+          vql_finish<T>(a, c, bias[k + w], res[u & 1][k + w], y[w], pre[w]);
+        }
+        const int64_t step = (int64_t)u * 32 * pitch + (v * 32 + 8 * k) * ES;
+        vql_swap16(y[0], y[1]);
+        vql_stream16<T>(stream, yb + step + yo, y[0]);
+        vql_stream16<T>(stream, yb + step + 16 * pitch + yo, y[1]);
+        if (a.pre) {
+          vql_swap16(pre[0], pre[1]);
+          vql_stream16<T>(stream, pb + step + yo, pre[0]);
+          vql_stream16<T>(stream, pb + step + 16 * pitch + yo, pre[1]);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -714,7 +776,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
 
-  const int64_t per_split = a.tiles_i * a.tiles_j, total = per_split * a.splits;
+  const int tiles_i = (int)a.tiles_i, per_split = tiles_i * a.tiles_j, total = per_split * a.splits;   // below 2^23
   const int steps = (int)((a.R + OA::BK - 1) / OA::BK), full = (int)(a.R / OA::BK);
   VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
   OA oa;
@@ -725,17 +787,16 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
 
   // Consecutive workgroups go to the 8 dies in turn: give each die a contiguous range of blocks, and walk the range in
   // groups of 8 block rows, so that the blocks in flight on a die share their operands in its L2.
-  auto choose = [&](int64_t n) {
-    const int64_t q8 = total >> 3, r8 = total & 7, x8 = n & 7;
-    int64_t id = x8 * q8 + (x8 < r8 ? x8 : r8) + (n >> 3);
-    split = (int)(id / per_split);
+  auto choose = [&](int n) {
+    const int q8 = total >> 3, r8 = total & 7, x8 = n & 7;
+    int id = x8 * q8 + (x8 < r8 ? x8 : r8) + (n >> 3);
+    split = a.splits == 1 ? 0 : id / per_split;
     id -= split * per_split;
-    const int64_t group = id / (8 * (int64_t)a.tiles_j);
-    const int64_t first = group * 8;
-    const int64_t gsz = a.tiles_i - first < 8 ? a.tiles_i - first : 8;
-    id -= group * 8 * a.tiles_j;
-    i0 = (first + id % gsz) * BI;
-    tj0 = (int)(id / gsz);
+    const int group = id / (8 * a.tiles_j), first = group * 8;
+    const int gsz = tiles_i - first < 8 ? tiles_i - first : 8;
+    id -= first * a.tiles_j;
+    tj0 = gsz == 8 ? id >> 3 : id / gsz;
+    i0 = (int64_t)(first + id - tj0 * gsz) * BI;
     j0 = (int64_t)tj0 * BJ;
     s0 = split * a.steps_per_split;
     s1 = steps - s0 < a.steps_per_split ? steps : s0 + a.steps_per_split;
@@ -772,7 +833,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
   // stores of a wave's epilogue: of one tensor, where the whole block exists, and of a partial sum
   constexpr int S = TI * TJ * (16 * (int)sizeof(T) / 16), P = TI * TJ * 4;
   int young = 0;
-  int64_t n = blockIdx.x;
+  int n = blockIdx.x;
   choose(n);
   begin_early();
   for (;;) {
@@ -859,6 +920,8 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     const int64_t this_split = split, this_block = i0 / BI * a.tiles_j + tj0;
     n += gridDim.x;
     const bool more = n < total;
+    u32x4 bias_of[TJ][16 * sizeof(T) / 16];
+    if (inside && a.splits == 1) vql_ask_bias<T, TJ>(a, jw, vql_fresh(lane) >> 5, bias_of);
     if (more) {
       choose(n);
       begin_early();
@@ -888,9 +951,13 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
             *reinterpret_cast<vql_f32x4*>(to + ((u * TJ + v) * 4 + g) * 256) = w;
           }
     } else if (inside) {
-      vql_write<T, TI, TJ, true>(a, iw, jw, vql_fresh(lane), acc);
+      vql_write<T, TI, TJ>(a, iw, jw, vql_fresh(lane), bias_of, acc);
     } else {
-      vql_write<T, TI, TJ, false>(a, iw, jw, vql_fresh(lane), acc);
+      const int l = vql_fresh(lane);
+#pragma unroll
+      for (int u = 0; u < TI; ++u)
+#pragma unroll
+        for (int v = 0; v < TJ; ++v) vql_write_lane<T>(a, iw + u * 32 + (l & 31), jw + v * 32, l >> 5, acc[u][v]);
     }
     young = a.splits > 1 ? P : inside ? (a.pre ? 2 * S : S) : 0;
     if (!more) break;

@@ -81,7 +81,7 @@ __global__ __launch_bounds__(1024) void vql_rows_kernel(VqLinearArgs a) {
 }
 
 // ------------------------------------------------------------------------------ join of a split sum
-// Adds the partial sums and applies the epilogue: a workgroup per 32x32 tile, a lane per 16 columns of a row as in the
+// Adds the partial sums and applies the epilogue: a workgroup per 32x32 tile, a lane per 16 values of a row as in the
 // product kernel; wave k adds the splits k, k + 4, .., then the four sums are added in order (the same bits on every run).
 template <typename T>
 __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a, int tile, int waves_j, int tiles_u, int tiles_v) {
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a, int tile,
   const int sub = blockIdx.x % per_block;
   const int w = sub / (tiles_u * tiles_v), u = sub / tiles_v % tiles_u, v = sub % tiles_v;
   const int64_t r = block / a.tiles_j * tile + ((w / waves_j) * tiles_u + u) * 32 + (lane & 31);
-  const int64_t cv = block % a.tiles_j * tile + ((w % waves_j) * tiles_v + v) * 32 + 16 * (lane >> 5);
+  const int64_t cv = block % a.tiles_j * tile + ((w % waves_j) * tiles_v + v) * 32;
   f32x4 c[4] = {};
   const float* p = a.part + (block * per_block + sub) * 1024 + lane * 4;
   for (int s = wave; s < a.splits; s += 4)
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a, int tile,
 #pragma unroll
     for (int e = 0; e < 4; ++e) all[4 * g + e] = t[e];
   }
-  vql_write16<T>(a, r, cv, all);
+  vql_write_lane<T>(a, r, cv, lane >> 5, all);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, int splits, int64_t n, T* out) {
