@@ -163,33 +163,26 @@ __device__ __forceinline__ float vql_cdf(float p) {
   const float half = 0.5f * vql_erfc_pos(fabsf(p) * 0.70710678f);
   return p < 0.0f ? half : 1.0f - half;
 }
-template <bool FAST>
-__device__ __forceinline__ float vql_act(float p, int act) {
-  switch (act) {
-    case VQ_ACT_RELU: return p < 0.0f ? 0.0f : p;
-    case VQ_ACT_SILU: return p * vql_sigmoid<FAST>(p);
-    case VQ_ACT_GELU: return p * vql_cdf(p);
-    case VQ_ACT_GELU_TANH: {
-      // (1 + tanh u) / 2 = sigmoid(2u)
-      const float u2 = 1.5957691216f * p * __builtin_fmaf(0.044715f * p, p, 1.0f);
-      return p * vql_sigmoid<FAST>(u2);
-    }
-    default: return p;
-  }
+// The epilogues of the product kernel, one to a kernel: the epilogue is unrolled over a wave's accumulators, and with all
+// activations in it the code outgrows the instruction cache (64 Ki x 256 -> 1024 bf16 with gelu_tanh 72 us, now 60; 8192 x 4096 x 4096 with a
+// residual 238 us, now 220).
+enum { VQL_PLAIN = 0,     // no bias, activation or residual: the products of the backward pass
+       VQL_THRESHOLD = 1, // none and relu
+       VQL_SIGMOID = 2,   // silu and gelu_tanh: p sigmoid(p) and p sigmoid(2u)
+       VQL_NORMAL = 3 };  // gelu
+__host__ __device__ inline int vql_kind(int act) {
+  return act == VQ_ACT_SILU || act == VQ_ACT_GELU_TANH ? VQL_SIGMOID : act == VQ_ACT_GELU ? VQL_NORMAL : VQL_THRESHOLD;
 }
-template <int ACT, bool FAST, int E>
-__device__ __forceinline__ void vql_act_each(float (&p)[E]) {
-#pragma unroll
-  for (int e = 0; e < E; ++e) p[e] = vql_act<FAST>(p[e], ACT);
-}
-template <bool FAST, int E>
-__device__ __forceinline__ void vql_act_all(float (&p)[E], int act) {   // one branch for all of them
-  switch (act) {
-    case VQ_ACT_RELU: vql_act_each<VQ_ACT_RELU, FAST, E>(p); break;
-    case VQ_ACT_SILU: vql_act_each<VQ_ACT_SILU, FAST, E>(p); break;
-    case VQ_ACT_GELU: vql_act_each<VQ_ACT_GELU, FAST, E>(p); break;
-    case VQ_ACT_GELU_TANH: vql_act_each<VQ_ACT_GELU_TANH, FAST, E>(p); break;
-    default: break;
+template <int KIND, bool FAST>
+__device__ __forceinline__ float vql_act_of(float p, int act) {
+  if constexpr (KIND == VQL_THRESHOLD) {
+    const float floor = act == VQ_ACT_RELU ? 0.0f : -__builtin_inff();
+    return p < floor ? floor : p;
+  } else if constexpr (KIND == VQL_SIGMOID) {
+    const float a = act == VQ_ACT_SILU ? 1.0f : 1.5957691216f, b = act == VQ_ACT_SILU ? 0.0f : 0.0713548163f;
+    return p * vql_sigmoid<FAST>(p * __builtin_fmaf(b * p, p, a));
+  } else {
+    return p * vql_cdf(p);
   }
 }
 // act'(p).  Beyond |p| = 100 every derivative has its limit, 0 or 1; the clamp keeps inf * 0 out of it.
@@ -435,19 +428,26 @@ struct VqOperand {
 // -------------------------------------------------------------------------------- epilogue
 // out = act(c + bias) + residual, rounded once, for 16 / sizeof(T) columns; pre = c + bias rounded (kept for the activation's
 // gradient); res: the residual's 16 bytes.
-template <typename T>
+template <typename T, int KIND>
 __device__ __forceinline__ void vql_finish(const VqLinearArgs& a, const float* c, const float* bias, u32x4 res, u32x4& out, u32x4& pre) {
   constexpr int E = 16 / sizeof(T);
   float p[E];
+  VqChunk<T> y;
+  if constexpr (KIND == VQL_PLAIN) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(c[e]);
+    out = __builtin_bit_cast(u32x4, y);
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) p[e] = c[e] + bias[e];
-  VqChunk<T> y;
   if (a.pre) {
 #pragma unroll
     for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(p[e]);
     pre = __builtin_bit_cast(u32x4, y);
   }
-  vql_act_all<sizeof(T) == 2, E>(p, a.act);
+#pragma unroll
+  for (int e = 0; e < E; ++e) p[e] = vql_act_of<KIND, sizeof(T) == 2>(p[e], a.act);
   if (a.res) {
     const VqChunk<T> r = __builtin_bit_cast(VqChunk<T>, res);
 #pragma unroll
@@ -480,7 +480,7 @@ __device__ __forceinline__ int vql_piece(int k, int h) {
 }
 // The epilogue of what one lane holds of one tile: row r, the columns of its pieces from cv on.  What does not exist is
 // left out.
-template <typename T, typename C>
+template <typename T, int KIND, typename C>
 __device__ __forceinline__ void vql_write_lane(const VqLinearArgs& a, int64_t r, int64_t cv, int h, const C& c) {
   constexpr int ES = sizeof(T), E = 16 / ES;
 #pragma unroll
@@ -488,14 +488,14 @@ __device__ __forceinline__ void vql_write_lane(const VqLinearArgs& a, int64_t r,
     const int64_t col = cv + vql_piece<T>(k, h), left = a.J - col, at = (r * a.J + col) * ES;
     if (r >= a.I || left <= 0) continue;
     float bias[E], v[E];
-    vql_bias<T, E>(a, col, bias);
+    if (KIND != VQL_PLAIN) vql_bias<T, E>(a, col, bias);
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = c[k * E + e];
     u32x4 res = {0, 0, 0, 0}, y, pre;
-    if (a.res) res = vql_load16_part<T>(a.res + r * a.ldr + col * ES, left);
-    vql_finish<T>(a, v, bias, res, y, pre);
+    if (KIND != VQL_PLAIN && a.res) res = vql_load16_part<T>(a.res + r * a.ldr + col * ES, left);
+    vql_finish<T, KIND>(a, v, bias, res, y, pre);
     vql_store16_part<T>(reinterpret_cast<char*>(a.out) + at, y, left);
-    if (a.pre) vql_store16_part<T>(reinterpret_cast<char*>(a.pre) + at, pre, left);
+    if (KIND != VQL_PLAIN && a.pre) vql_store16_part<T>(reinterpret_cast<char*>(a.pre) + at, pre, left);
   }
 }
 // Exchanges 16-lane rows: a lane with bit 4 clear keeps p and gets its neighbour's (lane + 16) p as q, one with bit 4 set keeps
@@ -523,7 +523,7 @@ __device__ __forceinline__ void vql_ask_bias(const VqLinearArgs& a, int64_t j, i
 // or 64 bytes of one row in pieces of 16; exchanging every other piece with the lane 16 away makes one access of the wave 64
 // consecutive bytes of 16 rows instead of twice 16 bytes of 32 rows (64 Ki x 256 -> 1024 bf16: 52 instead of 59 us: the L2 takes
 // a request per line and instruction).  The residual of the next row block is on its way while this one is worked on.
-template <typename T, int TI, int TJ>
+template <typename T, int KIND, int TI, int TJ>
 __device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int64_t j, int lane, const u32x4 (&bias_of)[TJ][16 * sizeof(T) / 16],
                                           const f32x16 (&acc)[TI][TJ]) {
   constexpr int ES = sizeof(T), E = 16 / ES, PV = 16 / E;
@@ -540,7 +540,7 @@ __device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int6
   for (int v = 0; v < TJ; ++v) {
     float bias[PV][E];
 #pragma unroll
-    for (int k = 0; k < PV; ++k) {
+    for (int k = 0; k < (KIND == VQL_PLAIN ? 0 : PV); ++k) {
       const VqChunk<T> b = __builtin_bit_cast(VqChunk<T>, bias_of[v][k]);
 #pragma unroll
       for (int e = 0; e < E; ++e) bias[k][e] = VqElem<T>::to(b.e[e]);
@@ -554,26 +554,26 @@ __device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int6
         to[k + 1] = vql_load16<T>(p + 16 * a.ldr);
       }
     };
-    if (a.res) load(0, res[0]);
+    if (KIND != VQL_PLAIN && a.res) load(0, res[0]);
 #pragma unroll
     for (int u = 0; u < TI; ++u) {
-      if (a.res && u + 1 < TI) load(u + 1, res[(u + 1) & 1]);
+      if (KIND != VQL_PLAIN && a.res && u + 1 < TI) load(u + 1, res[(u + 1) & 1]);
 #pragma unroll
       for (int k = 0; k < PV; k += 2) {
         u32x4 y[2], pre[2];
-        if (a.res) vql_swap16(res[u & 1][k], res[u & 1][k + 1]);
+        if (KIND != VQL_PLAIN && a.res) vql_swap16(res[u & 1][k], res[u & 1][k + 1]);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           float c[E];
 #pragma unroll
           for (int e = 0; e < E; ++e) c[e] = acc[u][v][(k + w) * E + e];
-          vql_finish<T>(a, c, bias[k + w], res[u & 1][k + w], y[w], pre[w]);
+          vql_finish<T, KIND>(a, c, bias[k + w], res[u & 1][k + w], y[w], pre[w]);
         }
         const int64_t step = (int64_t)u * 32 * pitch + (v * 32 + 8 * k) * ES;
         vql_swap16(y[0], y[1]);
         vql_stream16<T>(stream, yb + step + yo, y[0]);
         vql_stream16<T>(stream, yb + step + 16 * pitch + yo, y[1]);
-        if (a.pre) {
+        if (KIND != VQL_PLAIN && a.pre) {
           vql_swap16(pre[0], pre[1]);
           vql_stream16<T>(stream, pb + step + yo, pre[0]);
           vql_stream16<T>(stream, pb + step + 16 * pitch + yo, pre[1]);
@@ -764,7 +764,7 @@ namespace {   // the kernels of a translation unit are its own
 // A workgroup of WI x WJ waves owns a BI x BJ block of C (and, with splits, a range of the sum); a wave owns
 // (BI / WI) x (BJ / WJ) of it in 32x32 accumulator tiles.  DMA: rows start on 16 bytes, so that the tiles go straight into
 // LDS; otherwise they go through registers.
-template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
+template <typename T, bool AMM, bool BMM, int KIND, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
 __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_product_kernel(VqLinearArgs a) {
   constexpr int NT = WI * WJ * 64;
   constexpr int TI = BI / WI / 32, TJ = BJ / WJ / 32;
@@ -921,7 +921,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
     n += gridDim.x;
     const bool more = n < total;
     u32x4 bias_of[TJ][16 * sizeof(T) / 16];
-    if (inside && a.splits == 1) vql_ask_bias<T, TJ>(a, jw, vql_fresh(lane) >> 5, bias_of);
+    if (KIND != VQL_PLAIN && inside && a.splits == 1) vql_ask_bias<T, TJ>(a, jw, vql_fresh(lane) >> 5, bias_of);
     if (more) {
       choose(n);
       begin_early();
@@ -951,15 +951,15 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
             *reinterpret_cast<vql_f32x4*>(to + ((u * TJ + v) * 4 + g) * 256) = w;
           }
     } else if (inside) {
-      vql_write<T, TI, TJ>(a, iw, jw, vql_fresh(lane), bias_of, acc);
+      vql_write<T, KIND, TI, TJ>(a, iw, jw, vql_fresh(lane), bias_of, acc);
     } else {
       const int l = vql_fresh(lane);
 #pragma unroll
       for (int u = 0; u < TI; ++u)
 #pragma unroll
-        for (int v = 0; v < TJ; ++v) vql_write_lane<T>(a, iw + u * 32 + (l & 31), jw + v * 32, l >> 5, acc[u][v]);
+        for (int v = 0; v < TJ; ++v) vql_write_lane<T, KIND>(a, iw + u * 32 + (l & 31), jw + v * 32, l >> 5, acc[u][v]);
     }
-    young = a.splits > 1 ? P : inside ? (a.pre ? 2 * S : S) : 0;
+    young = a.splits > 1 ? P : inside ? (KIND != VQL_PLAIN && a.pre ? 2 * S : S) : 0;
     if (!more) break;
   }
 }
@@ -973,10 +973,10 @@ int vql_product_f16(const VqLinearArgs& a, int layout, int config, bool dma, hip
 
 namespace {
 // One kernel of the family: its entry in the table of kernels with large LDS, and its launch.
-template <typename T, bool AMM, bool BMM, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
+template <typename T, bool AMM, bool BMM, int KIND, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
 struct VqProduct {
   static constexpr int LDS = NS * (BI + BJ) * 128;
-  static const void* address() { return reinterpret_cast<const void*>(&vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, NS, DMA>); }
+  static const void* address() { return reinterpret_cast<const void*>(&vql_product_kernel<T, AMM, BMM, KIND, BI, BJ, WI, WJ, NS, DMA>); }
   static inline VqLdsRegistrar registrar{address(), LDS};
   static int launch(const VqLinearArgs& a, hipStream_t s) {
     (void)&registrar;
@@ -984,35 +984,41 @@ struct VqProduct {
     if (rc != VQ_OK) return rc;
     const int64_t total = a.tiles_i * a.tiles_j * a.splits;
     const int64_t blocks = total < a.workgroups ? total : a.workgroups;
-    hipLaunchKernelGGL((vql_product_kernel<T, AMM, BMM, BI, BJ, WI, WJ, NS, DMA>), dim3((unsigned)blocks), dim3(WI * WJ * 64), LDS, s, a);
+    hipLaunchKernelGGL((vql_product_kernel<T, AMM, BMM, KIND, BI, BJ, WI, WJ, NS, DMA>), dim3((unsigned)blocks), dim3(WI * WJ * 64), LDS, s, a);
     return vq_hip_status(hipGetLastError());
   }
 };
-template <typename T, bool AMM, bool BMM>
+template <typename T, bool AMM, bool BMM, int KIND>
 int vql_launch_layout(const VqLinearArgs& a, int config, bool dma, hipStream_t s) {
-  if (config == VQL_C256) return dma ? VqProduct<T, AMM, BMM, 256, 256, 2, 4, 2, true>::launch(a, s) : VQ_ERR_INVALID_ARG;
+  if (config == VQL_C256) return dma ? VqProduct<T, AMM, BMM, KIND, 256, 256, 2, 4, 2, true>::launch(a, s) : VQ_ERR_INVALID_ARG;
   if (config == VQL_C128)
-    return dma ? VqProduct<T, AMM, BMM, 128, 128, 2, 2, 2, true>::launch(a, s) : VqProduct<T, AMM, BMM, 128, 128, 2, 2, 2, false>::launch(a, s);
-  return dma ? VqProduct<T, AMM, BMM, 64, 64, 2, 2, 3, true>::launch(a, s) : VqProduct<T, AMM, BMM, 64, 64, 2, 2, 2, false>::launch(a, s);
+    return dma ? VqProduct<T, AMM, BMM, KIND, 128, 128, 2, 2, 2, true>::launch(a, s) : VqProduct<T, AMM, BMM, KIND, 128, 128, 2, 2, 2, false>::launch(a, s);
+  return dma ? VqProduct<T, AMM, BMM, KIND, 64, 64, 2, 2, 3, true>::launch(a, s) : VqProduct<T, AMM, BMM, KIND, 64, 64, 2, 2, 2, false>::launch(a, s);
 }
 template <typename T>
 int vql_product(const VqLinearArgs& a, int layout, int config, bool dma, hipStream_t s) {
-  if (layout == 0) return vql_launch_layout<T, false, false>(a, config, dma, s);
-  if (layout == 1) return vql_launch_layout<T, false, true>(a, config, dma, s);
-  return vql_launch_layout<T, true, true>(a, config, dma, s);
+  if (layout == 1) return vql_launch_layout<T, false, true, VQL_PLAIN>(a, config, dma, s);
+  if (layout == 2) return vql_launch_layout<T, true, true, VQL_PLAIN>(a, config, dma, s);
+  // a split sum's epilogue is the join's
+  const int kind = a.splits > 1 ? VQL_THRESHOLD : vql_kind(a.act);
+  if (kind == VQL_SIGMOID) return vql_launch_layout<T, false, false, VQL_SIGMOID>(a, config, dma, s);
+  if (kind == VQL_NORMAL) return vql_launch_layout<T, false, false, VQL_NORMAL>(a, config, dma, s);
+  return vql_launch_layout<T, false, false, VQL_THRESHOLD>(a, config, dma, s);
 }
 }  // namespace
 
 // The kernels of one element type (the compiler's host pass leaves kernels out that it meets only through VqProduct).
-#define VQL_KERNELS_OF(T, AMM, BMM)                                                       \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 256, 256, 2, 4, 2, true>(VqLinearArgs);  \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, 2, true>(VqLinearArgs);  \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 128, 128, 2, 2, 2, false>(VqLinearArgs); \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, 3, true>(VqLinearArgs);    \
-  template __global__ void vql_product_kernel<T, AMM, BMM, 64, 64, 2, 2, 2, false>(VqLinearArgs);
-#define VQL_KERNELS(T)           \
-  namespace {                    \
-  VQL_KERNELS_OF(T, false, false) \
-  VQL_KERNELS_OF(T, false, true) \
-  VQL_KERNELS_OF(T, true, true)  \
+#define VQL_KERNELS_OF(T, AMM, BMM, KIND)                                                       \
+  template __global__ void vql_product_kernel<T, AMM, BMM, KIND, 256, 256, 2, 4, 2, true>(VqLinearArgs);  \
+  template __global__ void vql_product_kernel<T, AMM, BMM, KIND, 128, 128, 2, 2, 2, true>(VqLinearArgs);  \
+  template __global__ void vql_product_kernel<T, AMM, BMM, KIND, 128, 128, 2, 2, 2, false>(VqLinearArgs); \
+  template __global__ void vql_product_kernel<T, AMM, BMM, KIND, 64, 64, 2, 2, 3, true>(VqLinearArgs);    \
+  template __global__ void vql_product_kernel<T, AMM, BMM, KIND, 64, 64, 2, 2, 2, false>(VqLinearArgs);
+#define VQL_KERNELS(T)                              \
+  namespace {                                       \
+  VQL_KERNELS_OF(T, false, false, VQL_THRESHOLD)    \
+  VQL_KERNELS_OF(T, false, false, VQL_SIGMOID)      \
+  VQL_KERNELS_OF(T, false, false, VQL_NORMAL)       \
+  VQL_KERNELS_OF(T, false, true, VQL_PLAIN)         \
+  VQL_KERNELS_OF(T, true, true, VQL_PLAIN)          \
   }

@@ -34,7 +34,10 @@ template <typename T>
 __device__ __forceinline__ void epilogue_one(const VqLinearArgs& a, int64_t i, int j, float c) {
   if (a.bias) c += VqElem<T>::to(reinterpret_cast<const T*>(a.bias)[j]);
   if (a.pre) reinterpret_cast<T*>(a.pre)[i * a.J + j] = VqElem<T>::from(c);
-  c = vql_act<sizeof(T) == 2>(c, a.act);
+  const int kind = vql_kind(a.act);
+  c = kind == VQL_THRESHOLD ? vql_act_of<VQL_THRESHOLD, sizeof(T) == 2>(c, a.act)
+      : kind == VQL_SIGMOID ? vql_act_of<VQL_SIGMOID, sizeof(T) == 2>(c, a.act)
+                            : vql_act_of<VQL_NORMAL, sizeof(T) == 2>(c, a.act);
   if (a.res) c += VqElem<T>::to(reinterpret_cast<const T*>(a.res + i * a.ldr)[j]);
   reinterpret_cast<T*>(a.out)[i * a.J + j] = VqElem<T>::from(c);
 }
@@ -117,7 +120,10 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a, int tile,
 #pragma unroll
     for (int e = 0; e < 4; ++e) all[4 * g + e] = t[e];
   }
-  vql_write_lane<T>(a, r, cv, lane >> 5, all);
+  const int kind = vql_kind(a.act);
+  if (kind == VQL_THRESHOLD) vql_write_lane<T, VQL_THRESHOLD>(a, r, cv, lane >> 5, all);
+  else if (kind == VQL_SIGMOID) vql_write_lane<T, VQL_SIGMOID>(a, r, cv, lane >> 5, all);
+  else vql_write_lane<T, VQL_NORMAL>(a, r, cv, lane >> 5, all);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, int splits, int64_t n, T* out) {
