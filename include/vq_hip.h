@@ -364,8 +364,9 @@ int vq_linear_backward(const void* gy, const void* pre, const void* x, int64_t l
  * vq_grad_norm:  norm[0] = (sum |g|^p)^(1/p) over all elements of all tensors, summed in 64 bits, a NaN or
  *                infinity included (no tensor at all, or only empty ones: 0).  dst is not looked at.
  * vq_clip_grads: that norm, then dst = round(src * min(1, max_norm / (norm + 1e-6))).  dst_type is src_type, or
- *                VQ_F32; dst == src (of one type) scales in place.  Otherwise no dst may overlap any src or other dst,
- *                and in place no tensor may be listed twice.  max_norm >= 0.
+ *                VQ_F32; dst == src (of one type) scales in place.  Apart from that no two of the srcs and dsts may
+ *                overlap (VQ_ERR_INVALID_ARG).  max_norm >= 0.
+ * vq_tensor_refs_overlap: 1 where vq_clip_grads would refuse the list for that reason, 0 otherwise (host only).
  * The result is the same bits on every run.  `work`: vq_grad_norm_work_bytes(n) bytes, 8-byte aligned, contents
  * irrelevant; calls that may overlap need one each.  At most 65536 tensors (VQ_ERR_TOO_LARGE).
  */
@@ -377,6 +378,7 @@ typedef struct vq_tensor_ref {
   int32_t src_type;
   int32_t dst_type;
 } vq_tensor_ref;
+int vq_tensor_refs_overlap(const vq_tensor_ref* refs, int n);
 int64_t vq_grad_norm_work_bytes(int n);
 int vq_grad_norm(const vq_tensor_ref* refs, int n, int kind, float* norm, void* work, void* stream);
 int vq_clip_grads(const vq_tensor_ref* refs, int n, int kind, float max_norm, float* norm, void* work, void* stream);

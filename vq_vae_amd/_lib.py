@@ -97,6 +97,7 @@ SIGNATURES = {
                                 c_void_p]),
     "vq_linear_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int64, c_int,
                                    c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "vq_tensor_refs_overlap": (c_int, [c_void_p, c_int]),
     "vq_grad_norm_work_bytes": (c_int64, [c_int]),
     "vq_grad_norm": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "vq_clip_grads": (c_int, [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),

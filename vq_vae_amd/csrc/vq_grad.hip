@@ -15,6 +15,7 @@
 //   * Every workgroup writes one partial sum; the readers add them all in a fixed order.  No atomics, no counter that
 //     would have to be cleared, the same bits on every run.
 #include <algorithm>
+#include <new>
 
 #include "vq_linear.h"
 
@@ -260,6 +261,27 @@ int run_partials(const vq_tensor_ref* refs, int n, int kind, int64_t chunks, dou
 
 }  // namespace
 
+extern "C" int vq_tensor_refs_overlap(const vq_tensor_ref* refs, int n) {
+  if (n <= 0 || !refs) return 0;
+  struct Run { uintptr_t at, end; };
+  Run few[256];
+  Run* runs = n <= 128 ? few : new (std::nothrow) Run[2 * (size_t)n];
+  if (!runs) return 1;
+  size_t k = 0;
+  for (int i = 0; i < n; ++i) {
+    const vq_tensor_ref& r = refs[i];
+    if (r.numel <= 0) continue;
+    const uintptr_t s = reinterpret_cast<uintptr_t>(r.src), d = reinterpret_cast<uintptr_t>(r.dst);
+    runs[k++] = {d, d + (uintptr_t)r.numel * (r.dst_type == VQ_F32 ? 4 : 2)};
+    if (s != d || r.src_type != r.dst_type) runs[k++] = {s, s + (uintptr_t)r.numel * (r.src_type == VQ_F32 ? 4 : 2)};
+  }
+  std::sort(runs, runs + k, [](const Run& a, const Run& b) { return a.at < b.at; });
+  int found = 0;
+  for (size_t i = 1; i < k; ++i) found |= runs[i].at < runs[i - 1].end;
+  if (runs != few) delete[] runs;
+  return found;
+}
+
 extern "C" int64_t vq_grad_norm_work_bytes(int n) { return n < 0 ? 0 : ((int64_t)G_WGS + launches_of(n)) * 8; }
 
 extern "C" int vq_grad_norm(const vq_tensor_ref* refs, int n, int kind, float* norm, void* work, void* stream) {
@@ -282,6 +304,7 @@ extern "C" int vq_clip_grads(const vq_tensor_ref* refs, int n, int kind, float m
   if (ok != VQ_OK) return ok;
   if (kind < VQ_NORM_INF || kind > VQ_NORM_2 || !norm || !work || (reinterpret_cast<uintptr_t>(work) & 7) || !(max_norm >= 0.0f))
     return VQ_ERR_INVALID_ARG;
+  if (vq_tensor_refs_overlap(refs, n)) return VQ_ERR_INVALID_ARG;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* part = reinterpret_cast<double*>(work);
   int n_part = 0;

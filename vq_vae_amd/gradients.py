@@ -6,10 +6,10 @@ to the host.  GPU only.
 """
 from __future__ import annotations
 
+import array
 import math
 from typing import Iterable, List, Optional, Sequence, Union
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -17,7 +17,6 @@ from ._lib import NORM_1, NORM_2, NORM_INF, check
 from .projection import DTYPES
 from .ops import _on_device, _raw_stream, _require_cuda
 
-_ITEM = np.array([4, 2, 2], np.int64)        # bytes of an element, by the C interface's types
 _KINDS = {1.0: NORM_1, 2.0: NORM_2, math.inf: NORM_INF}
 
 
@@ -66,37 +65,27 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _refs(srcs: Sequence[torch.Tensor], dsts: Sequence[torch.Tensor]) -> np.ndarray:
+def _refs(srcs: Sequence[torch.Tensor], dsts: Sequence[torch.Tensor]) -> array.array:
     """The vq_tensor_ref array of the C interface: four 64-bit words an entry."""
-    refs = np.empty((len(srcs), 4), np.int64)
-    refs[:, 0] = [t.data_ptr() for t in srcs]
-    refs[:, 2] = [t.numel() for t in srcs]
-    refs[:, 3] = [DTYPES[t.dtype] for t in srcs]
-    if dsts is srcs:
-        refs[:, 1] = refs[:, 0]
-        refs[:, 3] *= (1 << 32) + 1
-    else:
-        refs[:, 1] = [t.data_ptr() for t in dsts]
-        refs[:, 3] += [DTYPES[t.dtype] << 32 for t in dsts]
-    return refs
+    words: List[int] = []
+    for s, d in zip(srcs, dsts):
+        words += (s.data_ptr(), d.data_ptr(), s.numel(), DTYPES[s.dtype] | DTYPES[d.dtype] << 32)
+    return array.array("q", words)
 
 
-def _refuse_overlap(start: np.ndarray, size: np.ndarray) -> None:
-    """Raises where two runs of memory overlap: a kernel over all of them would race with itself."""
-    some = size > 0
-    start, size = start[some], size[some]
-    order = start.argsort()
-    start, end = start[order], (start + size)[order]
-    if (end[:-1] > start[1:]).any():
+def _spans(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]) -> array.array:
+    """The memory of all tensors as such an array, each from its first to its last element (a tensor with gaps, like columns of
+    a matrix, counts whole), once where it is scaled in place."""
+    words: List[int] = []
+    for t in (*written, *(g for g, o in zip(grads, written) if g is not o)):
+        span = t.numel() and 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+        words += (t.data_ptr(), t.data_ptr(), span, DTYPES[t.dtype] * ((1 << 32) + 1))
+    return array.array("q", words)
+
+
+def _refuse_overlap(refs: array.array) -> None:
+    if _lib.load().vq_tensor_refs_overlap(refs.buffer_info()[0], len(refs) // 4):
         raise ValueError("gradients that are to be scaled share memory: each may be given once")
-
-
-def _runs(refs: np.ndarray):
-    """Addresses and sizes of the memory that clipping touches: once for a tensor scaled in place."""
-    size = refs[:, 2]
-    apart = (refs[:, 0] != refs[:, 1]) | (refs[:, 3] & 0xff != refs[:, 3] >> 32)
-    return (np.concatenate((refs[apart, 0], refs[:, 1])),
-            np.concatenate((size[apart] * _ITEM[refs[apart, 3] & 0xff], size * _ITEM[refs[:, 3] >> 32])))
 
 
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
@@ -117,7 +106,7 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
         norm = torch.empty((), dtype=torch.float32, device=device)
         work = torch.empty(lib.vq_grad_norm_work_bytes(len(flat)), dtype=torch.uint8, device=device)
         refs = _refs(flat, flat)
-        check(lib.vq_grad_norm(refs.ctypes.data, len(flat), kind, norm.data_ptr(), work.data_ptr(), _raw_stream(device)), "vq_grad_norm")
+        check(lib.vq_grad_norm(refs.buffer_info()[0], len(flat), kind, norm.data_ptr(), work.data_ptr(), _raw_stream(device)), "vq_grad_norm")
     return norm
 
 
@@ -137,24 +126,29 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         out = _list(out, "out")
         if len(out) != len(grads):
             raise ValueError(f"{len(grads)} gradients but {len(out)} tensors in out")
-        for g, o in zip(grads, out):
+    if not grads:
+        return torch.zeros(())
+    written = grads if out is None else out
+    dense = True
+    for g, o in zip(grads, written):
+        if g is not o:
             if o.shape != g.shape:
                 raise ValueError(f"out has shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
             if o.dtype != g.dtype and o.dtype != torch.float32:
                 raise TypeError(f"out is {o.dtype} for a {g.dtype} gradient: the same type or float32")
-            if o.device != g.device:
-                raise ValueError(f"out is on {o.device}, the gradients on {g.device}")
             if o.requires_grad and o.is_leaf and torch.is_grad_enabled():
                 raise ValueError("out requires a gradient itself")
-    if not grads:
-        return torch.zeros(())
-    written = grads if out is None else out
-    dense = all([t.is_contiguous() for t in grads]) and (out is None or all([t.is_contiguous() for t in out]))
+        if not (g.is_contiguous() and o.is_contiguous()):
+            dense = False
+            if o.numel() and any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
+                raise ValueError("an expanded tensor cannot be scaled: several of its elements are one")
+    if written[0].device != grads[0].device:
+        raise ValueError(f"out is on {written[0].device}, the gradients on {grads[0].device}")
     if dense:
         refs = _refs(grads, written)
-        _refuse_overlap(*_runs(refs))
+        _refuse_overlap(refs)
     else:
-        _refuse_strides(grads, written)
+        _refuse_overlap(_spans(grads, written))
     _require_cuda(grads[0], "grads")
     device = grads[0].device
     with _on_device(device):
@@ -166,25 +160,14 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         lib = _lib.load()
         norm = torch.empty((), dtype=torch.float32, device=device)
         work = torch.empty(lib.vq_grad_norm_work_bytes(len(grads)), dtype=torch.uint8, device=device)
-        check(lib.vq_clip_grads(refs.ctypes.data, len(grads), kind, max_norm, norm.data_ptr(), work.data_ptr(),
+        check(lib.vq_clip_grads(refs.buffer_info()[0], len(grads), kind, max_norm, norm.data_ptr(), work.data_ptr(),
                                 _raw_stream(device)), "vq_clip_grads")
-        with torch.no_grad():
-            for o, c in back:
-                o.copy_(c)
+        if back:
+            with torch.no_grad():
+                for o, c in back:
+                    o.copy_(c)
         torch.autograd.graph.increment_version([t for t in dsts if not t.is_inference()])
     return norm
-
-
-def _refuse_strides(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]) -> None:
-    """Refusals of a list with tensors that are not contiguous.  One with gaps (columns of a matrix) counts from its first to
-    its last element."""
-    for t in written:
-        if t.numel() and any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
-            raise ValueError("an expanded tensor cannot be scaled: several of its elements are one")
-    tensors = list(written) + [g for g, o in zip(grads, written) if g.data_ptr() != o.data_ptr()]
-    _refuse_overlap(np.array([t.data_ptr() for t in tensors], np.int64),
-                    np.array([t.numel() and (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
-                              for t in tensors], np.int64))
 
 
 def _dense_pairs(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]):

@@ -135,14 +135,21 @@ class _LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, pre = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        gx = gw = gb = None
-        if any(need[:3]):
-            gx, gw, gb = linear_backward(grad, x, weight, pre, ctx.activation, *need[:3])
-        return gx, gw, gb, grad if need[3] else None, None
+        # under create_graph the result has to refuse a second derivative; the wrapper that sees to it takes 5 us
+        return _gradients_once(ctx, grad) if torch.is_grad_enabled() else _gradients(ctx, grad)
+
+
+def _gradients(ctx, grad):
+    x, weight, pre = ctx.saved_tensors
+    want_x, want_weight, want_bias, want_residual, _ = ctx.needs_input_grad
+    gx = gw = gb = None
+    if want_x or want_weight or want_bias:
+        gx, gw, gb = linear_backward(grad, x, weight, pre, ctx.activation, want_x, want_weight, want_bias)
+    return gx, gw, gb, grad if want_residual else None, None
+
+
+_gradients_once = torch.autograd.function.once_differentiable(_gradients)
 
 
 def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
