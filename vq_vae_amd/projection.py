@@ -107,27 +107,41 @@ def linear_forward(x, weight, bias=None, activation: str = "none", residual=None
 def linear_backward(grad, x, weight, pre, activation: str, want_x: bool, want_weight: bool, want_bias: bool):
     """Gradients ``(input, weight, bias)`` of ``act(x W^T + b)`` for the output gradient ``grad`` (None where not
     wanted); ``pre`` is what :func:`linear_forward` returned (None for activation "none")."""
-    N, K = weight.shape
-    dt = DTYPES[x.dtype]
-    device = x.device
-    with _on_device(device):
-        g = grad.reshape(-1, N).contiguous()
-        M = g.shape[0]
-        x2, w2 = _rows(x, K), _rows(weight, K)
-        gx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_x else None
-        gw = torch.empty((N, K), dtype=x.dtype, device=device) if want_weight else None
-        gb = torch.empty((N,), dtype=x.dtype, device=device) if want_bias else None
-        work = _work(LINEAR_BACKWARD, M, K, N, dt, device)
-        check(_lib.load().vq_linear_backward(g.data_ptr(), _address(pre), x2.data_ptr(), _pitch(x2), w2.data_ptr(),
-                                             _pitch(w2), dt, ACTIVATIONS[activation], M, K, N, _address(gx) if M else None,
-                                             _address(gw), _address(gb), _address(work), _raw_stream(device)),
-              "vq_linear_backward")
+    with _on_device(x.device):
+        x2, w2 = _rows(x, weight.shape[1]), _rows(weight, weight.shape[1])
+        return _backward(_facts(x2, w2, activation), grad, x.shape, x2, w2, pre, want_x, want_weight, want_bias)
+
+
+def _facts(x2: torch.Tensor, w2: torch.Tensor, activation: str):
+    """What a backward pass needs besides addresses."""
+    (M, K), N, dt = x2.shape, w2.shape[0], DTYPES[x2.dtype]
+    return M, K, N, dt, ACTIVATIONS[activation], _pitch(x2), _pitch(w2), _work_bytes(LINEAR_BACKWARD, M, K, N, dt)
+
+
+def _backward(facts, grad, shape, x2, w2, pre, want_x: bool, want_weight: bool, want_bias: bool):
+    # on the current device; x2, w2: tensors that start where the rows do
+    M, K, N, dt, act, ldx, ldw, work_bytes = facts
+    g = grad if grad.is_contiguous() else grad.contiguous()
+    dtype, device = g.dtype, g.device
+    gx = torch.empty(shape, dtype=dtype, device=device) if want_x else None
+    gw = torch.empty((N, K), dtype=dtype, device=device) if want_weight else None
+    gb = torch.empty((N,), dtype=dtype, device=device) if want_bias else None
+    work = torch.empty(work_bytes, dtype=torch.uint8, device=device) if work_bytes else None
+    check(_lib.load().vq_linear_backward(g.data_ptr(), None if pre is None else pre.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(),
+                                         ldw, dt, act, M, K, N, gx.data_ptr() if want_x and M else None,
+                                         gw.data_ptr() if want_weight else None, gb.data_ptr() if want_bias else None,
+                                         None if work is None else work.data_ptr(), _raw_stream(device)), "vq_linear_backward")
     return gx, gw, gb
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
+        N, K = weight.shape
+        x2, w2 = _rows(x, K), _rows(weight, K)
+        # a backward pass on the engine's thread takes about twice as long per line as here: what it can know is found out now
+        ctx.facts = _facts(x2, w2, activation)
+        ctx.in_place = x2.data_ptr() == x.data_ptr() and w2 is weight      # the rows are the tensors' own memory
         ctx.activation = activation
         want_pre = activation != "none" and any(ctx.needs_input_grad[:3])
         y, pre = linear_forward(x, weight, bias, activation, residual, want_pre)
@@ -145,7 +159,11 @@ def _gradients(ctx, grad):
     want_x, want_weight, want_bias, want_residual, _ = ctx.needs_input_grad
     gx = gw = gb = None
     if want_x or want_weight or want_bias:
-        gx, gw, gb = linear_backward(grad, x, weight, pre, ctx.activation, want_x, want_weight, want_bias)
+        if ctx.in_place:
+            with _on_device(x.device):
+                gx, gw, gb = _backward(ctx.facts, grad, x.shape, x, weight, pre, want_x, want_weight, want_bias)
+        else:
+            gx, gw, gb = linear_backward(grad, x, weight, pre, ctx.activation, want_x, want_weight, want_bias)
     return gx, gw, gb, grad if want_residual else None, None
 
 
