@@ -392,3 +392,26 @@ def test_captured_and_replayed(M):
             want = step(new[0].requires_grad_(), *new[1:])
             for o, e in zip(outs, want):
                 assert torch.equal(o, e)
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_hooks_on_saved_tensors(act):
+    # a hook may bring a saved tensor back with other strides (copied away and back, as offloading does): the gradients are
+    # those without it; one of another shape, type or device is refused
+    M, K, N = 70, 40, 24
+    x, w, b, r, gy = make(M, K, N, torch.bfloat16, True, True, True, 6)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+
+    def run(pack, unpack, gy=gy):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = vq.linear(x, w, b, act, r)
+        return torch.autograd.grad(y, leaves, gy)
+    want = run(lambda t: t, lambda t: t)
+    turned = gy.t().contiguous().t()
+    away = lambda t: t.cpu().contiguous()
+    for got in (run(away, lambda t: t.to(DEV)), run(away, lambda t: t.to(DEV).t().contiguous().t()),
+                run(lambda t: t, lambda t: t, turned), run(away, lambda t: t.to(DEV), turned)):
+        assert all(torch.equal(a, c) for a, c in zip(want, got))
+    for wrong in (lambda t: t, lambda t: t.to(DEV).float(), lambda t: t.to(DEV)[:, 1:], lambda t: t.to(DEV)[1:]):
+        with pytest.raises(RuntimeError, match="hook on saved tensors"):
+            run(away, wrong)

@@ -109,7 +109,8 @@ def linear_backward(grad, x, weight, pre, activation: str, want_x: bool, want_we
     wanted); ``pre`` is what :func:`linear_forward` returned (None for activation "none")."""
     with _on_device(x.device):
         x2, w2 = _rows(x, weight.shape[1]), _rows(weight, weight.shape[1])
-        return _backward(_facts(x2, w2, activation), grad, x.shape, x2, w2, pre, want_x, want_weight, want_bias)
+        p = None if pre is None else pre.contiguous()
+        return _backward(_facts(x2, w2, activation), grad, x.shape, x2, w2, p, want_x, want_weight, want_bias)
 
 
 def _facts(x2: torch.Tensor, w2: torch.Tensor, activation: str):
@@ -118,8 +119,12 @@ def _facts(x2: torch.Tensor, w2: torch.Tensor, activation: str):
     return M, K, N, dt, ACTIVATIONS[activation], _pitch(x2), _pitch(w2), _work_bytes(LINEAR_BACKWARD, M, K, N, dt)
 
 
+def _layout(t: torch.Tensor):
+    return t.shape, t.stride(), t.dtype, t.device
+
+
 def _backward(facts, grad, shape, x2, w2, pre, want_x: bool, want_weight: bool, want_bias: bool):
-    # on the current device; x2, w2: tensors that start where the rows do
+    # on the current device; x2, w2: tensors that start where the rows do; pre: dense
     M, K, N, dt, act, ldx, ldw, work_bytes = facts
     g = grad if grad.is_contiguous() else grad.contiguous()
     dtype, device = g.dtype, g.device
@@ -142,6 +147,7 @@ class _LinearFn(torch.autograd.Function):
         # a backward pass on the engine's thread takes about twice as long per line as here: what it can know is found out now
         ctx.facts = _facts(x2, w2, activation)
         ctx.in_place = x2.data_ptr() == x.data_ptr() and w2 is weight      # the rows are the tensors' own memory
+        ctx.layouts = _layout(x), _layout(weight)
         ctx.activation = activation
         want_pre = activation != "none" and any(ctx.needs_input_grad[:3])
         y, pre = linear_forward(x, weight, bias, activation, residual, want_pre)
@@ -154,15 +160,29 @@ class _LinearFn(torch.autograd.Function):
         return _gradients_once(ctx, grad) if torch.is_grad_enabled() else _gradients(ctx, grad)
 
 
+def _check_saved(ctx, grad, x, weight, pre) -> None:
+    """Hooks on saved tensors may hand back others than were saved: other strides are fine, nothing else is."""
+    wanted = [(t, (layout[0], *layout[2:])) for t, layout in zip((x, weight), ctx.layouts)]
+    if pre is not None:
+        wanted.append((pre, (grad.shape, grad.dtype, grad.device)))
+    for t, want in wanted:
+        if (t.shape, t.dtype, t.device) != want:
+            raise RuntimeError(f"a hook on saved tensors returned {tuple(t.shape)}, {t.dtype} on {t.device} "
+                               f"for {tuple(want[0])}, {want[1]} on {want[2]}")
+
+
 def _gradients(ctx, grad):
     x, weight, pre = ctx.saved_tensors
     want_x, want_weight, want_bias, want_residual, _ = ctx.needs_input_grad
     gx = gw = gb = None
     if want_x or want_weight or want_bias:
-        if ctx.in_place:
+        same = (_layout(x), _layout(weight)) == ctx.layouts and (pre is None or _layout(pre) == _layout(grad))
+        if same and ctx.in_place and grad.is_contiguous():
             with _on_device(x.device):
                 gx, gw, gb = _backward(ctx.facts, grad, x.shape, x, weight, pre, want_x, want_weight, want_bias)
         else:
+            if not same:
+                _check_saved(ctx, grad, x, weight, pre)
             gx, gw, gb = linear_backward(grad, x, weight, pre, ctx.activation, want_x, want_weight, want_bias)
     return gx, gw, gb, grad if want_residual else None, None
 
