@@ -81,14 +81,15 @@ __device__ __forceinline__ void vql_store16(void* p, u32x4 v) {
   if constexpr (sizeof(T) == 4) *reinterpret_cast<vql_u32x4_a4*>(p) = v;
   else *reinterpret_cast<vql_u32x4_a2*>(p) = v;
 }
-// The same, and past the caches if `stream`: outputs of the product are not read again by it, and keep its operands out of the
-// L2 otherwise (64 Ki x 1024 -> 1024 bf16 143 -> 130 us, 64 Ki x 64 -> 1024 42 -> 37).  Only for accesses that fill 64-byte
-// runs: with rows of 6766 bytes, whose runs straddle the lines, the same kernel took 103 us instead of 64.
-template <typename T>
-__device__ __forceinline__ void vql_stream16(bool stream, void* p, u32x4 v) {
-  if (!stream) vql_store16<T>(p, v);
-  else if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(v, reinterpret_cast<vql_u32x4_a4*>(p));
-  else __builtin_nontemporal_store(v, reinterpret_cast<vql_u32x4_a2*>(p));
+// The same, and past the caches if STREAM: outputs of the product are not read again by it, and keep its operands out of the
+// L2 otherwise (operands and outputs out of the caches, bf16: 64 Ki x 256 -> 1024 79 -> 55 us, 64 Ki x 1024 -> 256 49 -> 45).
+// Only for accesses that fill 64-byte runs: with rows of 6766 bytes, whose runs straddle the lines, the same kernel took
+// 103 us instead of 64.  And only for 16-bit types: fp32 products, bound by the matrix cores, gain nothing (16384 x 1024 -> 4096
+// 1002 us without, 1007 with).  A template argument, because the compiler makes one ordinary store of a branch's two.
+template <typename T, bool STREAM>
+__device__ __forceinline__ void vql_stream16(void* p, u32x4 v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<vql_u32x4_a2*>(p));
+  else vql_store16<T>(p, v);
 }
 // `valid` of the 16 / sizeof(T) elements at p, the others zero
 template <typename T>
@@ -523,7 +524,7 @@ __device__ __forceinline__ void vql_ask_bias(const VqLinearArgs& a, int64_t j, i
 // or 64 bytes of one row in pieces of 16; exchanging every other piece with the lane 16 away makes one access of the wave 64
 // consecutive bytes of 16 rows instead of twice 16 bytes of 32 rows (64 Ki x 256 -> 1024 bf16: 52 instead of 59 us: the L2 takes
 // a request per line and instruction).  The residual of the next row block is on its way while this one is worked on.
-template <typename T, int KIND, int TI, int TJ>
+template <typename T, int KIND, bool STREAM, int TI, int TJ>
 __device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int64_t j, int lane, const u32x4 (&bias_of)[TJ][16 * sizeof(T) / 16],
                                           const f32x16 (&acc)[TI][TJ]) {
   constexpr int ES = sizeof(T), E = 16 / ES, PV = 16 / E;
@@ -533,7 +534,6 @@ __device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int6
   char* const yb = reinterpret_cast<char*>(a.out) + origin;
   char* const pb = reinterpret_cast<char*>(a.pre) + origin;
   const char* const rb = a.res + i * a.ldr + j * ES;
-  const bool stream = ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.pre) | pitch) & 63) == 0;
   const int lc = vql_piece<T>((lane >> 4) & 1, h) * ES;
   const uint32_t yo = (uint32_t)((lane & 15) * (int)pitch + lc), ro = (uint32_t)((lane & 15) * (int)a.ldr + lc);
 #pragma unroll
@@ -571,12 +571,12 @@ __device__ __forceinline__ void vql_write(const VqLinearArgs& a, int64_t i, int6
         }
         const int64_t step = (int64_t)u * 32 * pitch + (v * 32 + 8 * k) * ES;
         vql_swap16(y[0], y[1]);
-        vql_stream16<T>(stream, yb + step + yo, y[0]);
-        vql_stream16<T>(stream, yb + step + 16 * pitch + yo, y[1]);
+        vql_stream16<T, STREAM>(yb + step + yo, y[0]);
+        vql_stream16<T, STREAM>(yb + step + 16 * pitch + yo, y[1]);
         if (KIND != VQL_PLAIN && a.pre) {
           vql_swap16(pre[0], pre[1]);
-          vql_stream16<T>(stream, pb + step + yo, pre[0]);
-          vql_stream16<T>(stream, pb + step + 16 * pitch + yo, pre[1]);
+          vql_stream16<T, STREAM>(pb + step + yo, pre[0]);
+          vql_stream16<T, STREAM>(pb + step + 16 * pitch + yo, pre[1]);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -765,7 +765,7 @@ namespace {   // the kernels of a translation unit are its own
 // (BI / WI) x (BJ / WJ) of it in 32x32 accumulator tiles.  DMA: rows start on 16 bytes, so that the tiles go straight into
 // LDS; otherwise they go through registers.
 template <typename T, bool AMM, bool BMM, int KIND, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
-__global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_product_kernel(VqLinearArgs a) {
+__global__ __launch_bounds__(WI * WJ * 64, 2) void vql_product_kernel(VqLinearArgs a) {
   constexpr int NT = WI * WJ * 64;
   constexpr int TI = BI / WI / 32, TJ = BJ / WJ / 32;
   constexpr int STAGE = (BI + BJ) * 128;
@@ -951,7 +951,13 @@ __global__ __launch_bounds__(WI * WJ * 64, WI * WJ == 8 ? 2 : 2) void vql_produc
             *reinterpret_cast<vql_f32x4*>(to + ((u * TJ + v) * 4 + g) * 256) = w;
           }
     } else if (inside) {
-      vql_write<T, KIND, TI, TJ>(a, iw, jw, vql_fresh(lane), bias_of, acc);
+      const uintptr_t runs = reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.pre) | (a.J * sizeof(T));
+      if (sizeof(T) == 2 && (runs & 63) == 0) {
+        asm volatile("; a block that starts unlike the other: else what both begin with is kept in registers, which spill");
+        vql_write<T, KIND, true, TI, TJ>(a, iw, jw, vql_fresh(lane), bias_of, acc);
+      } else {
+        vql_write<T, KIND, false, TI, TJ>(a, iw, jw, vql_fresh(lane), bias_of, acc);
+      }
     } else {
       const int l = vql_fresh(lane);
 #pragma unroll
