@@ -415,3 +415,15 @@ def test_hooks_on_saved_tensors(act):
     for wrong in (lambda t: t, lambda t: t.to(DEV).float(), lambda t: t.to(DEV)[:, 1:], lambda t: t.to(DEV)[1:]):
         with pytest.raises(RuntimeError, match="hook on saved tensors"):
             run(away, wrong)
+
+
+def test_recomputed_in_the_backward_pass():
+    # checkpointing hands the backward pass tensors of a second forward pass
+    from torch.utils.checkpoint import checkpoint
+    x, w, b, r, gy = make(33, 40, 24, torch.float16, True, True, False, 9)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    f = lambda x, r: vq.linear(vq.linear(x, w, b, "silu", r), w.t()[:, :24], None, "gelu")   # the second weight is copied first
+    def grads(out):
+        return torch.autograd.grad(out, leaves, torch.ones_like(out))
+    want = grads(f(x, r))
+    assert all(torch.equal(a, c) for a, c in zip(want, grads(checkpoint(f, x, r, use_reentrant=False))))

@@ -84,23 +84,25 @@ def _check(x, weight, bias, activation, residual) -> None:
 def linear_forward(x, weight, bias=None, activation: str = "none", residual=None, want_pre: bool = False):
     """``(y, pre)``: ``pre = x W^T + bias`` (None unless wanted) and ``y = act(pre) + residual``, without autograd.
     Arguments as :func:`linear`, already checked."""
-    N, K = weight.shape
-    dt = DTYPES[x.dtype]
-    device = x.device
-    with _on_device(device):
-        x2, w2 = _rows(x, K), _rows(weight, K)
-        M = x2.shape[0]
-        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=device)
-        pre = torch.empty_like(y) if want_pre else None
-        b = None if bias is None else bias.contiguous()
-        r2, ldr = None, 0
-        if residual is not None:
-            r2 = _rows(residual, N)
-            ldr = _pitch(r2)
-        work = _work(LINEAR_FORWARD, M, K, N, dt, device)
-        check(_lib.load().vq_linear(x2.data_ptr(), _pitch(x2), w2.data_ptr(), _pitch(w2), _address(b), _address(r2), ldr, dt,
-                                    ACTIVATIONS[activation], M, K, N, y.data_ptr(), _address(pre), _address(work),
-                                    _raw_stream(device)), "vq_linear")
+    with _on_device(x.device):
+        K = weight.shape[1]
+        return _forward(_rows(x, K), _rows(weight, K), x.shape[:-1], bias, activation, residual, want_pre)
+
+
+def _forward(x2, w2, outer, bias, activation: str, residual, want_pre: bool):
+    # on the current device; x2, w2: tensors that start where the rows do
+    (M, K), N, dt, device = x2.shape, w2.shape[0], DTYPES[x2.dtype], x2.device
+    y = torch.empty((*outer, N), dtype=x2.dtype, device=device)
+    pre = torch.empty_like(y) if want_pre else None
+    b = None if bias is None else bias.contiguous()
+    r2, ldr = None, 0
+    if residual is not None:
+        r2 = _rows(residual, N)
+        ldr = _pitch(r2)
+    work = _work(LINEAR_FORWARD, M, K, N, dt, device)
+    check(_lib.load().vq_linear(x2.data_ptr(), _pitch(x2), w2.data_ptr(), _pitch(w2), _address(b), _address(r2), ldr, dt,
+                                ACTIVATIONS[activation], M, K, N, y.data_ptr(), _address(pre), _address(work),
+                                _raw_stream(device)), "vq_linear")
     return y, pre
 
 
@@ -110,7 +112,7 @@ def linear_backward(grad, x, weight, pre, activation: str, want_x: bool, want_we
     with _on_device(x.device):
         x2, w2 = _rows(x, weight.shape[1]), _rows(weight, weight.shape[1])
         p = None if pre is None else pre.contiguous()
-        return _backward(_facts(x2, w2, activation), grad, x.shape, x2, w2, p, want_x, want_weight, want_bias)
+        return _backward(_facts(x2, w2, activation), grad.contiguous(), x.shape, x2, w2, p, want_x, want_weight, want_bias)
 
 
 def _facts(x2: torch.Tensor, w2: torch.Tensor, activation: str):
@@ -119,20 +121,15 @@ def _facts(x2: torch.Tensor, w2: torch.Tensor, activation: str):
     return M, K, N, dt, ACTIVATIONS[activation], _pitch(x2), _pitch(w2), _work_bytes(LINEAR_BACKWARD, M, K, N, dt)
 
 
-def _layout(t: torch.Tensor):
-    return t.shape, t.stride(), t.dtype, t.device
-
-
 def _backward(facts, grad, shape, x2, w2, pre, want_x: bool, want_weight: bool, want_bias: bool):
-    # on the current device; x2, w2: tensors that start where the rows do; pre: dense
+    # on the current device; x2, w2: tensors that start where the rows do; grad, pre: dense
     M, K, N, dt, act, ldx, ldw, work_bytes = facts
-    g = grad if grad.is_contiguous() else grad.contiguous()
-    dtype, device = g.dtype, g.device
+    dtype, device = grad.dtype, grad.device
     gx = torch.empty(shape, dtype=dtype, device=device) if want_x else None
     gw = torch.empty((N, K), dtype=dtype, device=device) if want_weight else None
     gb = torch.empty((N,), dtype=dtype, device=device) if want_bias else None
     work = torch.empty(work_bytes, dtype=torch.uint8, device=device) if work_bytes else None
-    check(_lib.load().vq_linear_backward(g.data_ptr(), None if pre is None else pre.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(),
+    check(_lib.load().vq_linear_backward(grad.data_ptr(), None if pre is None else pre.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(),
                                          ldw, dt, act, M, K, N, gx.data_ptr() if want_x and M else None,
                                          gw.data_ptr() if want_weight else None, gb.data_ptr() if want_bias else None,
                                          None if work is None else work.data_ptr(), _raw_stream(device)), "vq_linear_backward")
@@ -142,15 +139,16 @@ def _backward(facts, grad, shape, x2, w2, pre, want_x: bool, want_weight: bool, 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        N, K = weight.shape
-        x2, w2 = _rows(x, K), _rows(weight, K)
+        K = weight.shape[1]
+        want_pre = activation != "none" and any(ctx.needs_input_grad[:3])
+        with _on_device(x.device):
+            x2, w2 = _rows(x, K), _rows(weight, K)
+            y, pre = _forward(x2, w2, x.shape[:-1], bias, activation, residual, want_pre)
         # a backward pass on the engine's thread takes about twice as long per line as here: what it can know is found out now
         ctx.facts = _facts(x2, w2, activation)
         ctx.in_place = x2.data_ptr() == x.data_ptr() and w2 is weight      # the rows are the tensors' own memory
-        ctx.layouts = _layout(x), _layout(weight)
+        ctx.layout = x.shape, x.stride(), weight.shape, weight.stride(), x.dtype, x.device
         ctx.activation = activation
-        want_pre = activation != "none" and any(ctx.needs_input_grad[:3])
-        y, pre = linear_forward(x, weight, bias, activation, residual, want_pre)
         ctx.save_for_backward(x, weight, pre)
         return y
 
@@ -160,29 +158,22 @@ class _LinearFn(torch.autograd.Function):
         return _gradients_once(ctx, grad) if torch.is_grad_enabled() else _gradients(ctx, grad)
 
 
-def _check_saved(ctx, grad, x, weight, pre) -> None:
-    """Hooks on saved tensors may hand back others than were saved: other strides are fine, nothing else is."""
-    wanted = [(t, (layout[0], *layout[2:])) for t, layout in zip((x, weight), ctx.layouts)]
-    if pre is not None:
-        wanted.append((pre, (grad.shape, grad.dtype, grad.device)))
-    for t, want in wanted:
-        if (t.shape, t.dtype, t.device) != want:
-            raise RuntimeError(f"a hook on saved tensors returned {tuple(t.shape)}, {t.dtype} on {t.device} "
-                               f"for {tuple(want[0])}, {want[1]} on {want[2]}")
-
-
 def _gradients(ctx, grad):
     x, weight, pre = ctx.saved_tensors
     want_x, want_weight, want_bias, want_residual, _ = ctx.needs_input_grad
     gx = gw = gb = None
     if want_x or want_weight or want_bias:
-        same = (_layout(x), _layout(weight)) == ctx.layouts and (pre is None or _layout(pre) == _layout(grad))
-        if same and ctx.in_place and grad.is_contiguous():
-            with _on_device(x.device):
-                gx, gw, gb = _backward(ctx.facts, grad, x.shape, x, weight, pre, want_x, want_weight, want_bias)
+        # hooks on saved tensors may hand back others than were saved: other strides are fine, nothing else is
+        x_shape, x_stride, w_shape, w_stride, dtype, device = ctx.layout
+        if not (x.shape == x_shape and x.dtype is dtype and x.device == device
+                and weight.shape == w_shape and weight.dtype is dtype and weight.device == device
+                and (pre is None or (pre.shape == grad.shape and pre.dtype is dtype and pre.device == device))):
+            raise RuntimeError("a hook on saved tensors returned a tensor of another shape, type or device than was saved")
+        if (ctx.in_place and x.stride() == x_stride and weight.stride() == w_stride and grad.is_contiguous()
+                and (pre is None or pre.is_contiguous())):
+            with _on_device(device):
+                gx, gw, gb = _backward(ctx.facts, grad, x_shape, x, weight, pre, want_x, want_weight, want_bias)
         else:
-            if not same:
-                _check_saved(ctx, grad, x, weight, pre)
             gx, gw, gb = linear_backward(grad, x, weight, pre, ctx.activation, want_x, want_weight, want_bias)
     return gx, gw, gb, grad if want_residual else None, None
 
