@@ -427,3 +427,27 @@ def test_recomputed_in_the_backward_pass():
         return torch.autograd.grad(out, leaves, torch.ones_like(out))
     want = grads(f(x, r))
     assert all(torch.equal(a, c) for a, c in zip(want, grads(checkpoint(f, x, r, use_reentrant=False))))
+
+
+def test_first_calls_of_a_process_captured():
+    # a process of its own, where nothing of the library has run before the capture
+    import subprocess
+    import sys
+    code = """
+import torch, vq_vae_amd as vq
+x = torch.randn(300, 264, device="cuda").half(); w = torch.randn(136, 264, device="cuda").half()
+g = [torch.randn(5000, device="cuda"), torch.randn(70, device="cuda").half()]
+big = [torch.randn(2048, 1024, device="cuda").bfloat16() for _ in range(2)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, z, n = vq.linear(x, w, None, "silu"), vq.linear(big[0], big[1]), vq.clip_grads(g, 1e9)
+for _ in range(3):
+    y.zero_(); z.zero_(); n.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, vq.linear(x, w, None, "silu")) and torch.equal(z, vq.linear(big[0], big[1])) and torch.equal(n, vq.grad_norm(g))
+print("same")
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]

@@ -69,6 +69,7 @@ typedef u32x4 vql_u32x4_a4 __attribute__((aligned(4), may_alias));
 typedef u32x4 vql_u32x4_a16 __attribute__((may_alias));
 typedef f32x4 vql_f32x4 __attribute__((may_alias));
 #define VQL_LDS __attribute__((address_space(3)))
+#define VQL_GLOBAL __attribute__((address_space(1)))
 typedef uint32_t vql_u32 __attribute__((may_alias));
 typedef uint16_t vql_u16 __attribute__((may_alias));
 template <typename T>
@@ -933,7 +934,8 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void vql_product_kernel(VqLinearAr
         const float s = asum[u] + __shfl_xor(asum[u], 32);
         const int64_t i = iw + u * 32 + (lane & 31);
         if (lane < 32 && i < a.I) {
-          if (a.splits > 1) a.asum[this_split * a.I + i] = s;
+          if (a.splits > 1) ((VQL_GLOBAL float*)a.asum)[this_split * a.I + i] = s;
+          else if constexpr (sizeof(T) == 4) ((VQL_GLOBAL float*)a.gbias)[i] = s;   // the two may become one store: to a global address
           else reinterpret_cast<T*>(a.gbias)[i] = VqElem<T>::from(s);
         }
       }
