@@ -337,6 +337,7 @@ int vq_conv1x1_wgrad(const float* gy, const float* x, int layout, int64_t N, int
  * vq_linear_dgrad:    gx = dp W.
  * vq_linear_wgrad:    gW = dp^T x;  gbias[n] = sum_m dp[m][n].  One of the two may be NULL.
  * vq_linear_backward: the three in one call, of those of gx, gW and gbias that are not NULL (for an empty gx give NULL).
+ *                     gbias is summed there in fp32 from act'(pre) gy before that is rounded to the tensors' type.
  * Sums split over workgroups are added in a fixed order: the same bits on every run.
  * `work`: vq_linear_work_bytes(VQ_LINEAR_*, ...) bytes, 16-byte aligned, contents irrelevant before and after
  * the call; calls that may overlap need one each.

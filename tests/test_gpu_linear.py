@@ -451,3 +451,24 @@ print("same")
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("M, N", [(1, 1), (3, 7), (40, 33), (777, 515), (5000, 64), (4099, 1032), (100, 5000), (70, 9001)])
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+def test_bias_gradient_is_summed_before_rounding(M, N, kind):
+    # gy act'(pre) is rounded to the tensors' type for the products, but not for the bias gradient.  Against the formula at the
+    # pre that the forward pass kept: 32 u (|p| + 1) for the slope, a rounding of the product, the fp32 sum, one rounding at the
+    # end.  Alternating signs make the sum small beside its terms, where rounded terms would show.
+    from vq_vae_amd import projection
+    K = 16
+    x, w, b, _, gy = make(M, K, N, kind, True, False, False, M + N)
+    gy = gy.abs() * (1 - 2 * (torch.arange(M, device=DEV) % 2).to(kind))[:, None]
+    for act in ("silu", "gelu"):
+        _, pre = projection.linear_forward(x, w, b, act, want_pre=True)
+        _, _, gb = projection.linear_backward(gy, x, w, pre, act, False, M % 2 == 1, True)
+        p = pre.double()
+        _, slope = act64(p, act)
+        d = gy.double() * slope
+        each = gy.double().abs() * 32 * U * (p.abs() + 1) + U * d.abs()
+        bound = (each.sum(0) + (M + 1) * U * (d.abs() + each).sum(0)) * 1.001 + HALF[kind] * 1.01 * d.sum(0).abs() + TINY[kind]
+        close(gb, d.sum(0), bound, f"{act}")

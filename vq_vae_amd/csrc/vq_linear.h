@@ -38,7 +38,8 @@ struct VqLinearArgs {
   int act;
   float* part;               // splits > 1: the partial sums, as the product kernel's registers lie
   float* asum;               // weight gradient: the sums of A over r (the bias gradient) of a split sum, [splits][I], or null
-  void* gbias;               // the same in T, where the sum is not split
+  int sum_parts;             // rows of asum, for the join
+  void* gbias;               // the same in T, where the sum is not split, and for the join
 };
 
 // -------------------------------------------------------------------------------- element conversions

@@ -84,6 +84,24 @@ __global__ __launch_bounds__(1024) void vql_rows_kernel(VqLinearArgs a) {
 }
 
 // ------------------------------------------------------------------------------ join of a split sum
+// Sums of `parts` rows of n values, for 64 of them at a time from `first` on: wave k takes the rows k, k + 4, .., then the
+// four sums are added in order.  All 256 threads of a workgroup call it.
+template <typename T>
+__device__ __forceinline__ void join_rows(const float* part, int parts, int64_t n, T* out, int64_t first, int64_t step, float (&s)[4][64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t at = first; at < n; at += step) {
+    const int64_t i = at + lane;
+    float c = 0.0f;
+    if (i < n) {
+#pragma unroll 8
+      for (int k = wave; k < parts; k += 4) c += part[k * n + i];
+    }
+    s[wave][lane] = c;
+    __syncthreads();
+    if (wave == 0 && i < n) out[i] = VqElem<T>::from(((s[0][lane] + s[1][lane]) + s[2][lane]) + s[3][lane]);
+    __syncthreads();
+  }
+}
 // Adds the partial sums and applies the epilogue: a workgroup per 32x32 tile, a lane per 16 values of a row as in the
 // product kernel; wave k adds the splits k, k + 4, .., then the four sums are added in order (the same bits on every run).
 template <typename T>
@@ -91,11 +109,8 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a, int tile,
   __shared__ f32x4 sums[3][4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (a.asum) {   // weight gradient: the bias gradient's partial sums too
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.I; i += (int64_t)gridDim.x * 256) {
-      float c = 0.0f;
-      for (int s = 0; s < a.splits; ++s) c += a.asum[s * a.I + i];
-      reinterpret_cast<T*>(a.gbias)[i] = VqElem<T>::from(c);
-    }
+    __shared__ float rows[4][64];
+    join_rows<T>(a.asum, a.sum_parts, a.I, reinterpret_cast<T*>(a.gbias), (int64_t)blockIdx.x * 64, (int64_t)gridDim.x * 64, rows);
   }
   const int per_block = tile * tile / 1024;                 // 32x32 tiles of a block
   const int64_t block = blockIdx.x / per_block, blocks = a.tiles_i * a.tiles_j;
@@ -126,23 +141,25 @@ __global__ __launch_bounds__(256) void vql_join_kernel(VqLinearArgs a, int tile,
   else vql_write_lane<T, VQL_NORMAL>(a, r, cv, lane >> 5, all);
 }
 template <typename T>
-__global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, int splits, int64_t n, T* out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float c = 0.0f;
-  for (int s = 0; s < splits; ++s) c += part[s * n + i];
-  out[i] = VqElem<T>::from(c);
+__global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, int parts, int64_t n, T* out) {
+  __shared__ float rows[4][64];
+  join_rows<T>(part, parts, n, out, (int64_t)blockIdx.x * 64, n, rows);
 }
 
 // ------------------------------------------------------------------------------ activation's gradient
-// dp = gy * act'(pre), rounded to T: the operand of both products of the backward pass.
+// dp = gy * act'(pre), rounded to T: the operand of both products of the backward pass, whose matrix instructions take T.
+template <typename T>
+__device__ __forceinline__ u32x4 vql_once16(const char* p) {   // for what nobody reads again: dp, which is, stays in the caches
+  if constexpr (sizeof(T) == 4) return __builtin_nontemporal_load(reinterpret_cast<const vql_u32x4_a4*>(p));
+  else return __builtin_nontemporal_load(reinterpret_cast<const vql_u32x4_a2*>(p));
+}
 template <typename T>
 __global__ __launch_bounds__(256) void vql_act_grad_kernel(const T* gy, const T* pre, int act, int64_t count, T* dp) {
   constexpr int E = 16 / sizeof(T);
   const int64_t vecs = count / E, stride = (int64_t)gridDim.x * 256;
   for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < vecs; v += stride) {
-    const VqChunk<T> g = __builtin_bit_cast(VqChunk<T>, vql_load16<T>(reinterpret_cast<const char*>(gy + v * E)));
-    const VqChunk<T> p = __builtin_bit_cast(VqChunk<T>, vql_load16<T>(reinterpret_cast<const char*>(pre + v * E)));
+    const VqChunk<T> g = __builtin_bit_cast(VqChunk<T>, vql_once16<T>(reinterpret_cast<const char*>(gy + v * E)));
+    const VqChunk<T> p = __builtin_bit_cast(VqChunk<T>, vql_once16<T>(reinterpret_cast<const char*>(pre + v * E)));
     VqChunk<T> d;
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -152,6 +169,61 @@ __global__ __launch_bounds__(256) void vql_act_grad_kernel(const T* gy, const T*
   const int64_t at = vecs * E + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at < count)
     dp[at] = VqElem<T>::from(VqElem<T>::to(gy[at]) * vql_act_slope<sizeof(T) == 2>(VqElem<T>::to(pre[at]), act));
+}
+
+// The same with the bias gradient: the sums over the rows, of dp before it is rounded (sums of the rounded values are off by
+// 1.5 to 2.5 times as much).  A thread keeps the columns of one 16-byte piece and takes every so many-th row, two of them in
+// flight; the rows that a workgroup takes at a time are added in LDS at the end.
+constexpr int SUMS_NT = 1024, SUMS_WGS = 256;
+template <typename T>
+__global__ __launch_bounds__(SUMS_NT) void vql_act_grad_sums_kernel(const T* gy, const T* pre, int act, int64_t M, int N, int lanes,
+                                                                   T* dp, float* part) {
+  constexpr int E = 16 / sizeof(T), U = 2;
+  __shared__ float s[SUMS_NT * E];
+  const int rows = SUMS_NT / lanes, row = threadIdx.x / lanes, lane = threadIdx.x - row * lanes;
+  const int64_t col = ((int64_t)blockIdx.x * lanes + lane) * E, valid = N - col;
+  const int64_t stride = (int64_t)gridDim.y * rows;
+  float sum[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = 0.0f;
+  auto one = [&](int64_t m, u32x4 gv, u32x4 pv) {
+    const VqChunk<T> g = __builtin_bit_cast(VqChunk<T>, gv), p = __builtin_bit_cast(VqChunk<T>, pv);
+    VqChunk<T> d;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {   // elements behind the row's end are zero: g is
+      const float v = VqElem<T>::to(g.e[e]) * vql_act_slope<sizeof(T) == 2>(VqElem<T>::to(p.e[e]), act);
+      sum[e] += v;
+      d.e[e] = VqElem<T>::from(v);
+    }
+    vql_store16_part<T>(reinterpret_cast<char*>(dp + m * N + col), __builtin_bit_cast(u32x4, d), valid);
+  };
+  auto load = [&](const T* from, int64_t m) {
+    const char* q = reinterpret_cast<const char*>(from + m * N + col);
+    return valid >= E ? vql_once16<T>(q) : vql_load16_part<T>(q, valid);
+  };
+  if (row < rows && valid > 0) {
+    int64_t m = (int64_t)blockIdx.y * rows + row;
+    for (; m + (U - 1) * stride < M; m += U * stride) {
+      u32x4 g[U], p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) g[u] = load(gy, m + u * stride);
+#pragma unroll
+      for (int u = 0; u < U; ++u) p[u] = load(pre, m + u * stride);
+#pragma unroll
+      for (int u = 0; u < U; ++u) one(m + u * stride, g[u], p[u]);
+    }
+    for (; m < M; m += stride) one(m, load(gy, m), load(pre, m));
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s[threadIdx.x * E + e] = sum[e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < lanes * E; c += SUMS_NT) {
+    const int64_t at = (int64_t)blockIdx.x * lanes * E + c;
+    if (at >= N) continue;
+    float v = 0.0f;
+    for (int r = 0; r < rows; ++r) v += s[r * lanes * E + c];
+    part[blockIdx.y * (int64_t)N + at] = v;
+  }
 }
 
 // ------------------------------------------------------------------------------ column sums
@@ -251,6 +323,20 @@ int64_t colsum_slabs(int64_t M, int N) {
   return std::max<int64_t>(1, std::min<int64_t>((M + 63) / 64, std::max<int64_t>(1, 4 * CUS / groups)));
 }
 
+// how vql_act_grad_sums_kernel cuts its matrix: column groups of `lanes` 16-byte pieces, and `slabs` workgroups for the rows
+// of each, one to a CU in all, so that the sums to be joined stay few
+struct SumsPlan { int groups, lanes, slabs; };
+SumsPlan sums_plan(int64_t M, int N, int dtype) {
+  const int E = (int)(16 / elem_size(dtype)), pieces = (N + E - 1) / E;
+  SumsPlan p;
+  p.groups = (pieces + SUMS_NT / 4 - 1) / (SUMS_NT / 4);
+  p.lanes = (pieces + p.groups - 1) / p.groups;
+  const int64_t rows = SUMS_NT / p.lanes, most = std::max(1, SUMS_WGS / p.groups);
+  p.slabs = (int)std::max<int64_t>(1, std::min<int64_t>(most, (M + rows - 1) / rows));
+  return p;
+}
+int64_t sums_bytes(int64_t M, int N, int dtype) { return ((int64_t)sums_plan(M, N, dtype).slabs * N * 4 + 255) & ~(int64_t)255; }
+
 // the activation's gradient, at the head of the backward pass's workspace
 int64_t dp_bytes(int64_t M, int N, int dtype) { return (M * N * (int64_t)elem_size(dtype) + 255) & ~(int64_t)255; }
 
@@ -292,8 +378,8 @@ template <typename T> struct RunJoin {
   }
 };
 template <typename T> struct RunJoinSums {
-  static int run(const float* part, int splits, int64_t n, void* out, hipStream_t s) {
-    hipLaunchKernelGGL(vql_join_sums_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, splits, n,
+  static int run(const float* part, int parts, int64_t n, void* out, hipStream_t s) {
+    hipLaunchKernelGGL(vql_join_sums_kernel<T>, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, s, part, parts, n,
                        reinterpret_cast<T*>(out));
     return vq_hip_status(hipGetLastError());
   }
@@ -303,6 +389,14 @@ template <typename T> struct RunActGrad {
     const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((count / (16 / sizeof(T)) + 255) / 256, 16384));
     hipLaunchKernelGGL(vql_act_grad_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, reinterpret_cast<const T*>(gy),
                        reinterpret_cast<const T*>(pre), act, count, reinterpret_cast<T*>(dp));
+    return vq_hip_status(hipGetLastError());
+  }
+};
+template <typename T> struct RunActGradSums {
+  static int run(const void* gy, const void* pre, int act, int64_t M, int N, const SumsPlan& p, void* dp, float* part, hipStream_t s) {
+    hipLaunchKernelGGL(vql_act_grad_sums_kernel<T>, dim3((unsigned)p.groups, (unsigned)p.slabs), dim3(SUMS_NT), 0, s,
+                       reinterpret_cast<const T*>(gy), reinterpret_cast<const T*>(pre), act, M, N, p.lanes,
+                       reinterpret_cast<T*>(dp), part);
     return vq_hip_status(hipGetLastError());
   }
 };
@@ -317,8 +411,9 @@ template <typename T> struct RunColsum {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Runs one of the three products with its epilogue; `gbias` (weight gradient) receives the sums of A.
-int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, void* work, hipStream_t s) {
+// Runs one of the three products with its epilogue; `gbias` (weight gradient) receives the sums of A, or of the `sum_parts`
+// rows of `sums` where the caller has those.
+int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, const float* sums, int sum_parts, void* work, hipStream_t s) {
   const int64_t es = (int64_t)elem_size(dtype);
   const int E = (int)(16 / es);
   bool dma = aligned16(a.A) && aligned16(a.B) && a.lda % 16 == 0 && a.ldb % 16 == 0;
@@ -336,11 +431,20 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, void* work, 
   }
   if (p.rows) return by_type<RunRows>(dtype, a, s);
   if (p.tiles_i * p.tiles_j * p.splits >= (int64_t)1 << 23) return VQ_ERR_UNSUPPORTED;
-  a.gbias = gbias;
-  if (gbias && p.splits > 1) a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p));
+  if (!sums) a.gbias = gbias;
+  if (gbias && !sums && p.splits > 1) a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p));
   int rc = product(a, layout, dtype, p.config, dma, s);
-  if (rc == VQ_OK && a.splits > 1) rc = by_type<RunJoin>(dtype, a, p.config, s);
-  return rc;
+  if (rc != VQ_OK) return rc;
+  if (p.splits > 1) {
+    a.gbias = gbias;
+    a.sum_parts = p.splits;
+    if (gbias && sums) {
+      a.asum = const_cast<float*>(sums);
+      a.sum_parts = sum_parts;
+    }
+    return by_type<RunJoin>(dtype, a, p.config, s);
+  }
+  return gbias && sums ? by_type<RunJoinSums>(dtype, sums, sum_parts, a.I, gbias, s) : VQ_OK;
 }
 
 int64_t product_work(int layout, int64_t I, int J, int64_t R, int dtype, bool sums) {
@@ -358,7 +462,7 @@ extern "C" int64_t vq_linear_work_bytes(int pass, int64_t M, int K, int N, int d
   if (bad_sizes(M, K, N) || K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || !known(dtype)) return 0;
   if (pass < VQ_LINEAR_FORWARD || pass > VQ_LINEAR_BACKWARD) return 0;
   if (pass == VQ_LINEAR_BACKWARD)
-    return dp_bytes(M, N, dtype) + std::max(vq_linear_work_bytes(VQ_LINEAR_DGRAD, M, K, N, dtype),
+    return dp_bytes(M, N, dtype) + sums_bytes(M, N, dtype) + std::max(vq_linear_work_bytes(VQ_LINEAR_DGRAD, M, K, N, dtype),
                                             vq_linear_work_bytes(VQ_LINEAR_WGRAD, M, K, N, dtype));
   if (pass == VQ_LINEAR_FORWARD) return product_work(0, M, N, K, dtype, false);
   if (pass == VQ_LINEAR_DGRAD) return product_work(1, M, K, N, dtype, false);
@@ -390,7 +494,7 @@ extern "C" int vq_linear(const void* x, int64_t ldx, const void* W, int64_t ldw,
   a.res = reinterpret_cast<const char*>(residual);
   a.ldr = ldr * es;
   a.act = act;
-  return run_product(0, a, dtype, nullptr, work, reinterpret_cast<hipStream_t>(stream));
+  return run_product(0, a, dtype, nullptr, nullptr, 0, work, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int vq_linear_act_grad(const void* gy, const void* pre, int dtype, int act, int64_t count, void* dp, void* stream) {
@@ -416,17 +520,20 @@ extern "C" int vq_linear_dgrad(const void* dp, const void* W, int64_t ldw, int d
   a.J = K;
   a.R = N;
   a.out = gx;
-  return run_product(1, a, dtype, nullptr, work, reinterpret_cast<hipStream_t>(stream));
+  return run_product(1, a, dtype, nullptr, nullptr, 0, work, reinterpret_cast<hipStream_t>(stream));
 }
 
-extern "C" int vq_linear_wgrad(const void* dp, const void* x, int64_t ldx, int dtype, int64_t M, int K, int N, void* gW,
-                               void* gbias, void* work, void* stream) {
+namespace {
+// sums: `parts` rows whose sum is the bias gradient, or null: it is the column sums of dp then
+int weight_gradients(const void* dp, const void* x, int64_t ldx, int dtype, int64_t M, int K, int N, void* gW, void* gbias,
+                     const float* sums, int parts, void* work, void* stream) {
   if (bad_sizes(M, K, N) || !known(dtype) || ldx < K || (!gW && !gbias)) return VQ_ERR_INVALID_ARG;
   if (M > 0 && (!dp || (gW && !x))) return VQ_ERR_INVALID_ARG;
   const size_t es = elem_size(dtype);
   if (K > MAX_DIM || N > MAX_DIM || M > MAX_ROWS || pitch_too_wide(N, es) || pitch_too_wide(ldx, es)) return VQ_ERR_UNSUPPORTED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!gW) {
+    if (sums) return by_type<RunJoinSums>(dtype, sums, parts, (int64_t)N, gbias, s);
     if (!work) return VQ_ERR_INVALID_ARG;
     const int64_t slabs = colsum_slabs(M, N);
     float* part = reinterpret_cast<float*>(work);
@@ -442,7 +549,13 @@ extern "C" int vq_linear_wgrad(const void* dp, const void* x, int64_t ldx, int d
   a.J = K;
   a.R = M;
   a.out = gW;
-  return run_product(2, a, dtype, gbias, work, s);
+  return run_product(2, a, dtype, gbias, sums, parts, work, s);
+}
+}  // namespace
+
+extern "C" int vq_linear_wgrad(const void* dp, const void* x, int64_t ldx, int dtype, int64_t M, int K, int N, void* gW,
+                               void* gbias, void* work, void* stream) {
+  return weight_gradients(dp, x, ldx, dtype, M, K, N, gW, gbias, nullptr, 0, work, stream);
 }
 
 extern "C" int vq_linear_backward(const void* gy, const void* pre, const void* x, int64_t ldx, const void* W, int64_t ldw,
@@ -458,16 +571,28 @@ extern "C" int vq_linear_backward(const void* gy, const void* pre, const void* x
       (gW && pitch_too_wide(ldx, es)))
     return VQ_ERR_UNSUPPORTED;
   const void* dp = gy;
+  const float* sums = nullptr;
+  int parts = 0;
   if (act != VQ_ACT_NONE && M > 0) {
-    const int rc = vq_linear_act_grad(gy, pre, dtype, act, M * N, work, stream);
+    char* const after = reinterpret_cast<char*>(work) + dp_bytes(M, N, dtype);
+    int rc;
+    if (gbias) {
+      const SumsPlan p = sums_plan(M, N, dtype);
+      sums = reinterpret_cast<const float*>(after);
+      parts = p.slabs;
+      rc = by_type<RunActGradSums>(dtype, gy, pre, act, M, N, p, work, reinterpret_cast<float*>(after),
+                                   reinterpret_cast<hipStream_t>(stream));
+    } else {
+      rc = vq_linear_act_grad(gy, pre, dtype, act, M * N, work, stream);
+    }
     if (rc != VQ_OK) return rc;
     dp = work;
-    work = reinterpret_cast<char*>(work) + dp_bytes(M, N, dtype);
+    work = after + sums_bytes(M, N, dtype);
   }
   if (gx) {
     const int rc = vq_linear_dgrad(dp, W, ldw, dtype, M, K, N, gx, work, stream);
     if (rc != VQ_OK) return rc;
   }
-  if (gW || gbias) return vq_linear_wgrad(dp, x, ldx, dtype, M, K, N, gW, gbias, work, stream);
+  if (gW || gbias) return weight_gradients(dp, x, ldx, dtype, M, K, N, gW, gbias, sums, parts, work, stream);
   return VQ_OK;
 }

@@ -192,7 +192,8 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     every run.
 
     Differentiable once in all four tensors.  For an activation the forward keeps ``input @ weight.T + bias`` in the
-    tensors' type, and the backward rounds the gradient behind the activation to it before the two products.
+    tensors' type, and the backward rounds the gradient behind the activation to it before the two products (the bias
+    gradient is summed before that rounding).
     Under autocast the tensors keep their types.  May be captured in a graph, backward included (drop every eager autograd
     graph over the same leaves before capturing, as torch asks for any backward under capture)."""
     _check(input, weight, bias, activation, residual)
