@@ -79,14 +79,16 @@ __device__ __forceinline__ double norm_merge(double a, double b, int kind) {
   return (b > a || b != b) ? b : a;
 }
 
-template <typename T>
+// ONCE: nobody reads the gradients again, so they pass the caches by (792 MB fp32 141 -> 126 us, 66 MB 16.8 -> 15.2); where they
+// are clipped next they stay (360 us instead of 387).
+template <typename T, bool ONCE>
 __device__ __forceinline__ void norm_chunk(const char* src, int64_t at, int64_t count, int kind, double (&acc)[2]) {
   constexpr int E = 16 / sizeof(T), U = G_CHUNK / 16 / 256;
   const char* p = src + at * (int64_t)sizeof(T);
   if (count == G_CHUNK / (int64_t)sizeof(T)) {
     u32x4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = vql_load16<T>(p + (u * 256 + threadIdx.x) * 16);
+    for (int u = 0; u < U; ++u) v[u] = ONCE ? vql_once16<T>(p + (u * 256 + threadIdx.x) * 16) : vql_load16<T>(p + (u * 256 + threadIdx.x) * 16);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const VqChunk<T> c = __builtin_bit_cast(VqChunk<T>, v[u]);
@@ -113,15 +115,15 @@ __device__ __forceinline__ double block_merge(double v, int kind, double* s) {
   return v;
 }
 
-template <int KIND>
+template <int KIND, bool ONCE>
 __global__ __launch_bounds__(256) void vqg_partial_kernel(GradTable t, double* part) {
   __shared__ double s[4];
   double acc[2] = {0.0, 0.0};
   for_chunks<false>(t, [&](int i, int64_t at, int64_t count) {
     const int type = t.type[i] & 15;
-    if (type == VQ_F32) norm_chunk<float>(t.src[i], at, count, KIND, acc);
-    else if (type == VQ_BF16) norm_chunk<VqBf16>(t.src[i], at, count, KIND, acc);
-    else norm_chunk<_Float16>(t.src[i], at, count, KIND, acc);
+    if (type == VQ_F32) norm_chunk<float, ONCE>(t.src[i], at, count, KIND, acc);
+    else if (type == VQ_BF16) norm_chunk<VqBf16, ONCE>(t.src[i], at, count, KIND, acc);
+    else norm_chunk<_Float16, ONCE>(t.src[i], at, count, KIND, acc);
   });
   const double v = block_merge(norm_merge(acc[0], acc[1], KIND), KIND, s);
   if (threadIdx.x == 0) part[blockIdx.x] = v;
@@ -141,36 +143,48 @@ __global__ __launch_bounds__(256) void vqg_finish_kernel(const double* part, int
   if (threadIdx.x == 0) *norm = (float)v;
 }
 
+// Loads and stores past the caches: the gradients of the norm pass stay there, to be found by this one, instead of making room
+// for results (528 MB bf16 into fp32 422 -> 360 us, 264 MB fp32 into fp32 163 -> 129, 33 MB in place 22.8 -> 22.6; with somebody
+// who reads the result next 605 -> 539, 210 -> 181, 30.2 -> 30.4).  One access is 16 bytes of the result a lane, so that a wave
+// fills whole lines also where 16-bit gradients become fp32 (two stores of 16 bytes at 32-byte distance made it 650).
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 vqg_u32x2_a2 __attribute__((aligned(2), may_alias));
+template <typename S, int W>
+struct alignas(sizeof(S)) VqRun {
+  S e[W];
+};
+template <typename S, int W>
+__device__ __forceinline__ VqRun<S, W> load_run(const char* p) {
+  if constexpr (W * sizeof(S) == 8) return __builtin_bit_cast(VqRun<S, W>, (u32x2)__builtin_nontemporal_load(reinterpret_cast<const vqg_u32x2_a2*>(p)));
+  else return __builtin_bit_cast(VqRun<S, W>, vql_once16<S>(p));
+}
 template <typename S, typename D>
 __device__ __forceinline__ void scale_chunk(const char* src, char* dst, int64_t at, int64_t count, float c) {
-  constexpr int E = 16 / sizeof(S), U = G_CHUNK / 16 / 256;
+  constexpr int W = 16 / sizeof(D), U = G_CHUNK / (W * sizeof(S)) / 256;
   const char* p = src + at * (int64_t)sizeof(S);
   D* q = reinterpret_cast<D*>(dst) + at;
-  auto one = [&](u32x4 w, int64_t first, int64_t n) {
-    const VqChunk<S> g = __builtin_bit_cast(VqChunk<S>, w);
-    if (n >= E) {
+  auto one = [&](const VqRun<S, W>& g, int64_t first) {
+    VqChunk<D> o;
 #pragma unroll
-      for (int h = 0; h < (int)(sizeof(D) / sizeof(S)); ++h) {   // 16-bit gradients into fp32: two stores
-        constexpr int ED = 16 / sizeof(D);
-        VqChunk<D> o;
-#pragma unroll
-        for (int e = 0; e < ED; ++e) o.e[e] = VqElem<D>::from(VqElem<S>::to(g.e[h * ED + e]) * c);
-        vql_store16<D>(q + first + h * ED, __builtin_bit_cast(u32x4, o));
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E - 1; ++e)
-        if (e < n) q[first + e] = VqElem<D>::from(VqElem<S>::to(g.e[e]) * c);
-    }
+    for (int e = 0; e < W; ++e) o.e[e] = VqElem<D>::from(VqElem<S>::to(g.e[e]) * c);
+    const u32x4 w = __builtin_bit_cast(u32x4, o);
+    if constexpr (sizeof(D) == 4) __builtin_nontemporal_store(w, reinterpret_cast<vql_u32x4_a4*>(q + first));
+    else __builtin_nontemporal_store(w, reinterpret_cast<vql_u32x4_a2*>(q + first));
   };
   if (count == G_CHUNK / (int64_t)sizeof(S)) {
-    u32x4 v[U];
+    VqRun<S, W> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = vql_load16<S>(p + (u * 256 + threadIdx.x) * 16);
+    for (int u = 0; u < U; ++u) v[u] = load_run<S, W>(p + (u * 256 + threadIdx.x) * (int)(W * sizeof(S)));
 #pragma unroll
-    for (int u = 0; u < U; ++u) one(v[u], (int64_t)(u * 256 + threadIdx.x) * E, E);
+    for (int u = 0; u < U; ++u) one(v[u], (int64_t)(u * 256 + threadIdx.x) * W);
   } else {
-    for (int64_t v = threadIdx.x; v * E < count; v += 256) one(vql_load16_part<S>(p + v * 16, count - v * E), v * E, count - v * E);
+    for (int64_t v = threadIdx.x; v * W < count; v += 256) {
+      if (count - v * W >= W) {
+        one(load_run<S, W>(p + v * (int64_t)(W * sizeof(S))), v * W);
+      } else {
+        for (int64_t i = v * W; i < count; ++i) q[i] = VqElem<D>::from(VqElem<S>::to(reinterpret_cast<const S*>(p)[i]) * c);
+      }
+    }
   }
 }
 
@@ -247,13 +261,18 @@ int for_tables(const vq_tensor_ref* refs, int n, bool scale, int64_t chunks, F f
   return VQ_OK;
 }
 
-int run_partials(const vq_tensor_ref* refs, int n, int kind, int64_t chunks, double* part, int* n_part, hipStream_t s) {
+template <int KIND>
+void launch_partials(const GradTable& t, bool once, double* at, hipStream_t s) {
+  if (once) hipLaunchKernelGGL((vqg_partial_kernel<KIND, true>), dim3(t.wgs), dim3(256), 0, s, t, at);
+  else hipLaunchKernelGGL((vqg_partial_kernel<KIND, false>), dim3(t.wgs), dim3(256), 0, s, t, at);
+}
+int run_partials(const vq_tensor_ref* refs, int n, int kind, bool once, int64_t chunks, double* part, int* n_part, hipStream_t s) {
   *n_part = 0;
   return for_tables(refs, n, false, chunks, [&](const GradTable& t) {
     double* at = part + *n_part;
-    if (kind == VQ_NORM_2) hipLaunchKernelGGL(vqg_partial_kernel<VQ_NORM_2>, dim3(t.wgs), dim3(256), 0, s, t, at);
-    else if (kind == VQ_NORM_1) hipLaunchKernelGGL(vqg_partial_kernel<VQ_NORM_1>, dim3(t.wgs), dim3(256), 0, s, t, at);
-    else hipLaunchKernelGGL(vqg_partial_kernel<VQ_NORM_INF>, dim3(t.wgs), dim3(256), 0, s, t, at);
+    if (kind == VQ_NORM_2) launch_partials<VQ_NORM_2>(t, once, at, s);
+    else if (kind == VQ_NORM_1) launch_partials<VQ_NORM_1>(t, once, at, s);
+    else launch_partials<VQ_NORM_INF>(t, once, at, s);
     *n_part += t.wgs;
     return vq_hip_status(hipGetLastError());
   });
@@ -292,7 +311,7 @@ extern "C" int vq_grad_norm(const vq_tensor_ref* refs, int n, int kind, float* n
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* part = reinterpret_cast<double*>(work);
   int n_part = 0;
-  const int rc = run_partials(refs, n, kind, chunks, part, &n_part, s);
+  const int rc = run_partials(refs, n, kind, true, chunks, part, &n_part, s);
   if (rc != VQ_OK) return rc;
   hipLaunchKernelGGL(vqg_finish_kernel, dim3(1), dim3(256), 0, s, part, n_part, kind, norm);
   return vq_hip_status(hipGetLastError());
@@ -308,7 +327,7 @@ extern "C" int vq_clip_grads(const vq_tensor_ref* refs, int n, int kind, float m
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* part = reinterpret_cast<double*>(work);
   int n_part = 0;
-  int rc = run_partials(refs, n, kind, chunks, part, &n_part, s);
+  int rc = run_partials(refs, n, kind, false, chunks, part, &n_part, s);
   if (rc != VQ_OK) return rc;
   if (n_part == 0) {   // no elements: the norm is zero
     hipLaunchKernelGGL(vqg_finish_kernel, dim3(1), dim3(256), 0, s, part, 0, kind, norm);

@@ -79,6 +79,11 @@ __device__ __forceinline__ u32x4 vql_load16(const char* p) {
   else return *reinterpret_cast<const vql_u32x4_a2*>(p);
 }
 template <typename T>
+__device__ __forceinline__ u32x4 vql_once16(const char* p) {   // of what is not read again: past the caches
+  if constexpr (sizeof(T) == 4) return __builtin_nontemporal_load(reinterpret_cast<const vql_u32x4_a4*>(p));
+  else return __builtin_nontemporal_load(reinterpret_cast<const vql_u32x4_a2*>(p));
+}
+template <typename T>
 __device__ __forceinline__ void vql_store16(void* p, u32x4 v) {
   if constexpr (sizeof(T) == 4) *reinterpret_cast<vql_u32x4_a4*>(p) = v;
   else *reinterpret_cast<vql_u32x4_a2*>(p) = v;

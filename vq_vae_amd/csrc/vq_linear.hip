@@ -148,11 +148,8 @@ __global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, i
 
 // ------------------------------------------------------------------------------ activation's gradient
 // dp = gy * act'(pre), rounded to T: the operand of both products of the backward pass, whose matrix instructions take T.
-template <typename T>
-__device__ __forceinline__ u32x4 vql_once16(const char* p) {   // for what nobody reads again: dp, which is, stays in the caches
-  if constexpr (sizeof(T) == 4) return __builtin_nontemporal_load(reinterpret_cast<const vql_u32x4_a4*>(p));
-  else return __builtin_nontemporal_load(reinterpret_cast<const vql_u32x4_a2*>(p));
-}
+// What is read passes the caches by, so that dp, which is read next, stays there (64 Ki x 1024 bf16 and the weight gradient
+// behind it 132 -> 121 us).
 template <typename T>
 __global__ __launch_bounds__(256) void vql_act_grad_kernel(const T* gy, const T* pre, int act, int64_t count, T* dp) {
   constexpr int E = 16 / sizeof(T);
