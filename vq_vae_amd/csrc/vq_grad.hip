@@ -14,6 +14,8 @@
 //     what 32 bits hold, and the stream leaves the time (v_fma_f64 runs at half the fp32 rate).
 //   * Every workgroup writes one partial sum; the readers add them all in a fixed order.  No atomics, no counter that
 //     would have to be cleared, the same bits on every run.
+// 792 MB of fp32 gradients: norm 126 us, 6.3 TB/s; 528 MB bf16 clipped into 1056 MB fp32: 360 us, 5.9 TB/s of the 2.1 GB.
+// Chunks dealt out in turn instead of in runs: norm 123, clipping 370.
 #include <algorithm>
 #include <new>
 

@@ -771,6 +771,9 @@ namespace {   // the kernels of a translation unit are its own
 // A workgroup of WI x WJ waves owns a BI x BJ block of C (and, with splits, a range of the sum); a wave owns
 // (BI / WI) x (BJ / WJ) of it in 32x32 accumulator tiles.  DMA: rows start on 16 bytes, so that the tiles go straight into
 // LDS; otherwise they go through registers.
+// What bounds it (operands out of the caches): 8192 x 4096 -> 4096 bf16 with residual 242 us, 1.14 PFLOP/s, the matrix cores at the
+// clock they hold; 64 Ki x 256 -> 1024 bf16 54 us, 3.1 TB/s, with gelu_tanh 63: products, stores and the activation one
+// after the other in part; 16384 x 2048 -> 1024 fp32 480 us, 143 TFLOP/s, the matrix cores.
 template <typename T, bool AMM, bool BMM, int KIND, int BI, int BJ, int WI, int WJ, int NS, bool DMA>
 __global__ __launch_bounds__(WI * WJ * 64, 2) void vql_product_kernel(VqLinearArgs a) {
   constexpr int NT = WI * WJ * 64;
