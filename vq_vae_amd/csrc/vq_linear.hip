@@ -269,13 +269,14 @@ struct Cost {
 const Cost COST[VQL_CONFIGS] = {
     {64, 3, {{{{0.90f, 1.17f, 1.38f}, 4.2f}, {{1.17f, 1.65f, 2.05f}, 6.0f}},
              {{{0.32f, 0.45f, 0.60f}, 4.4f}, {{0.65f, 1.07f, 1.45f}, 6.5f}}}},
-    {128, 2, {{{{1.70f, 2.05f}, 8.0f}, {{2.95f, 4.60f}, 12.0f}}, {{{0.75f, 0.95f}, 6.5f}, {{2.00f, 3.72f}, 13.5f}}}},
+    {128, 2, {{{{1.70f, 2.05f}, 8.0f}, {{2.95f, 4.60f}, 12.0f}}, {{{0.72f, 0.95f}, 6.5f}, {{1.97f, 3.69f}, 13.5f}}}},
     {256, 1, {{}, {{{1.55f}, 12.5f}, {{7.15f}, 27.0f}}}},
 };
 // The cheapest tile with its best split of the sum: rounds of workgroups x (steps x time of a step + once), the last round
 // with as many on a CU as are left, and the join of a split sum (a launch, the partial sums written and read at 6.5 TB/s:
 // they stay in the last-level cache).  Over 36 random products of 17 to 65536 rows and 64 to 4096 channels, every layout, the
-// choice took 1.01 times as long on average as the best of all tiles and of 1, 2, 4 .. 32 splits, 1.14 times at worst.
+// choice took 1.03 times as long on average as the best of all tiles and of 1, 2, 4 .. 32 splits, 1.19 times at worst (5.1 us instead of
+// 4.3), 1.15 among those over 10 us.
 Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
   const size_t es = elem_size(dtype);
   Plan best{};
