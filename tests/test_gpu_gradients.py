@@ -243,3 +243,23 @@ def test_a_training_step():
     for p, g in zip(params, grads):
         g = g * min(1.0, 0.05 / (n + 1e-6))
         assert float((p.grad.double() - g).abs().max()) <= 2e-5 * float(g.abs().max())
+
+
+@pytest.mark.parametrize("src, dst", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                      (torch.float32, torch.float32)], ids=["bf16-f32", "f16-f32", "bf16", "f32"])
+def test_results_between_others(src, dst):
+    # results in the middle of a buffer, at every element offset within 16 bytes, around the sizes of a chunk and of an access
+    sizes = [1, 2, 3, 4, 5, 7, 8, 9, 255, 8191, 8192, 8193, 16383, 16384, 16385, 16387, 40003]
+    for shift in range(8):
+        grads = [torch.randn(n + shift, device=DEV)[shift:].to(src) for n in sizes]
+        bufs = [torch.full((n + 64,), 7.0, device=DEV, dtype=dst) for n in sizes]
+        outs = [b[16 + shift:16 + shift + n] for b, n in zip(bufs, sizes)]
+        norm = vq.clip_grads(grads, 3.0, out=outs)
+        want = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+        assert abs(float(norm) - want) <= 2.0 ** -23 * want
+        c = min(1.0, 3.0 / (want + 1e-6))
+        for b, o, g, n in zip(bufs, outs, grads, sizes):
+            assert bool((b[:16 + shift] == 7).all()) and bool((b[16 + shift + n:] == 7).all())
+            h = torch.finfo(dst).eps / 2
+            # c in fp32 and a rounding of the product; one of the result
+            assert bool(((o.double() - g.double() * c).abs() <= (2.0 ** -22 + 1.01 * h) * g.double().abs() * c + 1e-37).all())

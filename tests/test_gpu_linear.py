@@ -472,3 +472,27 @@ def test_bias_gradient_is_summed_before_rounding(M, N, kind):
         each = gy.double().abs() * 32 * U * (p.abs() + 1) + U * d.abs()
         bound = (each.sum(0) + (M + 1) * U * (d.abs() + each).sum(0)) * 1.001 + HALF[kind] * 1.01 * d.sum(0).abs() + TINY[kind]
         close(gb, d.sum(0), bound, f"{act}")
+
+
+@pytest.mark.parametrize("M, K, N", [(1, 1, 1), (3, 40, 50), (70, 33, 2500), (777, 130, 515), (300, 256, 520), (40, 16, 9001)])
+@pytest.mark.parametrize("kind, dt", [(torch.float32, 0), (torch.bfloat16, 1)], ids=["f32", "bf16"])
+def test_backward_stays_within_its_outputs_and_workspace(M, K, N, kind, dt):
+    lib = _lib.load()
+    x, w, _, _, gy = make(M, K, N, kind, False, False, False, 2)
+    pre = torch.nn.functional.linear(x.float(), w.float()).to(kind)
+    bytes_of = lambda n: n * kind.itemsize
+
+    def band(n):       # 256 bytes on either side
+        buf = torch.full((n + 512,), 0x5a, device=DEV, dtype=torch.uint8)
+        return buf, buf.data_ptr() + 256
+    n_work = lib.vq_linear_work_bytes(3, M, K, N, dt)
+    bands = [band(n) for n in (bytes_of(M * K), bytes_of(N * K), bytes_of(N), n_work)]
+    P = ops._ptr
+    assert lib.vq_linear_backward(P(gy), P(pre), P(x), K, P(w), K, dt, 2, M, K, N, *(p for _, p in bands), ops._stream(DEV)) == 0
+    torch.cuda.synchronize()
+    for buf, _ in bands:
+        assert bool((buf[:256] == 0x5a).all()) and bool((buf[-256:] == 0x5a).all())
+    p, (_, slope) = pre.double(), act64(pre.double(), "silu")
+    (gx, ex), (gw, ew), (gb, eb) = backward64(gy, x, w, p, torch.zeros_like(p), slope, "silu")
+    for (buf, _), want, bound, what in zip(bands, (gx, gw, gb), (ex, ew, eb), ("input", "weight", "bias")):
+        close(buf[256:-256].view(kind).view(want.shape), want, bound, what)
