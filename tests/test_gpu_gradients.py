@@ -263,3 +263,14 @@ def test_results_between_others(src, dst):
             h = torch.finfo(dst).eps / 2
             # c in fp32 and a rounding of the product; one of the result
             assert bool(((o.double() - g.double() * c).abs() <= (2.0 ** -22 + 1.01 * h) * g.double().abs() * c + 1e-37).all())
+
+
+def test_inference_tensors():
+    with torch.inference_mode():
+        g = [torch.full((5,), 3.0, device=DEV), torch.full((7, 3), 4.0, device=DEV).t()]
+        norm = vq.clip_grads(g, 1.0)
+    for _ in range(2):      # outside too
+        want = math.sqrt(45 + 21 * 16)
+        assert abs(float(norm) - want) <= 2.0 ** -22 * want
+        assert abs(float(vq.grad_norm(g)) - 1.0) <= 1e-5
+        norm = vq.clip_grads([g[0] * want, g[1] * want], 1e9)

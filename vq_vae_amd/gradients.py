@@ -17,6 +17,9 @@ from ._lib import NORM_1, NORM_2, NORM_INF, check
 from .projection import DTYPES
 from .ops import _on_device, _raw_stream, _require_cuda
 
+#: source and result type of a tensor scaled in place, as one word of the C interface's entry
+_TWICE = {dtype: code | code << 32 for dtype, code in DTYPES.items()}
+
 _KINDS = {1.0: NORM_1, 2.0: NORM_2, math.inf: NORM_INF}
 
 
@@ -68,8 +71,13 @@ def _dense(t: torch.Tensor) -> bool:
 def _refs(srcs: Sequence[torch.Tensor], dsts: Sequence[torch.Tensor]) -> array.array:
     """The vq_tensor_ref array of the C interface: four 64-bit words an entry."""
     words: List[int] = []
-    for s, d in zip(srcs, dsts):
-        words += (s.data_ptr(), d.data_ptr(), s.numel(), DTYPES[s.dtype] | DTYPES[d.dtype] << 32)
+    if srcs is dsts:
+        for s in srcs:
+            at = s.data_ptr()
+            words += (at, at, s.numel(), _TWICE[s.dtype])
+    else:
+        for s, d in zip(srcs, dsts):
+            words += (s.data_ptr(), d.data_ptr(), s.numel(), DTYPES[s.dtype] | DTYPES[d.dtype] << 32)
     return array.array("q", words)
 
 
@@ -79,7 +87,7 @@ def _spans(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]) -> ar
     words: List[int] = []
     for t in (*written, *(g for g, o in zip(grads, written) if g is not o)):
         span = t.numel() and 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-        words += (t.data_ptr(), t.data_ptr(), span, DTYPES[t.dtype] * ((1 << 32) + 1))
+        words += (t.data_ptr(), t.data_ptr(), span, _TWICE[t.dtype])
     return array.array("q", words)
 
 
@@ -102,7 +110,7 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
     lib = _lib.load()
     device = grads[0].device
     with _on_device(device):
-        flat = [t if _dense(t) else t.contiguous() for t in grads]
+        flat = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in grads]
         norm = torch.empty((), dtype=torch.float32, device=device)
         work = torch.empty(lib.vq_grad_norm_work_bytes(len(flat)), dtype=torch.uint8, device=device)
         refs = _refs(flat, flat)
@@ -166,7 +174,7 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
             with torch.no_grad():
                 for o, c in back:
                     o.copy_(c)
-        torch.autograd.graph.increment_version([t for t in dsts if not t.is_inference()])
+        torch.autograd.graph.increment_version(dsts)
     return norm
 
 

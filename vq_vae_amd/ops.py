@@ -31,7 +31,7 @@ _HERE = nullcontext()
 
 def _on_device(device):
     """Makes `device` the current one for a launch; nothing where it is already."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _raw_stream(device) -> int:

@@ -22,6 +22,8 @@ DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _li
 #: the widest distance between two rows that the kernels address (bytes)
 _MAX_PITCH = 0x7fffffff // 256 - 128
 
+_MAX_FEATURES = 1 << 20
+
 
 @functools.lru_cache(maxsize=4096)
 def _work_bytes(which: int, M: int, K: int, N: int, dtype: int) -> int:
@@ -38,22 +40,30 @@ def _address(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
-    """t as a (rows, width) matrix whose rows are dense, at any distance from each other; copied only if it is not one."""
+def _matrix(t: torch.Tensor, width: int):
+    """t as rows of ``width`` elements, dense each and at any distance from each other: ``(a tensor that starts where they do, how
+    many, elements between them)``; copied only if it is not such."""
+    if t.is_contiguous():
+        return t, t.numel() // width, width
     t = t if t.dim() == 2 else t.reshape(-1, width)
-    if t.stride(1) == 1 or width == 1:
-        pitch = t.stride(0)
-        if t.shape[0] <= 1 or width <= pitch <= _MAX_PITCH // t.element_size():
-            return t
-    return t.contiguous()
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Elements between the rows of what ``_rows`` returned (the width where there is only one row)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, pitch = t.shape[0], t.stride(0)
+    if (t.stride(1) == 1 or width == 1) and (rows <= 1 or width <= pitch <= _MAX_PITCH // t.element_size()):
+        return t, rows, pitch if rows > 1 else width
+    return t.contiguous(), rows, width
 
 
 def _check(x, weight, bias, activation, residual) -> None:
+    # what nearly every call passes in a third of the time of the tests below, which say what is wrong with the others
+    if (isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and x.is_cuda and activation in ACTIVATIONS
+            and weight.dim() == 2 and x.dim() > 0):
+        dtype, device, (N, K), shape = x.dtype, x.get_device(), weight.shape, x.shape
+        if (dtype in DTYPES and weight.dtype is dtype and weight.get_device() == device and shape[-1] == K and 0 < K <= _MAX_FEATURES
+                and 0 < N <= _MAX_FEATURES
+                and (bias is None or (isinstance(bias, torch.Tensor) and bias.dtype is dtype and bias.get_device() == device
+                                      and bias.shape == (N,)))
+                and (residual is None or (isinstance(residual, torch.Tensor) and residual.dtype is dtype
+                                          and residual.get_device() == device and residual.shape == (*shape[:-1], N)))):
+            return
     for t, name, optional in ((x, "input", False), (weight, "weight", False), (bias, "bias", True), (residual, "residual", True)):
         if t is None and optional:
             continue
@@ -70,8 +80,8 @@ def _check(x, weight, bias, activation, residual) -> None:
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight must be (out features, in features), both at least 1, got {tuple(weight.shape)}")
     N, K = weight.shape
-    if max(N, K) > 1 << 20:
-        raise ValueError(f"linear takes up to {1 << 20} features, got {tuple(weight.shape)}")
+    if max(N, K) > _MAX_FEATURES:
+        raise ValueError(f"linear takes up to {_MAX_FEATURES} features, got {tuple(weight.shape)}")
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"input {tuple(x.shape)} does not end in the weight's {K} in features")
     if bias is not None and bias.shape != (N,):
@@ -84,25 +94,25 @@ def _check(x, weight, bias, activation, residual) -> None:
 def linear_forward(x, weight, bias=None, activation: str = "none", residual=None, want_pre: bool = False):
     """``(y, pre)``: ``pre = x W^T + bias`` (None unless wanted) and ``y = act(pre) + residual``, without autograd.
     Arguments as :func:`linear`, already checked."""
-    with _on_device(x.device):
+    device = x.device
+    with _on_device(device):
         K = weight.shape[1]
-        return _forward(_rows(x, K), _rows(weight, K), x.shape[:-1], bias, activation, residual, want_pre)
+        return _forward(_matrix(x, K), _matrix(weight, K), K, x.shape, bias, activation, residual, want_pre, device)
 
 
-def _forward(x2, w2, outer, bias, activation: str, residual, want_pre: bool):
-    # on the current device; x2, w2: tensors that start where the rows do
-    (M, K), N, dt, device = x2.shape, w2.shape[0], DTYPES[x2.dtype], x2.device
-    y = torch.empty((*outer, N), dtype=x2.dtype, device=device)
+def _forward(x2, w2, K: int, shape, bias, activation: str, residual, want_pre: bool, device):
+    # on the current device; x2, w2: as _matrix returns them
+    (x2, M, ldx), (w2, N, ldw) = x2, w2
+    dt = DTYPES[x2.dtype]
+    y = x2.new_empty((*shape[:-1], N))
     pre = torch.empty_like(y) if want_pre else None
-    b = None if bias is None else bias.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     r2, ldr = None, 0
     if residual is not None:
-        r2 = _rows(residual, N)
-        ldr = _pitch(r2)
+        r2, _, ldr = _matrix(residual, N)
     work = _work(LINEAR_FORWARD, M, K, N, dt, device)
-    check(_lib.load().vq_linear(x2.data_ptr(), _pitch(x2), w2.data_ptr(), _pitch(w2), _address(b), _address(r2), ldr, dt,
-                                ACTIVATIONS[activation], M, K, N, y.data_ptr(), _address(pre), _address(work),
-                                _raw_stream(device)), "vq_linear")
+    check(_lib.load().vq_linear(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _address(b), _address(r2), ldr, dt, ACTIVATIONS[activation], M, K,
+                                N, y.data_ptr(), _address(pre), _address(work), _raw_stream(device)), "vq_linear")
     return y, pre
 
 
@@ -110,24 +120,25 @@ def linear_backward(grad, x, weight, pre, activation: str, want_x: bool, want_we
     """Gradients ``(input, weight, bias)`` of ``act(x W^T + b)`` for the output gradient ``grad`` (None where not
     wanted); ``pre`` is what :func:`linear_forward` returned (None for activation "none")."""
     with _on_device(x.device):
-        x2, w2 = _rows(x, weight.shape[1]), _rows(weight, weight.shape[1])
+        K = weight.shape[1]
+        x2, w2 = _matrix(x, K), _matrix(weight, K)
         p = None if pre is None else pre.contiguous()
-        return _backward(_facts(x2, w2, activation), grad.contiguous(), x.shape, x2, w2, p, want_x, want_weight, want_bias)
+        return _backward(_facts(x2, w2, K, activation), grad.contiguous(), x.shape, x2[0], w2[0], p, want_x, want_weight, want_bias)
 
 
-def _facts(x2: torch.Tensor, w2: torch.Tensor, activation: str):
+def _facts(x2, w2, K: int, activation: str):
     """What a backward pass needs besides addresses."""
-    (M, K), N, dt = x2.shape, w2.shape[0], DTYPES[x2.dtype]
-    return M, K, N, dt, ACTIVATIONS[activation], _pitch(x2), _pitch(w2), _work_bytes(LINEAR_BACKWARD, M, K, N, dt)
+    (x2, M, ldx), (_, N, ldw), dt = x2, w2, DTYPES[x2[0].dtype]
+    return M, K, N, dt, ACTIVATIONS[activation], ldx, ldw, _work_bytes(LINEAR_BACKWARD, M, K, N, dt)
 
 
 def _backward(facts, grad, shape, x2, w2, pre, want_x: bool, want_weight: bool, want_bias: bool):
     # on the current device; x2, w2: tensors that start where the rows do; grad, pre: dense
     M, K, N, dt, act, ldx, ldw, work_bytes = facts
-    dtype, device = grad.dtype, grad.device
-    gx = torch.empty(shape, dtype=dtype, device=device) if want_x else None
-    gw = torch.empty((N, K), dtype=dtype, device=device) if want_weight else None
-    gb = torch.empty((N,), dtype=dtype, device=device) if want_bias else None
+    device = grad.device
+    gx = grad.new_empty(shape) if want_x else None
+    gw = grad.new_empty((N, K)) if want_weight else None
+    gb = grad.new_empty((N,)) if want_bias else None
     work = torch.empty(work_bytes, dtype=torch.uint8, device=device) if work_bytes else None
     check(_lib.load().vq_linear_backward(grad.data_ptr(), None if pre is None else pre.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(),
                                          ldw, dt, act, M, K, N, gx.data_ptr() if want_x and M else None,
@@ -141,12 +152,13 @@ class _LinearFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, activation):
         K = weight.shape[1]
         want_pre = activation != "none" and any(ctx.needs_input_grad[:3])
-        with _on_device(x.device):
-            x2, w2 = _rows(x, K), _rows(weight, K)
-            y, pre = _forward(x2, w2, x.shape[:-1], bias, activation, residual, want_pre)
+        device = x.device
+        with _on_device(device):
+            x2, w2 = _matrix(x, K), _matrix(weight, K)
+            y, pre = _forward(x2, w2, K, x.shape, bias, activation, residual, want_pre, device)
         # a backward pass on the engine's thread takes about twice as long per line as here: what it can know is found out now
-        ctx.facts = _facts(x2, w2, activation)
-        ctx.in_place = x2.data_ptr() == x.data_ptr() and w2 is weight      # the rows are the tensors' own memory
+        ctx.facts = _facts(x2, w2, K, activation)
+        ctx.in_place = x2[0].data_ptr() == x.data_ptr() and w2[0] is weight      # the rows are the tensors' own memory
         ctx.layout = x.shape, x.stride(), weight.shape, weight.stride(), x.dtype, x.device
         ctx.activation = activation
         ctx.save_for_backward(x, weight, pre)
