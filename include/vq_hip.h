@@ -332,8 +332,11 @@ int vq_conv1x1_wgrad(const float* gy, const float* x, int layout, int64_t N, int
  * are dense.  Any K, N from 1 to 2^20, any M >= 0 (M = 0: y and gx are empty, gW and gbias zero), any element-
  * aligned pointers.  Limits beyond these: VQ_ERR_UNSUPPORTED (rows more than 8 MiB apart, M > 2^31).
  *
- * vq_linear:          p = x W^T + bias;  y = act(p) + residual;  pre (NULL: not wanted) = p in dtype.
- * vq_linear_act_grad: dp = gy * act'(pre) for `count` elements, act other than VQ_ACT_NONE.  May run in place.
+ * vq_linear:          p = x W^T + bias;  y = act(p) + residual;  pre (NULL: not wanted) = p for the activation's
+ *                     gradient: fp32 for VQ_F32, fp16 for VQ_F16, and for VQ_BF16 fp16 too (bf16 where act is
+ *                     VQ_ACT_NONE or VQ_ACT_RELU).
+ * vq_linear_act_grad: dp = gy * act'(pre) for `count` elements, act other than VQ_ACT_NONE, pre as vq_linear wrote it.
+ *                     May run in place.
  * vq_linear_dgrad:    gx = dp W.
  * vq_linear_wgrad:    gW = dp^T x;  gbias[n] = sum_m dp[m][n].  One of the two may be NULL.
  * vq_linear_backward: the three in one call, of those of gx, gW and gbias that are not NULL (for an empty gx give NULL).

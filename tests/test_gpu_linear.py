@@ -479,7 +479,7 @@ def test_bias_gradient_is_summed_before_rounding(M, N, kind):
 def test_backward_stays_within_its_outputs_and_workspace(M, K, N, kind, dt):
     lib = _lib.load()
     x, w, _, _, gy = make(M, K, N, kind, False, False, False, 2)
-    pre = torch.nn.functional.linear(x.float(), w.float()).to(kind)
+    pre = torch.nn.functional.linear(x.float(), w.float()).to(torch.float16 if kind is torch.bfloat16 else kind)   # as it is kept for silu
     bytes_of = lambda n: n * kind.itemsize
 
     def band(n):       # 256 bytes on either side
@@ -496,3 +496,23 @@ def test_backward_stays_within_its_outputs_and_workspace(M, K, N, kind, dt):
     (gx, ex), (gw, ew), (gb, eb) = backward64(gy, x, w, p, torch.zeros_like(p), slope, "silu")
     for (buf, _), want, bound, what in zip(bands, (gx, gw, gb), (ex, ew, eb), ("input", "weight", "bias")):
         close(buf[256:-256].view(kind).view(want.shape), want, bound, what)
+
+
+@pytest.mark.parametrize("M", [4, 40])
+def test_bf16_beyond_the_range_of_fp16(M):
+    # p is kept in fp16 for a bf16 layer: infinite beyond 65504, where every slope has its limit; for relu the smallest p counts
+    one = torch.ones(M, 64, device=DEV, dtype=torch.bfloat16)
+    for size in (1e3, 1e6, 1e30):
+        for act in ACTS[1:]:
+            for sign in (1.0, -1.0):
+                w = torch.full((8, 64), sign * size, device=DEV, dtype=torch.bfloat16)
+                x = one.clone().requires_grad_()
+                (gx,) = torch.autograd.grad(vq.linear(x, w, activation=act), x, torch.ones(M, 8, device=DEV, dtype=torch.bfloat16))
+                want = 8.0 * float(w[0, 0]) if sign > 0 else 0.0
+                assert bool((gx == want).all()), (size, act, sign)
+    for tiny in (1e-9, 1e-30):
+        for sign in (1.0, -1.0):
+            w = torch.full((8, 64), sign * tiny, device=DEV, dtype=torch.bfloat16)
+            x = one.clone().requires_grad_()
+            (gx,) = torch.autograd.grad(vq.linear(x, w, activation="relu"), x, torch.ones(M, 8, device=DEV, dtype=torch.bfloat16))
+            assert bool((gx == (8.0 * float(w[0, 0]) if sign > 0 else 0.0)).all())

@@ -31,7 +31,7 @@ struct VqLinearArgs {
   int64_t tiles_i;
   int tiles_j;
   void* out;                 // [I][J]
-  void* pre;                 // [I][J] or null: C + bias in T, what the activation's gradient needs
+  void* pre;                 // [I][J] or null: C + bias as VqKept, what the activation's gradient needs
   const void* bias;          // [J] or null
   const char* res;           // [I][J] or null
   int64_t ldr;               // bytes between rows of res
@@ -192,6 +192,17 @@ __device__ __forceinline__ float vql_act_of(float p, int act) {
   } else {
     return p * vql_cdf(p);
   }
+}
+// As what p is kept for the activation's gradient.  fp16 for both 16-bit types: its rounding shifts act' by an eighth of what that of
+// bf16 does (gradients off by 1.43 instead of 1.5 times the last rounding), and what it takes for infinite lies far beyond where
+// act' has its limit.  But relu's needs the sign of the smallest p.
+template <typename T, int KIND> struct VqKept { typedef _Float16 type; };
+template <int KIND> struct VqKept<float, KIND> { typedef float type; };
+template <> struct VqKept<VqBf16, VQL_THRESHOLD> { typedef VqBf16 type; };
+__device__ __forceinline__ float vql_kept(float p, int) { return p; }
+__device__ __forceinline__ float vql_kept(_Float16 p, int) { return (float)p; }
+__device__ __forceinline__ float vql_kept(VqBf16 p, int act) {
+  return act == VQ_ACT_RELU ? VqElem<VqBf16>::to(p) : (float)__builtin_bit_cast(_Float16, p.v);
 }
 // act'(p).  Beyond |p| = 100 every derivative has its limit, 0 or 1; the clamp keeps inf * 0 out of it.
 template <bool FAST>
@@ -434,13 +445,15 @@ struct VqOperand {
 };
 
 // -------------------------------------------------------------------------------- epilogue
-// out = act(c + bias) + residual, rounded once, for 16 / sizeof(T) columns; pre = c + bias rounded (kept for the activation's
+// out = act(c + bias) + residual, rounded once, for 16 / sizeof(T) columns; pre = c + bias (kept for the activation's
 // gradient); res: the residual's 16 bytes.
 template <typename T, int KIND>
 __device__ __forceinline__ void vql_finish(const VqLinearArgs& a, const float* c, const float* bias, u32x4 res, u32x4& out, u32x4& pre) {
   constexpr int E = 16 / sizeof(T);
+  typedef typename VqKept<T, KIND>::type Kept;
   float p[E];
   VqChunk<T> y;
+  VqChunk<Kept> kept;
   if constexpr (KIND == VQL_PLAIN) {
 #pragma unroll
     for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(c[e]);
@@ -451,8 +464,8 @@ __device__ __forceinline__ void vql_finish(const VqLinearArgs& a, const float* c
   for (int e = 0; e < E; ++e) p[e] = c[e] + bias[e];
   if (a.pre) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) y.e[e] = VqElem<T>::from(p[e]);
-    pre = __builtin_bit_cast(u32x4, y);
+    for (int e = 0; e < E; ++e) kept.e[e] = VqElem<Kept>::from(p[e]);
+    pre = __builtin_bit_cast(u32x4, kept);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) p[e] = vql_act_of<KIND, sizeof(T) == 2>(p[e], a.act);

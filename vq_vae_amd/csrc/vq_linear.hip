@@ -35,8 +35,12 @@ __device__ __forceinline__ f32x4 rows_mma(u32x4 a, u32x4 b, f32x4 c) {
 template <typename T>
 __device__ __forceinline__ void epilogue_one(const VqLinearArgs& a, int64_t i, int j, float c) {
   if (a.bias) c += VqElem<T>::to(reinterpret_cast<const T*>(a.bias)[j]);
-  if (a.pre) reinterpret_cast<T*>(a.pre)[i * a.J + j] = VqElem<T>::from(c);
   const int kind = vql_kind(a.act);
+  if (a.pre) {
+    typedef typename VqKept<T, VQL_SIGMOID>::type Kept;
+    if (kind == VQL_THRESHOLD) reinterpret_cast<T*>(a.pre)[i * a.J + j] = VqElem<T>::from(c);
+    else reinterpret_cast<Kept*>(a.pre)[i * a.J + j] = VqElem<Kept>::from(c);
+  }
   c = kind == VQL_THRESHOLD ? vql_act_of<VQL_THRESHOLD, sizeof(T) == 2>(c, a.act)
       : kind == VQL_SIGMOID ? vql_act_of<VQL_SIGMOID, sizeof(T) == 2>(c, a.act)
                             : vql_act_of<VQL_NORMAL, sizeof(T) == 2>(c, a.act);
@@ -153,6 +157,7 @@ __global__ __launch_bounds__(256) void vql_join_sums_kernel(const float* part, i
 // dp = gy * act'(pre), rounded to T: the operand of both products of the backward pass, whose matrix instructions take T.
 // What is read passes the caches by, so that dp, which is read next, stays there (64 Ki x 1024 bf16 and the weight gradient
 // behind it 132 -> 121 us).
+// pre: T by its size; what it is, vql_kept knows
 template <typename T>
 __global__ __launch_bounds__(256) void vql_act_grad_kernel(const T* gy, const T* pre, int act, int64_t count, T* dp) {
   constexpr int E = 16 / sizeof(T);
@@ -163,12 +168,12 @@ __global__ __launch_bounds__(256) void vql_act_grad_kernel(const T* gy, const T*
     VqChunk<T> d;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      d.e[e] = VqElem<T>::from(VqElem<T>::to(g.e[e]) * vql_act_slope<sizeof(T) == 2>(VqElem<T>::to(p.e[e]), act));
+      d.e[e] = VqElem<T>::from(VqElem<T>::to(g.e[e]) * vql_act_slope<sizeof(T) == 2>(vql_kept(p.e[e], act), act));
     vql_store16<T>(dp + v * E, __builtin_bit_cast(u32x4, d));
   }
   const int64_t at = vecs * E + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at < count)
-    dp[at] = VqElem<T>::from(VqElem<T>::to(gy[at]) * vql_act_slope<sizeof(T) == 2>(VqElem<T>::to(pre[at]), act));
+    dp[at] = VqElem<T>::from(VqElem<T>::to(gy[at]) * vql_act_slope<sizeof(T) == 2>(vql_kept(pre[at], act), act));
 }
 
 // The same with the bias gradient: the sums over the rows, of dp before it is rounded (sums of the rounded values are off by
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(SUMS_NT) void vql_act_grad_sums_kernel(const T* gy,
     VqChunk<T> d;
 #pragma unroll
     for (int e = 0; e < E; ++e) {   // elements behind the row's end are zero: g is
-      const float v = VqElem<T>::to(g.e[e]) * vql_act_slope<sizeof(T) == 2>(VqElem<T>::to(p.e[e]), act);
+      const float v = VqElem<T>::to(g.e[e]) * vql_act_slope<sizeof(T) == 2>(vql_kept(p.e[e], act), act);
       sum[e] += v;
       d.e[e] = VqElem<T>::from(v);
     }

@@ -40,6 +40,11 @@ def _address(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _kept(dtype: torch.dtype, activation: str) -> torch.dtype:
+    """As what ``input @ weight.T + bias`` is kept for the gradient: fp16 is eight times as exact as bf16 where it matters."""
+    return torch.float16 if dtype is torch.bfloat16 and activation not in ("none", "relu") else dtype
+
+
 def _matrix(t: torch.Tensor, width: int):
     """t as rows of ``width`` elements, dense each and at any distance from each other: ``(a tensor that starts where they do, how
     many, elements between them)``; copied only if it is not such."""
@@ -105,7 +110,7 @@ def _forward(x2, w2, K: int, shape, bias, activation: str, residual, want_pre: b
     (x2, M, ldx), (w2, N, ldw) = x2, w2
     dt = DTYPES[x2.dtype]
     y = x2.new_empty((*shape[:-1], N))
-    pre = torch.empty_like(y) if want_pre else None
+    pre = y.new_empty(y.shape, dtype=_kept(y.dtype, activation)) if want_pre else None
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     r2, ldr = None, 0
     if residual is not None:
@@ -179,7 +184,7 @@ def _gradients(ctx, grad):
         x_shape, x_stride, w_shape, w_stride, dtype, device = ctx.layout
         if not (x.shape == x_shape and x.dtype is dtype and x.device == device
                 and weight.shape == w_shape and weight.dtype is dtype and weight.device == device
-                and (pre is None or (pre.shape == grad.shape and pre.dtype is dtype and pre.device == device))):
+                and (pre is None or (pre.shape == grad.shape and pre.dtype is _kept(dtype, ctx.activation) and pre.device == device))):
             raise RuntimeError("a hook on saved tensors returned a tensor of another shape, type or device than was saved")
         if (ctx.in_place and x.stride() == x_stride and weight.stride() == w_stride and grad.is_contiguous()
                 and (pre is None or pre.is_contiguous())):
@@ -203,8 +208,8 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     other strides are copied first.  Sums are fp32 and every output is rounded once; the result is the same bits on
     every run.
 
-    Differentiable once in all four tensors.  For an activation the forward keeps ``input @ weight.T + bias`` in the
-    tensors' type, and the backward rounds the gradient behind the activation to it before the two products (the bias
+    Differentiable once in all four tensors.  For an activation the forward keeps ``input @ weight.T + bias`` in fp32 or
+    fp16 (bf16 layers too, but for relu), and the backward rounds the gradient behind the activation to it before the two products (the bias
     gradient is summed before that rounding).
     Under autocast the tensors keep their types.  May be captured in a graph, backward included (drop every eager autograd
     graph over the same leaves before capturing, as torch asks for any backward under capture)."""
