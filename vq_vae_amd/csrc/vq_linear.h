@@ -680,7 +680,7 @@ __device__ __forceinline__ void vql_publish_lds() {
 // sets of fragments, one read while the other is multiplied, so that neither the LDS reads nor the barrier of a step leave
 // the matrix cores idle:
 //     q0 | read q1, multiply q0 | read q2, multiply q1 | read q3, multiply q2 | barrier, fill, read the next q0, multiply q3
-// `fly`: this wave's DMA instructions that may still be in flight behind those of the next step, or 0.  `into` and `from`
+// `counted`: FLYING of this wave's DMA instructions, those behind the next step's, may still be in flight.  `into` and `from`
 // are the same memory; __restrict__ tells the compiler that a fragment read need not wait for the DMA in flight: the
 // barriers and the counted waits see to that.
 template <typename T, typename OA, typename OB, int TI, int TJ, int FLYING, int S, int P>

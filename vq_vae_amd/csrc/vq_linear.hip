@@ -285,15 +285,17 @@ const Cost COST[VQL_CONFIGS] = {
 Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
   const size_t es = elem_size(dtype);
   Plan best{};
-  // Few rows: the kernel that reads W once, with 16 channels to a workgroup.  A sum of more than 32 KiB a channel over few
-  // channels leaves most of the device idle there: the tiled kernel splits it.
-  if (layout == 0 && I <= ROWS_MAX && ((J + 15) / 16 * 4 > CUS || R * es <= 32768)) {
-    best.rows = true;
-    best.splits = 1;
-    return best;
-  }
   const int64_t steps = (R * es + 127) / 128;
   double best_t = 1e300;
+  // Few rows: the kernel that reads W once, 16 channels to a workgroup whose waves share the sum.  Its time goes by the bytes of a
+  // channel and the rows, as measured from 12 to 64 KiB a channel and 128 to 8192 channels; long sums over few channels leave
+  // most of the device idle there, and the tiled kernel splits them (us, rows kernel and tiled one: 8 rows, 4096 -> 4096 bf16 9.1 and
+  // 13.7, 16 rows, 8192 -> 512 16.7 and 11.9, 1 row, 16384 -> 2048 20.4 and 18.1, -> 4096 23.2 and 26.7).
+  if (layout == 0 && I <= ROWS_MAX) {
+    best.rows = true;
+    best.splits = 1;
+    best_t = 2.4 + R * es / 1024.0 * (0.54 + 0.0225 * I) * std::max(1.0, (J + 15) / 16 / (double)CUS);
+  }
   for (int c = 0; c < VQL_CONFIGS; ++c) {
     const Cost& cost = COST[c];
     const auto& of = cost.of[dma][es == 4];
@@ -309,6 +311,7 @@ Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
       if (sp > 1) t += 3.0 + (double)ti * tj * cost.tile * cost.tile * 8 * sp / 6.5e6;
       if (t < best_t) {
         best_t = t;
+        best.rows = false;
         best.config = c;
         best.splits = (int)sp;
         best.steps_per_split = per;
