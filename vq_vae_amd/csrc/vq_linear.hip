@@ -277,24 +277,29 @@ const Cost COST[VQL_CONFIGS] = {
     {128, 2, {{{{1.70f, 2.05f}, 8.0f}, {{2.95f, 4.60f}, 12.0f}}, {{{0.72f, 0.95f}, 6.5f}, {{1.97f, 3.69f}, 13.5f}}}},
     {256, 1, {{}, {{{1.55f}, 12.5f}, {{7.15f}, 27.0f}}}},
 };
+// How the operands' rows lie: 16-bit ones at odd addresses, on 4 bytes at least, on 16 (and so filled by DMA).
+enum { ROWS_ODD = 0, ROWS_WORDS = 1, ROWS_DMA = 2 };
 // The cheapest tile with its best split of the sum: rounds of workgroups x (steps x time of a step + once), the last round
 // with as many on a CU as are left, and the join of a split sum (a launch, the partial sums written and read at 6.5 TB/s:
 // they stay in the last-level cache).  Over 36 random products of 17 to 65536 rows and 64 to 4096 channels, every layout, the
 // choice took 1.03 times as long on average as the best of all tiles and of 1, 2, 4 .. 32 splits, 1.19 times at worst (5.1 us instead of
 // 4.3), 1.15 among those over 10 us.
-Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, bool dma) {
+Plan make_plan(int layout, int64_t I, int J, int64_t R, int dtype, int lie) {
   const size_t es = elem_size(dtype);
+  const bool dma = lie == ROWS_DMA;
   Plan best{};
   const int64_t steps = (R * es + 127) / 128;
   double best_t = 1e300;
   // Few rows: the kernel that reads W once, 16 channels to a workgroup whose waves share the sum.  Its time goes by the bytes of a
   // channel and the rows, as measured from 12 to 64 KiB a channel and 128 to 8192 channels; long sums over few channels leave
   // most of the device idle there, and the tiled kernel splits them (us, rows kernel and tiled one: 8 rows, 4096 -> 4096 bf16 9.1 and
-  // 13.7, 16 rows, 8192 -> 512 16.7 and 11.9, 1 row, 16384 -> 2048 20.4 and 18.1, -> 4096 23.2 and 26.7).
+  // 13.7, 16 rows, 8192 -> 512 16.7 and 11.9, 1 row, 16384 -> 2048 20.4 and 18.1, -> 4096 23.2 and 26.7; at odd
+  // addresses 8 rows, 4097 -> 512 22.8 and 12.3, 1025 -> 512 8.2 and 11.1).
   if (layout == 0 && I <= ROWS_MAX) {
     best.rows = true;
     best.splits = 1;
-    best_t = 2.4 + R * es / 1024.0 * (0.54 + 0.0225 * I) * std::max(1.0, (J + 15) / 16 / (double)CUS);
+    const double kib = lie == ROWS_ODD ? 1.75 + 0.085 * I : 0.54 + 0.0225 * I;
+    best_t = 2.4 + R * es / 1024.0 * kib * std::max(1.0, (J + 15) / 16 / (double)CUS);
   }
   for (int c = 0; c < VQL_CONFIGS; ++c) {
     const Cost& cost = COST[c];
@@ -429,7 +434,8 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, const float*
   bool dma = aligned16(a.A) && aligned16(a.B) && a.lda % 16 == 0 && a.ldb % 16 == 0;
   if (layout == 1 && a.J % E) dma = false;                 // a piece of an m-major operand must not pass its row's end
   if (layout == 2 && (a.I % E || a.J % E)) dma = false;
-  const Plan p = make_plan(layout, a.I, a.J, a.R, dtype, dma);
+  const bool odd = ((reinterpret_cast<uintptr_t>(a.A) | reinterpret_cast<uintptr_t>(a.B) | a.lda | a.ldb) & 3) != 0;
+  const Plan p = make_plan(layout, a.I, a.J, a.R, dtype, dma ? ROWS_DMA : odd ? ROWS_ODD : ROWS_WORDS);
   a.splits = p.splits;
   a.steps_per_split = (int)p.steps_per_split;
   a.tiles_i = p.tiles_i;
@@ -459,8 +465,8 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, const float*
 
 int64_t product_work(int layout, int64_t I, int J, int64_t R, int dtype, bool sums) {
   int64_t bytes = 0;
-  for (int dma = 0; dma < 2; ++dma) {
-    const Plan p = make_plan(layout, I, J, R, dtype, dma);
+  for (int lie = ROWS_ODD; lie <= ROWS_DMA; ++lie) {
+    const Plan p = make_plan(layout, I, J, R, dtype, lie);
     bytes = std::max(bytes, part_bytes(p) + (sums && p.splits > 1 ? (int64_t)p.splits * I * 4 : 0));
   }
   return bytes;
