@@ -516,3 +516,37 @@ def test_bf16_beyond_the_range_of_fp16(M):
             x = one.clone().requires_grad_()
             (gx,) = torch.autograd.grad(vq.linear(x, w, activation="relu"), x, torch.ones(M, 8, device=DEV, dtype=torch.bfloat16))
             assert bool((gx == (8.0 * float(w[0, 0]) if sign > 0 else 0.0)).all())
+
+
+def test_threads_on_streams_of_their_own():
+    import threading
+    sizes = [(300, 264, 136), (16, 8192, 512), (777, 130, 515), (2048, 256, 512)]
+    cases = [make(*size, torch.bfloat16, True, True, False, 20 + i) for i, size in enumerate(sizes)]
+
+    def step(case):
+        x, w, b, r, gy = case
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = vq.linear(*leaves, "silu", r)
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+    want = [step(c) for c in cases]
+    norms = [vq.grad_norm(w[1:]) for w in want]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = step(cases[i])
+                    norm = vq.grad_norm(got[1:])
+                    torch.cuda.current_stream().synchronize()
+                    if not (all(torch.equal(a, c) for a, c in zip(got, want[i])) and torch.equal(norm, norms[i])):
+                        wrong.append(i)
+        except Exception as e:      # would be lost with the thread
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

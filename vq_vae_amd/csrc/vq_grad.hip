@@ -90,7 +90,10 @@ __device__ __forceinline__ void norm_chunk(const char* src, int64_t at, int64_t 
   if (count == G_CHUNK / (int64_t)sizeof(T)) {
     u32x4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = ONCE ? vql_once16<T>(p + (u * 256 + threadIdx.x) * 16) : vql_load16<T>(p + (u * 256 + threadIdx.x) * 16);
+    for (int u = 0; u < U; ++u) {
+      const char* at_u = p + (u * 256 + threadIdx.x) * 16;
+      v[u] = ONCE ? vql_once16<T>(at_u) : vql_load16<T>(at_u);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const VqChunk<T> c = __builtin_bit_cast(VqChunk<T>, v[u]);
@@ -157,8 +160,12 @@ struct alignas(sizeof(S)) VqRun {
 };
 template <typename S, int W>
 __device__ __forceinline__ VqRun<S, W> load_run(const char* p) {
-  if constexpr (W * sizeof(S) == 8) return __builtin_bit_cast(VqRun<S, W>, (u32x2)__builtin_nontemporal_load(reinterpret_cast<const vqg_u32x2_a2*>(p)));
-  else return __builtin_bit_cast(VqRun<S, W>, vql_once16<S>(p));
+  if constexpr (W * sizeof(S) == 8) {
+    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const vqg_u32x2_a2*>(p));
+    return __builtin_bit_cast(VqRun<S, W>, v);
+  } else {
+    return __builtin_bit_cast(VqRun<S, W>, vql_once16<S>(p));
+  }
 }
 template <typename S, typename D>
 __device__ __forceinline__ void scale_chunk(const char* src, char* dst, int64_t at, int64_t count, float c) {

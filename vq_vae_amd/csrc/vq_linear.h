@@ -172,8 +172,8 @@ __device__ __forceinline__ float vql_cdf(float p) {
   return p < 0.0f ? half : 1.0f - half;
 }
 // The epilogues of the product kernel, one to a kernel: the epilogue is unrolled over a wave's accumulators, and with all
-// activations in it the code outgrows the instruction cache (64 Ki x 256 -> 1024 bf16 with gelu_tanh 72 us, now 60; 8192 x 4096 x 4096 with a
-// residual 238 us, now 220).
+// activations in it the code outgrows the instruction cache (operands in the caches: 64 Ki x 256 -> 1024 bf16 with gelu_tanh 72 us
+// instead of 60; 8192 x 4096 x 4096 with a residual 238 instead of 220).
 enum { VQL_PLAIN = 0,     // no bias, activation or residual: the products of the backward pass
        VQL_THRESHOLD = 1, // none and relu
        VQL_SIGMOID = 2,   // silu and gelu_tanh: p sigmoid(p) and p sigmoid(2u)

@@ -177,9 +177,9 @@ __global__ __launch_bounds__(256) void vql_act_grad_kernel(const T* gy, const T*
 }
 
 // The same with the bias gradient: the sums over the rows, of dp before it is rounded (sums of the rounded values are off by
-// 1.5 to 2.5 times as much).  64 Ki x 1024 bf16: 69 us, 5.9 TB/s.  A thread keeps the columns of one 16-byte piece and takes every so many-th row, two of them in
-// flight (four: 87 instead of 82 us; a workgroup's rows next to each other 89); the rows that a workgroup takes at a time are added
-// in LDS at the end.
+// 1.5 to 2.5 times as much).  A thread keeps the columns of one 16-byte piece and takes every so many-th row, two of them in flight;
+// the rows that a workgroup takes at a time are added in LDS at the end.  64 Ki x 1024 bf16: 69 us, 5.9 TB/s.  Before the loads
+// passed the caches by, 82; four rows in flight 87, a workgroup's rows next to each other 89.
 constexpr int SUMS_NT = 1024, SUMS_WGS = 256;
 template <typename T>
 __global__ __launch_bounds__(SUMS_NT) void vql_act_grad_sums_kernel(const T* gy, const T* pre, int act, int64_t M, int N, int lanes,
