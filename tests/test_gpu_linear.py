@@ -550,3 +550,25 @@ def test_threads_on_streams_of_their_own():
     for t in threads:
         t.join()
     assert not wrong
+
+
+# few rows; tiles by DMA; by registers; a split sum joined; the 256 tile
+@pytest.mark.parametrize("M, K, N", [(5, 70, 66), (100, 64, 72), (100, 70, 66), (40, 8192, 72), (2048, 64, 2048)])
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+def test_activations_of_infinities_and_of_the_largest_values(M, K, N, kind):
+    # p is one of the values exactly: one input channel with a weight of one, and the bias of a product of zeros
+    top = torch.finfo(kind).max
+    values = torch.tensor([math.inf, -math.inf, math.nan, top, -top], device=DEV).to(kind)
+    by_row, by_col = values[torch.arange(M, device=DEV) % 5][:, None].expand(M, N), values[torch.arange(N, device=DEV) % 5].expand(M, N)
+    x = torch.zeros(M, K, device=DEV, dtype=kind)
+    w = torch.zeros(N, K, device=DEV, dtype=kind)
+    w[:, 0] = 1.0
+    hot = x.clone()
+    hot[:, 0] = by_row[:, 0]
+    for act in ACTS:
+        for got, p in ((vq.linear(hot, w, None, act), by_row), (vq.linear(x, w, by_col[0].contiguous(), act), by_col)):
+            want = act64(p.double(), act)[0]
+            assert torch.equal(got.isnan(), want.isnan()), act
+            assert torch.equal(got.isinf(), want.isinf()), act
+            # largest values: act(p) is p or, below, less than the smallest number
+            assert torch.equal(got.nan_to_num(nan=7.0).double(), want.to(kind).nan_to_num(nan=7.0).double()), act
