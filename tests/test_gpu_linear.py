@@ -572,3 +572,29 @@ def test_activations_of_infinities_and_of_the_largest_values(M, K, N, kind):
             assert torch.equal(got.isinf(), want.isinf()), act
             # largest values: act(p) is p or, below, less than the smallest number
             assert torch.equal(got.nan_to_num(nan=7.0).double(), want.to(kind).nan_to_num(nan=7.0).double()), act
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_recorded_calls(requires_grad):
+    # a trace and a tangent are refused; a compiler runs the call outside its graphs
+    import torch.autograd.forward_ad as fwad
+    x, w, b, r, gy = make(40, 33, 21, torch.float32, True, True, False, 5)
+    new = make(70, 33, 21, torch.float32, True, True, True, 6)
+    f = lambda x, w, b, r: vq.linear(x, w, b, "gelu", r) * 2
+    args = [t.clone().requires_grad_(requires_grad) for t in (x, w, b, r)]
+    with pytest.raises(NotImplementedError, match="traced"):
+        torch.jit.trace(f, args, check_trace=False)
+    compiled = torch.compile(f, backend="eager")
+    for tensors in ((x, w, b, r, gy), new):
+        ins = [t.detach().clone().requires_grad_() for t in tensors[:4]]
+        assert torch.equal(compiled(*tensors[:4]), f(*tensors[:4]))
+        for a, c in zip(torch.autograd.grad(compiled(*ins), ins, tensors[4]), torch.autograd.grad(f(*ins), ins, tensors[4])):
+            assert torch.equal(a, c)
+    with fwad.dual_level():
+        for i in range(4):
+            dual = [fwad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+            with pytest.raises(NotImplementedError):
+                f(*dual)
+        with pytest.raises(NotImplementedError):
+            vq.grad_norm([fwad.make_dual(x, x)])
+        assert torch.equal(f(*args), f(x, w, b, r))

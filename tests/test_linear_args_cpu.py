@@ -1,5 +1,6 @@
 """Refusals of the linear layer, the gradient norm and clipping: wrong arguments end in an error before anything is
 launched, in Python and at the C interface.  Nothing here needs a GPU."""
+import contextlib
 import ctypes
 
 import numpy as np
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 import vq_vae_amd as vq
-from vq_vae_amd import _lib
+from vq_vae_amd import _lib, projection
 
 BF, F32 = torch.bfloat16, torch.float32
 
@@ -181,3 +182,99 @@ def test_c_interface_checks_the_tensor_list():
     many = (Ref * 65537)()
     assert lib.vq_grad_norm(many, 65537, 2, p, p, None) == TOO_LARGE
     assert lib.vq_grad_norm_work_bytes(-1) == 0 and lib.vq_grad_norm_work_bytes(0) > 0
+
+
+class Products:
+    """The calls of the library that a layer without activation makes, on host memory (fp32)."""
+
+    @staticmethod
+    def at(address, rows, cols, pitch):
+        flat = np.ctypeslib.as_array((ctypes.c_float * ((rows - 1) * pitch + cols)).from_address(address))
+        return np.lib.stride_tricks.as_strided(flat, (rows, cols), (4 * pitch, 4))
+
+    def vq_linear(self, x, ldx, W, ldw, bias, residual, ldr, dtype, act, M, K, N, y, pre, work, stream):
+        assert all(type(v) is int for v in (ldx, ldw, ldr, M, K, N))
+        out = self.at(x, M, K, ldx) @ self.at(W, N, K, ldw).T
+        if bias:
+            out = out + self.at(bias, 1, N, N)
+        if residual:
+            out = out + self.at(residual, M, N, ldr)
+        self.at(y, M, N, N)[:] = out
+        return 0
+
+    def vq_linear_backward(self, gy, pre, x, ldx, W, ldw, dtype, act, M, K, N, gx, gW, gbias, work, stream):
+        g = self.at(gy, M, N, N)
+        for to, shape, value in ((gx, (M, K), g @ self.at(W, N, K, ldw)), (gW, (N, K), g.T @ self.at(x, M, K, ldx)), (gbias, (1, N), g.sum(0))):
+            if to:
+                self.at(to, *shape, shape[1])[:] = value
+        return 0
+
+
+@pytest.fixture
+def products(monkeypatch):
+    """What the layer hands to the library, and what torch makes of it, without a GPU."""
+    monkeypatch.setattr(projection._lib, "load", Products)
+    monkeypatch.setattr(projection, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(projection, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(projection, "_require_cuda", lambda t, name: None)
+    monkeypatch.setattr(projection, "_work_bytes", lambda *a: 0)
+
+
+def layer_inputs(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(*s, generator=g) for s in ((7, 3), (4, 3), (4,), (7, 4))]
+
+
+def formula(x, w, b, r):
+    return x @ w.t() + b + r
+
+
+def test_stand_in_for_the_library(products):
+    args = [a.requires_grad_() for a in layer_inputs()]
+    y, want = vq.linear(*args[:3], residual=args[3]), formula(*args)
+    assert torch.allclose(y, want)
+    for a, b in zip(torch.autograd.grad(y.square().sum(), args), torch.autograd.grad(want.square().sum(), args)):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_derivatives_are_refused(products, requires_grad):
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level():
+        for i in range(4):
+            args = [a.requires_grad_(requires_grad) for a in layer_inputs()]
+            args[i] = fwad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError):
+                vq.linear(*args[:3], residual=args[3])
+        # what carries no tangent is answered
+        args = [a.requires_grad_(requires_grad) for a in layer_inputs()]
+        y = vq.linear(*args[:3], residual=args[3])
+        assert torch.allclose(y, formula(*args))
+        # a tangent that arrives with the output's gradient
+        if requires_grad:
+            for at in (0, 3):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    torch.autograd.grad(y, args[at], fwad.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
+        g = fwad.make_dual(torch.ones(3), torch.ones(3))
+        for call in (lambda: vq.grad_norm([torch.ones(2), g]), lambda: vq.clip_grads([g], 1.0),
+                     lambda: vq.clip_grads([torch.ones(3)], 1.0, out=[g])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_traces_are_refused(products, requires_grad):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    args = [a.requires_grad_(requires_grad) for a in layer_inputs()]
+    for call in (lambda g: vq.linear(g, args[1]), lambda g: vq.grad_norm([g.detach()]), lambda g: vq.clip_grads([g.detach()], 1.0)):
+        with pytest.raises(NotImplementedError, match="traced"):
+            make_fx(call)(args[0])
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(call, args[0], check_trace=False)
+
+    class Passing(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    with Passing():
+        assert torch.allclose(vq.linear(*args[:3], residual=args[3]), formula(*args))

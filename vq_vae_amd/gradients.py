@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from ._lib import NORM_1, NORM_2, NORM_INF, check
 from .projection import DTYPES
-from .ops import _on_device, _raw_stream, _require_cuda
+from .ops import _on_device, _raw_stream, _recording, _refuse_recording, _require_cuda
 
 #: source and result type of a tensor scaled in place, as one word of the C interface's entry
 _TWICE = {dtype: code | code << 32 for dtype, code in DTYPES.items()}
@@ -104,6 +104,8 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
     host).  The same bits on every run; may be captured in a graph."""
     kind = _kind(norm_type)
     grads = _list(grads, "grads")
+    if _recording():
+        _refuse_recording(grads, "grad_norm")
     if not grads:
         return torch.zeros(())
     _require_cuda(grads[0], "grads")
@@ -134,6 +136,8 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         out = _list(out, "out")
         if len(out) != len(grads):
             raise ValueError(f"{len(grads)} gradients but {len(out)} tensors in out")
+    if _recording():
+        _refuse_recording([*grads, *(out or ())], "clip_grads")
     if not grads:
         return torch.zeros(())
     written = grads if out is None else out

@@ -15,7 +15,7 @@ import torch.nn as nn
 
 from . import _lib
 from ._lib import ACTIVATIONS, LINEAR_BACKWARD, LINEAR_FORWARD, check
-from .ops import _on_device, _raw_stream, _require_cuda
+from .ops import _on_device, _raw_stream, _recording, _refuse_recording, _require_cuda
 
 DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -171,6 +171,8 @@ class _LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
+        if _recording():
+            _refuse_recording([grad], "the gradient of linear")
         # under create_graph the result has to refuse a second derivative; the wrapper that sees to it takes 5 us
         return _gradients_once(ctx, grad) if torch.is_grad_enabled() else _gradients(ctx, grad)
 
@@ -211,8 +213,11 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     Differentiable once in all four tensors.  For an activation the forward keeps ``input @ weight.T + bias`` in fp32 or
     fp16 (bf16 layers too, but for relu), and the backward rounds the gradient behind the activation to it before the two products (the bias
     gradient is summed before that rounding).
+    Forward-mode derivatives, transforms of ``torch.func`` and traces (``torch.jit.trace``, ``make_fx``) are refused.
     Under autocast the tensors keep their types.  May be captured in a graph, backward included (drop every eager autograd
     graph over the same leaves before capturing, as torch asks for any backward under capture)."""
+    if _recording():
+        _refuse_recording((input, weight, bias, residual), "linear")
     _check(input, weight, bias, activation, residual)
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
