@@ -274,3 +274,19 @@ def test_inference_tensors():
         assert abs(float(norm) - want) <= 2.0 ** -22 * want
         assert abs(float(vq.grad_norm(g)) - 1.0) <= 1e-5
         norm = vq.clip_grads([g[0] * want, g[1] * want], 1e9)
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0])
+def test_norms_beyond_fp32_scale_by_zero(p):
+    # the norm of finite gradients that fp32 has no number for is infinite, and scales by max_norm / inf; one just inside does not
+    n = 1 << 16
+    for outs in (False, True):
+        g = [torch.full((n,), 3e38, device=DEV), torch.full((9,), -3e38, device=DEV).bfloat16()]
+        to = [torch.full((n,), 7.0, device=DEV), torch.full((9,), 7.0, device=DEV)] if outs else g
+        assert float(vq.clip_grads(g, 1.0, p, out=to if outs else None)) == math.inf
+        assert not any(bool(t.any()) for t in to)
+    inside = [torch.full((n,), 1e38 * n ** (-1 / p), device=DEV)]
+    keep = [t.clone() for t in inside]
+    norm = vq.clip_grads(inside, 1e30, p)
+    assert math.isfinite(float(norm))
+    clipped_ok(inside, keep, 1e30, p)

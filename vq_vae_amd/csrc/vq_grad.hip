@@ -204,10 +204,11 @@ __global__ __launch_bounds__(256) void vqg_scale_kernel(GradTable t, const doubl
                                                         float* norm) {
   __shared__ double s[4];
   const double total = whole_norm(part, n_part, kind, s);
-  double cd = (double)max_norm / (total + 1e-6);
+  const float rounded = (float)total;                // c goes by the norm that is returned: infinite beyond fp32, and then zero
+  double cd = (double)max_norm / ((double)rounded + 1e-6);
   cd = cd > 1.0 ? 1.0 : cd;                          // NaN passes
   const float c = (float)cd;
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = rounded;
   for_chunks<true>(t, [&](int i, int64_t at, int64_t count) {
     if (c == 1.0f && t.src[i] == t.dst[i]) return;
     switch (t.type[i]) {
