@@ -290,3 +290,18 @@ def test_norms_beyond_fp32_scale_by_zero(p):
     norm = vq.clip_grads(inside, 1e30, p)
     assert math.isfinite(float(norm))
     clipped_ok(inside, keep, 1e30, p)
+
+
+def test_max_norms_beyond_fp32():
+    # a finite max_norm that fp32 has no number for leaves finite norms alone and is nothing beside an infinite one
+    for max_norm in (1e39, 1e300):
+        g = make([1000, 7], TYPES)
+        keep = [t.clone() for t in g]
+        vq.clip_grads(g, max_norm)
+        assert all(torch.equal(a, b) for a, b in zip(g, keep))
+        g[1][3] = math.inf
+        assert float(vq.clip_grads(g, max_norm)) == math.inf
+        assert not bool(g[0].any()) and bool(g[1][3].isnan()) and not bool(g[1][:3].any())
+    top = torch.full((1,), torch.finfo(torch.float32).max, device=DEV)
+    vq.clip_grads([top], 1e39)
+    assert float(top) == torch.finfo(torch.float32).max

@@ -20,6 +20,8 @@ from .ops import _on_device, _raw_stream, _recording, _refuse_recording, _requir
 #: source and result type of a tensor scaled in place, as one word of the C interface's entry
 _TWICE = {dtype: code | code << 32 for dtype, code in DTYPES.items()}
 
+_FP32_MAX = torch.finfo(torch.float32).max
+
 _KINDS = {1.0: NORM_1, 2.0: NORM_2, math.inf: NORM_INF}
 
 
@@ -34,7 +36,8 @@ def _max_norm(max_norm) -> float:
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
-    return max_norm
+    # the C interface takes fp32: a finite one beyond it would turn infinite, and NaN over an infinite norm
+    return min(max_norm, _FP32_MAX) if math.isfinite(max_norm) else max_norm
 
 
 def _list(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], name: str) -> List[torch.Tensor]:
