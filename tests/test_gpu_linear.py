@@ -598,3 +598,17 @@ def test_recorded_calls(requires_grad):
         with pytest.raises(NotImplementedError):
             vq.grad_norm([fwad.make_dual(x, x)])
         assert torch.equal(f(*args), f(x, w, b, r))
+
+
+@pytest.mark.parametrize("M, K", [(4, 64), (40, 64), (40, 70), (40, 8192)])
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+def test_relu_slope_of_the_smallest_values(M, K, kind):
+    # p = +-2^-27 is nothing in fp16, but above or below zero: the slope is 1 or 0
+    x = torch.zeros(M, K, device=DEV, dtype=kind)
+    x[:, 0] = 2.0 ** -13
+    x.requires_grad_()
+    for sign in (1.0, -1.0, 0.0, -0.0):
+        w = torch.zeros(72, K, device=DEV, dtype=kind)
+        w[:, 0] = sign * 2.0 ** -14
+        (gx,) = torch.autograd.grad(vq.linear(x, w, activation="relu"), x, torch.ones(M, 72, device=DEV, dtype=kind))
+        assert bool((gx[:, 0] == (72 * 2.0 ** -14 if sign > 0 else 0.0)).all()) and not bool(gx[:, 1:].any()), sign

@@ -197,10 +197,19 @@ __device__ __forceinline__ float vql_act_of(float p, int act) {
 }
 // As what p is kept for the activation's gradient.  fp16 for both 16-bit types: its rounding shifts act' by an eighth of what that of
 // bf16 does (gradients off by 1.43 instead of 1.5 times the last rounding), and what it takes for infinite lies far beyond where
-// act' has its limit.  But relu's needs the sign of the smallest p.
+// act' has its limit.  But relu's needs the sign of the smallest p: bf16 has it.
 template <typename T, int KIND> struct VqKept { typedef _Float16 type; };
 template <int KIND> struct VqKept<float, KIND> { typedef float type; };
 template <> struct VqKept<VqBf16, VQL_THRESHOLD> { typedef VqBf16 type; };
+// Rounded as it is kept.  A layer of fp16 keeps relu's p in fp16 too: what is above zero stays there.
+template <typename T, int KIND>
+__device__ __forceinline__ typename VqKept<T, KIND>::type vql_keep(float p, int act) {
+  if constexpr (__is_same(T, _Float16) && KIND == VQL_THRESHOLD) {
+    const float least = act == VQ_ACT_RELU ? 0x1p-24f : 0.0f;
+    p = p > 0.0f && p < least ? least : p;
+  }
+  return VqElem<typename VqKept<T, KIND>::type>::from(p);
+}
 __device__ __forceinline__ float vql_kept(float p, int) { return p; }
 __device__ __forceinline__ float vql_kept(_Float16 p, int) { return (float)p; }
 __device__ __forceinline__ float vql_kept(VqBf16 p, int act) {
@@ -466,7 +475,7 @@ __device__ __forceinline__ void vql_finish(const VqLinearArgs& a, const float* c
   for (int e = 0; e < E; ++e) p[e] = c[e] + bias[e];
   if (a.pre) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) kept.e[e] = VqElem<Kept>::from(p[e]);
+    for (int e = 0; e < E; ++e) kept.e[e] = vql_keep<T, KIND>(p[e], a.act);
     pre = __builtin_bit_cast(u32x4, kept);
   }
 #pragma unroll

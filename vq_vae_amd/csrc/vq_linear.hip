@@ -38,8 +38,8 @@ __device__ __forceinline__ void epilogue_one(const VqLinearArgs& a, int64_t i, i
   const int kind = vql_kind(a.act);
   if (a.pre) {
     typedef typename VqKept<T, VQL_SIGMOID>::type Kept;
-    if (kind == VQL_THRESHOLD) reinterpret_cast<T*>(a.pre)[i * a.J + j] = VqElem<T>::from(c);
-    else reinterpret_cast<Kept*>(a.pre)[i * a.J + j] = VqElem<Kept>::from(c);
+    if (kind == VQL_THRESHOLD) reinterpret_cast<T*>(a.pre)[i * a.J + j] = vql_keep<T, VQL_THRESHOLD>(c, a.act);
+    else reinterpret_cast<Kept*>(a.pre)[i * a.J + j] = vql_keep<T, VQL_SIGMOID>(c, a.act);
   }
   c = kind == VQL_THRESHOLD ? vql_act_of<VQL_THRESHOLD, sizeof(T) == 2>(c, a.act)
       : kind == VQL_SIGMOID ? vql_act_of<VQL_SIGMOID, sizeof(T) == 2>(c, a.act)
