@@ -612,3 +612,38 @@ def test_relu_slope_of_the_smallest_values(M, K, kind):
         w[:, 0] = sign * 2.0 ** -14
         (gx,) = torch.autograd.grad(vq.linear(x, w, activation="relu"), x, torch.ones(M, 72, device=DEV, dtype=kind))
         assert bool((gx[:, 0] == (72 * 2.0 ** -14 if sign > 0 else 0.0)).all()) and not bool(gx[:, 1:].any()), sign
+
+
+@pytest.mark.parametrize("kind, M", [(torch.float32, 2 ** 29 + 77), (torch.float16, 2 ** 29 + 77), (torch.bfloat16, 2 ** 31)],
+                         ids=["f32", "f16", "bf16"])
+def test_narrow_rows_to_two_to_the_31(kind, M):
+    # more tiles of 64 rows than 2^23, to the most rows there may be.  Rows at both ends and round every power of two between
+    K, N = 4, 3
+    w = torch.randn(N, K, device=DEV).to(kind)
+    b = torch.randn(N, device=DEV).to(kind)
+    x = torch.empty(M, K, device=DEV, dtype=kind)
+    for part in x.split(2 ** 26):
+        part.copy_(torch.randn(2 ** 16, K, device=DEV).repeat(2 ** 10, 1)[:len(part)])
+    rows = torch.tensor(sorted({0, 1, M - 1, M - 2, M - 78, *(2 ** k + d for k in range(20, 32) for d in (-1, 0, 1) if 2 ** k + d < M)}), device=DEV)
+    y = vq.linear(x, w, b, "relu")
+    want, _, _, ey, _ = forward64(x[rows], w, b, "relu", None)
+    close(y[rows], want, ey, "forward")
+    # every row, against the product of the 2^16 rows that a part repeats
+    for i in (0, 3, M - 1 >> 26):
+        part = x[i * 2 ** 26:(i + 1) * 2 ** 26]
+        one = vq.linear(part[:2 ** 16], w, b, "relu")
+        assert torch.equal(y[i * 2 ** 26:i * 2 ** 26 + len(part)], one.repeat(2 ** 10, 1)[:len(part)])
+    del y
+    # gradients: gy is one at those rows, zero elsewhere
+    gy = torch.zeros(M, N, device=DEV, dtype=kind)
+    gy[rows] = 1.0
+    xg, wg = x.requires_grad_(), w.requires_grad_()
+    gx, gw = torch.autograd.grad(vq.linear(xg, wg), [xg, wg], gy)
+    want = x.detach()[rows].double().sum(0).expand(N, K)
+    bound = 50 * U * x.detach()[rows].double().abs().sum(0).expand(N, K) + HALF[kind] * 1.01 * want.abs() + 1e-30
+    close(gw, want, bound, "weight gradient")
+    wsum = w.detach().double().sum(0)
+    bound = (N + 1) * U * w.detach().double().abs().sum(0) + HALF[kind] * 1.01 * wsum.abs() + TINY[kind]
+    close(gx[rows], wsum.expand(len(rows), K), bound.expand(len(rows), K), "input gradient")
+    gx[rows] = 0
+    assert not bool(gx.any())

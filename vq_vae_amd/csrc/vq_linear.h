@@ -849,7 +849,7 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void vql_product_kernel(VqLinearAr
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
 
-  const int tiles_i = (int)a.tiles_i, per_split = tiles_i * a.tiles_j, total = per_split * a.splits;   // below 2^23
+  const int tiles_i = (int)a.tiles_i, per_split = tiles_i * a.tiles_j, total = per_split * a.splits;   // at most MAX_BLOCKS
   const int steps = (int)((a.R + OA::BK - 1) / OA::BK), full = (int)(a.R / OA::BK);
   VQL_LDS char* lds = (VQL_LDS char*)vql_lds;
   OA oa;

@@ -359,6 +359,9 @@ bool bad_sizes(int64_t M, int K, int N) { return M < 0 || K <= 0 || N <= 0; }
 bool known(int dtype) { return dtype == VQ_F32 || dtype == VQ_BF16 || dtype == VQ_F16; }
 constexpr int MAX_DIM = 1 << 20;
 constexpr int64_t MAX_ROWS = (int64_t)1 << 31;
+// The product kernel counts its blocks in 32 bits, one round of workgroups beyond the last.  No output that fits the memory has as
+// many: 2^30 tiles of 64 x 64 from 64 columns on, and MAX_ROWS / 64 = 2^25 tiles for each 64 columns below.
+constexpr int64_t MAX_BLOCKS = (int64_t)1 << 30;
 bool pitch_too_wide(int64_t ld, size_t es) { return ld * (int64_t)es > 0x7fffffff / 256 - 128; }
 
 int product(const VqLinearArgs& a, int layout, int dtype, int config, bool dma, hipStream_t s) {
@@ -446,7 +449,7 @@ int run_product(int layout, VqLinearArgs a, int dtype, void* gbias, const float*
     a.part = reinterpret_cast<float*>(work);
   }
   if (p.rows) return by_type<RunRows>(dtype, a, s);
-  if (p.tiles_i * p.tiles_j * p.splits >= (int64_t)1 << 23) return VQ_ERR_UNSUPPORTED;
+  if (p.tiles_i * p.tiles_j * p.splits > MAX_BLOCKS) return VQ_ERR_UNSUPPORTED;
   if (!sums) a.gbias = gbias;
   if (gbias && !sums && p.splits > 1) a.asum = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + part_bytes(p));
   int rc = product(a, layout, dtype, p.config, dma, s);
