@@ -647,3 +647,69 @@ def test_narrow_rows_to_two_to_the_31(kind, M):
     close(gx[rows], wsum.expand(len(rows), K), bound.expand(len(rows), K), "input gradient")
     gx[rows] = 0
     assert not bool(gx.any())
+
+
+@pytest.mark.parametrize("M", [16, 3000])
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_tails_of_the_activations(act, kind, M):
+    """Relative to the value, so that a tail which is lost shows.  With s = 1 / (1 + exp(-v)), q = |v| and a 1-ulp exponential
+    and reciprocal (2 u each), v exact up to 4 u: 1 + exp and p s round twice, exp carries q times v's error and, as 2^(v log2 e), two
+    roundings of its own argument: (8 + 7 q) u.  v = p for silu, p (a + b p^2) for gelu_tanh.
+    Phi by erfc(z) = t exp(fit(t) - z^2), z = |p| / sqrt 2, t = 1 / (1 + z / 2): the fit 2 u; z 1.3 u, which moves erfc by 1 + 2 z^2 times
+    that; t 3 u, and 1.4 u more through the fit; nine steps of the fit 3 u; the exponent, at most z^2 + 1.3, rounded at the end and
+    twice as 2^(.. log2 e); the exponential 2 u; two products: (18 + 2.5 p^2) u, below 18 (1 + p^2 / 2) u.  Values that end below
+    2^-120 may be zero (an exponential that overflows, or whose reciprocal is subnormal).  p comes exactly: one input channel."""
+    p = torch.linspace(-13, 13, 15 * M, device=DEV).to(kind).view(15, M)
+    for row in p:
+        x = torch.zeros(M, 4, device=DEV, dtype=kind)
+        x[:, 1] = row
+        w = torch.zeros(24, 4, device=DEV, dtype=kind)
+        w[:, 1] = 1.0
+        got = vq.linear(x, w, None, act)
+        assert torch.equal(got, got[:, :1].expand(-1, 24))
+        v = row.double()
+        if act == "gelu":
+            want, each = v * 0.5 * torch.special.erfc(-v / math.sqrt(2)), 18 * (1 + v * v / 2)
+        else:
+            arg = v if act == "silu" else 2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)
+            want, each = v * torch.sigmoid(arg), 8 + 7 * arg.abs()
+        bound = (each * U + (HALF[kind] if kind is not torch.float32 else 0)) * 1.001 * want.abs() + 2.0 ** -120 + TINY[kind]
+        seen = (want.abs() > 2.0 ** -100) & (want.abs() > 4 * TINY[kind])
+        assert bool((bound < 0.5 * want.abs())[seen].all())      # zero would not pass
+        close(got[:, 0], want, bound, act)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_tails_of_the_slopes(act):
+    """The same for act'(p) below zero in fp32, where p is kept exactly; s = sigmoid(v) is off by (4 + d) u with v off by d / |v| u.
+    silu: s (1 + p (1 - s)), each factor's error and three roundings: 8 s (1 + 2 |p|) u.  gelu: p phi + Phi; phi's exponent p^2 / 2
+    is rounded once, and five more: (6 + p^2) |p| phi, Phi's as above, and the last rounding.  gelu_tanh: v rounded five times on
+    the way, s + p s (1 - s) v': (10 + 6 |v|) (s + |p| s (1 - s) v') and 1 - s, rounded beside s, 8 |p| v' s^2."""
+    p = -torch.linspace(0, 13, 4001, device=DEV)
+    x = torch.zeros(4001, 4, device=DEV)
+    x[:, 1] = p
+    x.requires_grad_()
+    w = torch.zeros(1, 4, device=DEV)
+    w[:, 1] = 1.0
+    (gx,) = torch.autograd.grad(vq.linear(x, w, activation=act), x, torch.ones(4001, 1, device=DEV))
+    v = p.double()
+    a = v.abs()
+    if act == "silu":
+        s = torch.sigmoid(v)
+        want, bound = s * (1 + v * torch.sigmoid(-v)), 8 * s * (1 + 2 * a)
+    elif act == "gelu":
+        phi, cdf = torch.exp(-v * v / 2) / math.sqrt(2 * math.pi), 0.5 * torch.special.erfc(-v / math.sqrt(2))
+        want = v * phi + cdf
+        bound = (6 + v * v) * a * phi + (18 + 9 * v * v) * cdf + want.abs()
+    else:
+        k = 2 * math.sqrt(2 / math.pi)
+        arg, d = k * (v + 0.044715 * v ** 3), k * (1 + 3 * 0.044715 * v * v)
+        s, o = torch.sigmoid(arg), torch.sigmoid(-arg)
+        want = s + v * s * o * d
+        bound = (10 + 6 * arg.abs()) * (s + a * s * o * d) + 8 * a * d * s * s
+    bound = bound * U * 1.001 + 2.0 ** -110
+    seen = (a > 3) & (want.abs() > 2.0 ** -90)
+    assert bool((bound < 0.5 * want.abs())[seen].all())
+    close(gx[:, 1], want, bound, act)
+    assert not bool(gx[:, [0, 2, 3]].any())

@@ -142,8 +142,8 @@ __device__ __forceinline__ void vql_store16_part(char* p, u32x4 v, int64_t valid
 }
 
 // -------------------------------------------------------------------------------- activations
-// erfc(z) for z >= 0: the Chebyshev fit of Numerical Recipes' erfcc (W. H. Press), relative error below 1.2e-7
-// everywhere, and a dozen instructions without a branch.
+// erfc(z) for z >= 0: the Chebyshev fit of Numerical Recipes' erfcc (W. H. Press), itself off by less than 1.2e-7 of the
+// value everywhere, and a dozen instructions without a branch.  Their roundings come on top (vql_cdf).
 __device__ __forceinline__ float vql_erfc_pos(float z) {
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.0f));
   float q = 0.17087277f;
@@ -159,14 +159,16 @@ __device__ __forceinline__ float vql_erfc_pos(float z) {
   return t * __expf(__builtin_fmaf(-z, z, q));
 }
 // FAST: 16-bit results. 1-ulp reciprocal and the hardware exponential, errors of some 1e-7 against a rounding of
-// 2^-9 or 2^-12; fp32 results take the library's functions and true divisions.
+// 2^-9 or 2^-12; the sigmoid and the normal density of fp32 results take the library's functions and true divisions.
 template <bool FAST>
 __device__ __forceinline__ float vql_sigmoid(float p) {
   if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __expf(-p));
   return 1.0f / (1.0f + expf(-p));
 }
-// Phi(p), for every type: the library's erfcf takes the branches of all its ranges in a wave with mixed arguments, and the fit
-// is off by 2^-23 of the value, times 1 + p^2 / 2 in the tails, where the exponent's own rounding shows
+// Phi(p), for every type, fp32 too: the library's erfcf takes the branches of all its ranges in a wave with mixed arguments.
+// p Phi(p) is off by up to 7.1 * 2^-24 (1 + p^2 / 2) of the value below zero and 7 * 2^-24 above (largest over 2e6 arguments in each
+// of nine ranges of -13 .. 8): 2 for the fit, the rest for the fit's own steps, its reciprocal and, in the tail, the exponent's
+// rounding.  0.5 (1 + erf) in fp32 is closer above zero and loses the tail below.
 __device__ __forceinline__ float vql_cdf(float p) {
   const float half = 0.5f * vql_erfc_pos(fabsf(p) * 0.70710678f);
   return p < 0.0f ? half : 1.0f - half;
