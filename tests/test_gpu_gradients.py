@@ -305,3 +305,18 @@ def test_max_norms_beyond_fp32():
     top = torch.full((1,), torch.finfo(torch.float32).max, device=DEV)
     vq.clip_grads([top], 1e39)
     assert float(top) == torch.finfo(torch.float32).max
+
+
+def test_gradients_that_have_a_graph():
+    # as torch's clip_grad_norm_: scaled in place, outside the graph, and known to it as changed
+    x = torch.linspace(1, 2, 50, device=DEV).requires_grad_()
+    y = x.detach().clone().requires_grad_()
+    for v in (x, y):
+        (v ** 3).sum().backward(create_graph=True)
+    norm = vq.clip_grad_norm_([x], 0.5, error_if_nonfinite=True)
+    want = torch.nn.utils.clip_grad_norm_([y], 0.5)
+    assert not norm.requires_grad and abs(float(norm) - float(want)) <= 2.0 ** -20 * float(want)
+    assert x.grad.grad_fn is not None and float((x.grad - y.grad).abs().max()) <= 2.0 ** -20 * float(y.grad.abs().max())
+    (x.grad ** 2).sum()
+    with torch.no_grad():
+        assert abs(float(vq.grad_norm([x.grad])) - 0.5) <= 1e-6

@@ -278,3 +278,22 @@ def test_traces_are_refused(products, requires_grad):
             return func(*args, **(kwargs or {}))
     with Passing():
         assert torch.allclose(vq.linear(*args[:3], residual=args[3]), formula(*args))
+
+
+def test_the_norm_is_not_part_of_a_graph():
+    # a penalty on it would contribute nothing: refused, not detached
+    x = torch.ones(3, requires_grad=True)
+    (g,) = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    for bad in ([g], [t(3), x]):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            vq.grad_norm(bad)
+        for fine in (torch.no_grad(), torch.inference_mode()):
+            with fine, pytest.raises(RuntimeError, match="GPU"):
+                vq.grad_norm(bad)
+        with pytest.raises(RuntimeError, match="GPU"):
+            vq.grad_norm([b.detach() for b in bad])
+    # torch's clipping takes such gradients, and so does this
+    x.grad = g
+    for error_if_nonfinite in (False, True):
+        with pytest.raises(RuntimeError, match="GPU"):
+            vq.clip_grad_norm_([x], 1.0, error_if_nonfinite=error_if_nonfinite)

@@ -104,11 +104,14 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
 
     grads: float32, bfloat16 and float16 tensors, mixed as they come, of any shape and strides, on one GPU.  norm_type: 1, 2
     or inf.  Summed in 64 bits.  NaN and infinity come through as the formula has them.  No tensor at all: 0 (on the
-    host).  The same bits on every run; may be captured in a graph."""
+    host).  The same bits on every run; may be captured in a graph.  Not differentiable: tensors that require a gradient (those
+    of ``create_graph=True`` do) are refused unless under ``torch.no_grad``."""
     kind = _kind(norm_type)
     grads = _list(grads, "grads")
     if _recording():
         _refuse_recording(grads, "grad_norm")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in grads):
+        raise RuntimeError("grad_norm is not differentiable, and a tensor requires a gradient: detach it, or call under torch.no_grad()")
     if not grads:
         return torch.zeros(())
     _require_cuda(grads[0], "grads")
@@ -131,7 +134,8 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     In place, or into ``out``: one tensor per gradient, of its shape and either its type or float32 (an optimizer's
     gradients beside 16-bit ones); ``grads`` are then only read.  Every result is rounded once.  An infinite norm scales by
     0 and a NaN by NaN, as the formula has it.  A tensor given twice, tensors that share memory, and expanded tensors to
-    be written are refused.  The same bits on every run; may be captured in a graph."""
+    be written are refused.  As under ``torch.no_grad``: neither the norm nor the scaling is part of a graph.  The same bits on
+    every run; may be captured in a graph."""
     kind = _kind(norm_type)
     max_norm = _max_norm(max_norm)
     grads = _list(grads, "grads")
@@ -210,14 +214,16 @@ def _dense_pairs(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor])
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_`` on :func:`clip_grads`: scales the ``grad`` of every parameter in place and returns
-    the norm they had.  Parameters without a gradient are passed over.  ``error_if_nonfinite`` raises RuntimeError, before
-    anything is scaled, if the norm is not finite (this is the one case that waits for the GPU)."""
+    the norm they had, both as under ``torch.no_grad``, like torch's.  Parameters without a gradient are passed over.
+    ``error_if_nonfinite`` raises RuntimeError, before anything is scaled, if the norm is not finite (this is the one case that
+    waits for the GPU)."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     _kind(norm_type)
     _max_norm(max_norm)
     if error_if_nonfinite and grads:
-        norm = grad_norm(grads, norm_type)
+        with torch.no_grad():
+            norm = grad_norm(grads, norm_type)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, "
                                "so it cannot be clipped.")
