@@ -320,3 +320,23 @@ def test_gradients_that_have_a_graph():
     (x.grad ** 2).sum()
     with torch.no_grad():
         assert abs(float(vq.grad_norm([x.grad])) - 0.5) <= 1e-6
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+def test_views_of_one_tensor_that_share_no_element(kind):
+    # the gradients of a fused projection's parts, in place, by other views of themselves, and into other columns
+    whole = torch.randn(300, 96, device=DEV).to(kind)
+    parts = lambda m: [m[:, :31], m[:, 31:64], m[10:, 64:90], m[:10, 64:90:2], m[:10, 65:90:2]]
+    for again in (False, True):
+        m = whole.clone()
+        grads = parts(m)
+        keep = [g.clone() for g in grads]
+        norm = vq.clip_grads(grads, 3.0, out=parts(m) if again else None)
+        want = norm64(keep)
+        assert abs(float(norm) - want) <= 2.0 ** -23 * want
+        clipped_ok(grads, keep, 3.0)
+        assert torch.equal(m[:, 90:], whole[:, 90:])
+    m = torch.cat([whole, torch.zeros_like(whole)], 1)
+    vq.clip_grads(parts(m), 3.0, out=parts(m[:, 96:]))
+    clipped_ok(parts(m[:, 96:]), parts(whole), 3.0)
+    assert torch.equal(m[:, :96], whole) and not bool(m[:, 186:].any())

@@ -297,3 +297,58 @@ def test_the_norm_is_not_part_of_a_graph():
     for error_if_nonfinite in (False, True):
         with pytest.raises(RuntimeError, match="GPU"):
             vq.clip_grad_norm_([x], 1.0, error_if_nonfinite=error_if_nonfinite)
+
+
+def test_clipping_takes_views_that_share_no_element():
+    a, c = t(6, 4), t(3, 8, 10)
+    fine = ([a[:, :2], a[:, 2:]], [a[:, 0], a[:, 1:3], a[:, 3]], [a[::2], a[1::2]], [a.view(-1)[::3], a.view(-1)[1::3], a.view(-1)[2::3]],
+            [c[:, :4, :5], c[:, 4:, :5], c[..., 5:]], [c[:, ::2, ::2], c[:, ::2, 1::2], c[:, 1::2]], [a.t()[:2], a.t()[2:]],
+            [a[:2, :2], a[2:], a[:2, 2:]], [t(4096, 30)[:, k::7] for k in range(7)])
+    for grads in fine:
+        with pytest.raises(RuntimeError, match="GPU"):
+            vq.clip_grads(grads, 1.0)
+        with pytest.raises(RuntimeError, match="GPU"):      # in place by another view of the same memory
+            vq.clip_grads(grads, 1.0, out=[g[...] for g in grads])
+    with pytest.raises(RuntimeError, match="GPU"):
+        vq.clip_grads([a[:, :2]], 1.0, out=[a[:, 2:]])
+    for bad in ([a[:, :2], a[:, 1:]], [a[::2], a[2:4, :1]], [c[:, :4, :5], c[2, 3:, 4:]], [a.view(-1)[::3], a.view(-1)[::2]]):
+        with pytest.raises(ValueError, match="share memory"):
+            vq.clip_grads(bad, 1.0)
+    with pytest.raises(ValueError, match="share memory"):
+        vq.clip_grads([a[:, :2]], 1.0, out=[a[:, 1:3]])
+    with pytest.raises(ValueError, match="share memory"):
+        vq.clip_grads([t(5, 8, dtype=BF)[:, :4]] + [a[:, :2]], 1.0, out=[a.view(-1)[:20].view(5, 4), a[:, 2:]])
+
+
+def test_shared_elements_are_found_exactly():
+    # against the bytes themselves, strided windows of one small buffer; a search that would take too long refuses
+    from vq_vae_amd import gradients
+    rng = np.random.default_rng(0)
+    buf = torch.zeros(400, dtype=torch.int8)
+
+    def window():
+        while True:
+            kind = (torch.float32, torch.bfloat16)[rng.integers(2)]
+            shape, stride = rng.integers(1, 6, rng.integers(0, 4)), rng.integers(0, 14, 3)
+            stride = stride[:len(shape)]
+            end = int(((shape - 1) * stride).sum()) + 1
+            room = buf.numel() // kind.itemsize - end
+            if room >= 0:
+                return torch.as_strided(buf.view(kind), tuple(map(int, shape)), tuple(map(int, stride)), int(rng.integers(0, room + 1)))
+
+    def bytes_of(v):
+        at = {0}
+        for n, st in zip(v.shape, v.stride()):
+            at = {p + k * st * v.element_size() for p in at for k in range(n)}
+        return {v.data_ptr() + p + k for p in at for k in range(v.element_size())}
+    seen = [0, 0]
+    for _ in range(3000):
+        a, b = window(), window()
+        want = bool(bytes_of(a) & bytes_of(b))
+        assert gradients._meet(gradients._runs(a), gradients._runs(b)) == want
+        assert gradients._shared([a, b]) == want
+        seen[want] += 1
+    assert min(seen) > 500
+    big = torch.zeros(1, dtype=torch.float32)
+    far = lambda first, dims: (first, first + 4 + sum(d * (n - 1) for d, n in dims), 4, dims)
+    assert gradients._meet(far(0, [(1000003 * 8, 4000), (1000033 * 8, 4000)]), far(4, [(999983 * 8, 4000), (999979 * 8, 4000)]))

@@ -84,18 +84,80 @@ def _refs(srcs: Sequence[torch.Tensor], dsts: Sequence[torch.Tensor]) -> array.a
     return array.array("q", words)
 
 
-def _spans(grads: Sequence[torch.Tensor], written: Sequence[torch.Tensor]) -> array.array:
-    """The memory of all tensors as such an array, each from its first to its last element (a tensor with gaps, like columns of
-    a matrix, counts whole), once where it is scaled in place."""
+def _same(g: torch.Tensor, o: torch.Tensor) -> bool:
+    """Whether o, of g's shape, is g's own memory in g's order: scaled in place."""
+    return g is o or (g.data_ptr() == o.data_ptr() and g.dtype is o.dtype and g.stride() == o.stride())
+
+
+def _spans(tensors: Sequence[torch.Tensor]) -> array.array:
+    """The memory of all tensors as such an array, each from its first to its last element (with the gaps between)."""
     words: List[int] = []
-    for t in (*written, *(g for g, o in zip(grads, written) if g is not o)):
+    for t in tensors:
         span = t.numel() and 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
         words += (t.data_ptr(), t.data_ptr(), span, _TWICE[t.dtype])
     return array.array("q", words)
 
 
-def _refuse_overlap(refs: array.array) -> None:
-    if _lib.load().vq_tensor_refs_overlap(refs.buffer_info()[0], len(refs) // 4):
+def _runs(t: torch.Tensor):
+    """t's memory as ``(first byte, byte behind the last, bytes of a run, ((distance, count) of the runs' repetitions, in bytes))``."""
+    size = run = t.element_size()
+    dims = sorted((st * size, n) for st, n in zip(t.stride(), t.shape) if n > 1 and st > 0)
+    while dims and dims[0][0] <= run:
+        distance, n = dims.pop(0)
+        run += distance * (n - 1)
+    return t.data_ptr(), t.data_ptr() + run + sum(distance * (n - 1) for distance, n in dims), run, dims
+
+
+#: steps that the search for a common element of two tensors may take: views of one tensor need one or two for each dimension
+_MEET_STEPS = 4096
+
+
+def _meet(a, b) -> bool:
+    """Whether two tensors, as `_runs` gives them, share a byte: whether a sum of distances, each taken as often as the places of
+    a's run and of b's run along it may differ, falls where the two runs touch.  True too where that takes too long to say."""
+    reach = {}
+    for dims, sign in ((a[3], 1), (b[3], -1)):
+        for distance, n in dims:
+            low, high = reach.get(distance, (0, 0))
+            reach[distance] = (low, high + n - 1) if sign > 0 else (low - n + 1, high)
+    levels = sorted(reach.items(), reverse=True)
+    rest = [(0, 0)]                       # least and largest sum of the levels behind each
+    for distance, (low, high) in reversed(levels):
+        rest.append((rest[-1][0] + distance * low, rest[-1][1] + distance * high))
+    rest.reverse()
+    apart = b[0] - a[0]
+    todo, steps = [(0, apart - a[2] + 1, apart + b[2] - 1)], 0
+    while todo:
+        level, least, most = todo.pop()
+        if not rest[level][0] <= most or not rest[level][1] >= least:
+            continue
+        if level == len(levels):
+            return True
+        distance, (low, high) = levels[level]
+        first = max(low, -((rest[level + 1][1] - least) // distance))
+        last = min(high, (most - rest[level + 1][0]) // distance)
+        steps += max(0, last - first + 1)
+        if steps > _MEET_STEPS:
+            return True
+        todo += [(level + 1, least - k * distance, most - k * distance) for k in range(first, last + 1)]
+    return False
+
+
+def _shared(tensors: Sequence[torch.Tensor]) -> bool:
+    """Whether any two tensors share memory, gaps not counted (the columns of a matrix in several tensors do not)."""
+    runs = sorted(_runs(t) for t in tensors if t.numel())
+    for i, a in enumerate(runs):
+        for b in runs[i + 1:]:
+            if b[0] >= a[1]:
+                break
+            if _meet(a, b):
+                return True
+    return False
+
+
+def _refuse_overlap(refs: array.array, strided: Optional[Sequence[torch.Tensor]] = None) -> None:
+    """refs: dense tensors, or the spans of `strided` ones, which are looked at closer where those overlap."""
+    if _lib.load().vq_tensor_refs_overlap(refs.buffer_info()[0], len(refs) // 4) and (strided is None or _shared(strided)):
         raise ValueError("gradients that are to be scaled share memory: each may be given once")
 
 
@@ -133,8 +195,8 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
 
     In place, or into ``out``: one tensor per gradient, of its shape and either its type or float32 (an optimizer's
     gradients beside 16-bit ones); ``grads`` are then only read.  Every result is rounded once.  An infinite norm scales by
-    0 and a NaN by NaN, as the formula has it.  A tensor given twice, tensors that share memory, and expanded tensors to
-    be written are refused.  As under ``torch.no_grad``: neither the norm nor the scaling is part of a graph.  The same bits on
+    0 and a NaN by NaN, as the formula has it.  A tensor given twice, tensors that share elements, and expanded tensors to
+    be written are refused (views of one tensor that share none, as the columns of a matrix in two halves, are fine).  As under ``torch.no_grad``: neither the norm nor the scaling is part of a graph.  The same bits on
     every run; may be captured in a graph."""
     kind = _kind(norm_type)
     max_norm = _max_norm(max_norm)
@@ -167,7 +229,8 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         refs = _refs(grads, written)
         _refuse_overlap(refs)
     else:
-        _refuse_overlap(_spans(grads, written))
+        strided = [*written, *(g for g, o in zip(grads, written) if not _same(g, o))]
+        _refuse_overlap(_spans(strided), strided)
     _require_cuda(grads[0], "grads")
     device = grads[0].device
     with _on_device(device):
