@@ -713,3 +713,17 @@ def test_tails_of_the_slopes(act):
     assert bool((bound < 0.5 * want.abs())[seen].all())
     close(gx[:, 1], want, bound, act)
     assert not bool(gx[:, [0, 2, 3]].any())
+
+
+@pytest.mark.parametrize("M", [5, 100])
+@pytest.mark.parametrize("kind", TYPES, ids=["f32", "bf16", "f16"])
+def test_what_is_kept_for_the_activation(kind, M):
+    # fp32, or one rounding to fp16 (half a step 2^-11, 2^-25 near zero) of the product's and the bias's fp32 sum
+    from vq_vae_amd import projection
+    x, w, b, _, _ = make(M, 96, 130, kind, True, False, False, 31)
+    for act in ("silu", "gelu", "gelu_tanh"):
+        _, p, _, _, ep = forward64(x, w, b, act, None)
+        _, pre = projection.linear_forward(x, w, b, act, want_pre=True)
+        assert pre.dtype is (torch.float32 if kind is torch.float32 else torch.float16)
+        h, tiny = (0.0, 0.0) if kind is torch.float32 else (2.0 ** -11, 2.0 ** -25)
+        close(pre, p, 1.001 * (ep + h * p.abs()) + tiny, act)
