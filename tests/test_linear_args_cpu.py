@@ -352,3 +352,14 @@ def test_shared_elements_are_found_exactly():
     big = torch.zeros(1, dtype=torch.float32)
     far = lambda first, dims: (first, first + 4 + sum(d * (n - 1) for d, n in dims), 4, dims)
     assert gradients._meet(far(0, [(1000003 * 8, 4000), (1000033 * 8, 4000)]), far(4, [(999983 * 8, 4000), (999979 * 8, 4000)]))
+
+
+def test_layer_under_autocast(products):
+    # the types stay: nothing is cast, and an input of another type than the parameters' is refused
+    layer, x = vq.Linear(3, 4), torch.randn(7, 3)
+    with torch.autocast("cpu", dtype=BF):
+        assert torch.nn.Linear(3, 4)(x.to(BF)).dtype is BF
+        with pytest.raises(TypeError, match="share one type"):
+            layer(x.to(BF))
+        y = layer(x)
+    assert y.dtype is F32 and torch.equal(y, layer(x))

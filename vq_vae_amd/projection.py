@@ -214,7 +214,7 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     fp16 (bf16 layers too, but for relu), and the backward rounds the gradient behind the activation to it before the two products (the bias
     gradient is summed before that rounding).
     Forward-mode derivatives, transforms of ``torch.func`` and traces (``torch.jit.trace``, ``make_fx``) are refused.
-    Under autocast the tensors keep their types.  May be captured in a graph, backward included (drop every eager autograd
+    Under autocast the tensors keep their types, and all have to share one there too.  May be captured in a graph, backward included (drop every eager autograd
     graph over the same leaves before capturing, as torch asks for any backward under capture)."""
     if _recording():
         _refuse_recording((input, weight, bias, residual), "linear")
@@ -227,7 +227,10 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
 class Linear(nn.Linear):
     """``nn.Linear`` (same parameters, initialisation and state dict) on :func:`linear`, with the activation and an optional
-    residual in the same kernel: ``layer(x, residual)`` is ``act(x W^T + b) + residual``."""
+    residual in the same kernel: ``layer(x, residual)`` is ``act(x W^T + b) + residual``.
+
+    Autocast does not reach it: with fp32 parameters it refuses the 16-bit input that ``nn.Linear`` would take there.  Put the
+    layer itself into the type it computes in (``layer.to(torch.bfloat16)``), or cast its input."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str = "none", device=None,
                  dtype=None):
