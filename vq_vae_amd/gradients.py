@@ -172,7 +172,7 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
     grads = _list(grads, "grads")
     if _recording():
         _refuse_recording(grads, "grad_norm")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in grads):
+    if torch.is_grad_enabled() and True in [t.requires_grad for t in grads]:
         raise RuntimeError("grad_norm is not differentiable, and a tensor requires a gradient: detach it, or call under torch.no_grad()")
     if not grads:
         return torch.zeros(())

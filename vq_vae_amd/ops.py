@@ -40,15 +40,18 @@ def _raw_stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+_is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+
+
 def _recording() -> bool:
     """Whether torch may be recording a call's tensor operations besides running them: forward-mode differentiation, a trace, a
     dispatch mode.  None of them sees a kernel launch, and what they record without it is wrong."""
-    return _forward_ad._current_level >= 0 or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack() > 0
+    return _forward_ad._current_level >= 0 or _is_tracing() or _dispatch_modes() > 0
 
 
 def _refuse_recording(tensors, what: str) -> None:
     """Refuses a trace and a tangent; a dual level without one and other dispatch modes are fine."""
-    if torch._C._is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    if _is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         raise NotImplementedError(f"{what} cannot be traced: its kernels are no torch operations")
     if _forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
