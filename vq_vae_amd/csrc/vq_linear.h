@@ -168,7 +168,7 @@ __device__ __forceinline__ float vql_sigmoid(float p) {
 // Phi(p), for every type, fp32 too: the library's erfcf takes the branches of all its ranges in a wave with mixed arguments.
 // p Phi(p) is off by up to 7.1 * 2^-24 (1 + p^2 / 2) of the value below zero and 7 * 2^-24 above (largest over 2e6 arguments in each
 // of nine ranges of -13 .. 8): 2 for the fit, the rest for the fit's own steps, its reciprocal and, in the tail, the exponent's
-// rounding.  0.5 (1 + erf) in fp32 is closer above zero and loses the tail below.
+// rounding.  (0.5 (1 + erf) in fp32 would lose the tail altogether.)
 __device__ __forceinline__ float vql_cdf(float p) {
   const float half = 0.5f * vql_erfc_pos(fabsf(p) * 0.70710678f);
   return p < 0.0f ? half : 1.0f - half;

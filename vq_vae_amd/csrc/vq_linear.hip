@@ -12,7 +12,8 @@ namespace {
 // sum; a wave reads W straight into the fragments of a 16x16 product (lane l: channel l % 16, 16 bytes at piece l / 16
 // of a 64-byte step, so consecutive steps of one channel are consecutive lines), eight steps in flight, with x, which
 // stays in the L2, in the other operand.  The waves' partial products are added in LDS in wave order.  8 rows, 4096 -> 4096 bf16:
-// 8.6 us with W in the caches, 9.9 without (an empty launch takes 2.6, the 34 MB 5.3 at 6.3 TB/s); 1 row, 256 -> 1024: 2.7.
+// 8.6 us with W in the caches, 9.9 without (an empty launch takes 2.6, the 34 MB 5.3 at 6.3 TB/s), with gelu and a residual 10.2;
+// 1 row, 256 -> 1024: 2.7, with bias and silu 3.5.
 // W past the caches gains nothing: 10.1, and 9.4 instead of 9.1 where 100 MB of weights take turns.
 constexpr int ROWS_MAX = 16;
 constexpr int ROWS_UNROLL = 8;
