@@ -334,7 +334,7 @@ int vq_conv1x1_wgrad(const float* gy, const float* x, int layout, int64_t N, int
  *
  * vq_linear:          p = x W^T + bias;  y = act(p) + residual;  pre (NULL: not wanted) = p for the activation's
  *                     gradient: fp32 for VQ_F32, fp16 for VQ_F16, and for VQ_BF16 fp16 too (bf16 where act is
- *                     VQ_ACT_NONE or VQ_ACT_RELU).
+ *                     VQ_ACT_NONE or VQ_ACT_RELU).  For VQ_ACT_RELU what is above zero is kept above zero.
  * vq_linear_act_grad: dp = gy * act'(pre) for `count` elements, act other than VQ_ACT_NONE, pre as vq_linear wrote it.
  *                     May run in place.
  * vq_linear_dgrad:    gx = dp W.

@@ -340,3 +340,11 @@ def test_views_of_one_tensor_that_share_no_element(kind):
     vq.clip_grads(parts(m), 3.0, out=parts(m[:, 96:]))
     clipped_ok(parts(m[:, 96:]), parts(whole), 3.0)
     assert torch.equal(m[:, :96], whole) and not bool(m[:, 186:].any())
+
+
+def test_lists_without_an_element():
+    for grads in ([torch.zeros(0, device=DEV)], [torch.zeros(3, 0, device=DEV, dtype=t) for t in TYPES] * 60):
+        for p in (1.0, 2.0, math.inf):
+            assert float(vq.grad_norm(grads, p)) == 0.0
+            assert float(vq.clip_grads(grads, 1.0, p)) == 0.0
+            assert float(vq.clip_grads(grads, 0.0, p, out=[torch.empty_like(g, dtype=torch.float32) for g in grads])) == 0.0

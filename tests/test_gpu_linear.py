@@ -727,3 +727,32 @@ def test_what_is_kept_for_the_activation(kind, M):
         assert pre.dtype is (torch.float32 if kind is torch.float32 else torch.float16)
         h, tiny = (0.0, 0.0) if kind is torch.float32 else (2.0 ** -11, 2.0 ** -25)
         close(pre, p, 1.001 * (ep + h * p.abs()) + tiny, act)
+
+
+@pytest.mark.parametrize("M, K, N", [(1, 2 ** 20, 3), (40, 2 ** 20, 3), (3, 2, 2 ** 20), (33, 2, 2 ** 20)])
+def test_the_most_features(M, K, N):
+    x, w, b, r, gy = make(M, K, N, torch.bfloat16, True, True, False, 12)
+    y, p, slope, ey, ep = forward64(x, w, b, "relu", r)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    out = vq.linear(*leaves, "relu", r)
+    close(out.detach(), y, ey, "forward")
+    grads = torch.autograd.grad(out, leaves, gy)
+    for g, (want, bound), what in zip(grads, backward64(gy, x.detach(), w.detach(), p, ep, slope, "relu"), ("input", "weight", "bias")):
+        close(g, want, bound, what)
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_rows_far_apart_and_odd_vectors(M):
+    # rows further apart than the kernels address are copied first; a bias with gaps and an expanded one too
+    K, N = 40, 24
+    wide = torch.randn(M, 2 ** 22 + 64, device=DEV).half()
+    x, r = wide[:, 5:5 + K], wide[:, 2 ** 22:2 ** 22 + N]
+    w = torch.randn(N, 2 ** 22 + 64, device=DEV).half()[:, 3:3 + K]
+    for b in (torch.randn(N, 3, device=DEV).half()[:, 1], torch.randn(1, device=DEV).half().expand(N)):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w, b, r)]
+        views = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        results = []
+        for tensors in (leaves, views):
+            y = vq.linear(*tensors[:3], "silu", tensors[3])
+            results.append([y.detach(), *torch.autograd.grad(y, tensors, torch.ones(M, N, device=DEV, dtype=torch.half))])
+        assert all(torch.equal(a, c) for a, c in zip(*results))

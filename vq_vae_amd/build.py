@@ -27,7 +27,8 @@ HEADERS = [os.path.join(CSRC, "vq_common.h"), os.path.join(CSRC, "vq_linear.h"),
 # or the distances would stop matching the documented rounding.
 FLAGS = ["-O3", "--offload-arch=gfx950", "-ffp-contract=off", "-fPIC", "-std=c++17", "-Wall",
          "-Wno-unused-function", "-fno-gpu-rdc",
-         # no packed fp32 instructions, which -O3 makes of pairs of ordinary float operations: a precaution, nothing here was tested with them
+         # no packed fp32 instructions, which -O3 makes of pairs of ordinary float operations: a precaution, nothing here was
+         # tested with them
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

@@ -158,7 +158,7 @@ def _shared(tensors: Sequence[torch.Tensor]) -> bool:
 def _refuse_overlap(refs: array.array, strided: Optional[Sequence[torch.Tensor]] = None) -> None:
     """refs: dense tensors, or the spans of `strided` ones, which are looked at closer where those overlap."""
     if _lib.load().vq_tensor_refs_overlap(refs.buffer_info()[0], len(refs) // 4) and (strided is None or _shared(strided)):
-        raise ValueError("gradients that are to be scaled share memory: each may be given once")
+        raise ValueError("gradients that are to be scaled share memory: each element may be given once")
 
 
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
@@ -196,8 +196,9 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     In place, or into ``out``: one tensor per gradient, of its shape and either its type or float32 (an optimizer's
     gradients beside 16-bit ones); ``grads`` are then only read.  Every result is rounded once.  An infinite norm scales by
     0 and a NaN by NaN, as the formula has it.  A tensor given twice, tensors that share elements, and expanded tensors to
-    be written are refused (views of one tensor that share none, as the columns of a matrix in two halves, are fine).  As under ``torch.no_grad``: neither the norm nor the scaling is part of a graph.  The same bits on
-    every run; may be captured in a graph."""
+    be written are refused (views of one tensor that share none, as the columns of a matrix in two halves, are fine).  As under
+    ``torch.no_grad``: neither the norm nor the scaling is part of a graph of autograd.  The same bits on every run; may be
+    captured in a graph."""
     kind = _kind(norm_type)
     max_norm = _max_norm(max_norm)
     grads = _list(grads, "grads")

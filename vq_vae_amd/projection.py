@@ -214,8 +214,9 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     fp16 (bf16 layers too, but for relu), and the backward rounds the gradient behind the activation to it before the two products (the bias
     gradient is summed before that rounding).
     Forward-mode derivatives, transforms of ``torch.func`` and traces (``torch.jit.trace``, ``make_fx``) are refused.
-    Under autocast the tensors keep their types, and all have to share one there too.  May be captured in a graph, backward included (drop every eager autograd
-    graph over the same leaves before capturing, as torch asks for any backward under capture)."""
+    Under autocast the tensors keep their types, and all have to share one there too.  May be captured in a graph, backward
+    included (drop every eager autograd graph over the same leaves before capturing, as torch asks for any backward under
+    capture)."""
     if _recording():
         _refuse_recording((input, weight, bias, residual), "linear")
     _check(input, weight, bias, activation, residual)
